@@ -44,6 +44,7 @@ extern "C" {
 #define DUPLEX_DEVERR_TIMEOUT 2   /* a bounded pipeline wait gave up */
 #define DUPLEX_DEVERR_NONFINITE 4 /* duplex_stack_forward: a partial layer output was NaN or
                                      beyond +-2^26 and was clamped (its fixed-point sum) */
+#define DUPLEX_DEVERR_BLOCK 8     /* a KV cache's block id outside [0, n_blocks): its tokens were left out */
 /* duplex_stack_forward also records, from this bit up, which of its waits gave up
  * first: 1 ring slot free, 2 routing plan, 3 ring slot filled, 4 grid barrier,
  * 5 drain, 6 cluster exchange. */
@@ -481,6 +482,94 @@ int duplex_moe_forward_noalloc(const void* x, int act_dtype, int32_t T, const vo
                                int32_t group, const void* residual, void* out, float* w_out,
                                int32_t* sel_out, int32_t* err, float rms_eps, int pdl,
                                void* stream);
+
+/*
+ * The 8-bit paged KV cache -- no counterpart in the reference, whose decode runs
+ * transformers' attention over 16-bit caches (src/duplex/streaming/clock.py:155-156).
+ * What a decoder layer runs between its q|k|v and its o projection.
+ *
+ * codes  k, v [n_blocks][kv_heads][block][dim], one byte each (DUPLEX_KV_*), 16-byte aligned
+ * scales k_scale, v_scale [n_blocks][kv_heads] fp32 >= 0: value = code * scale.  The entry
+ *        points write powers of two: 2^e, the least e >= -126 with max|value| <= top * 2^e
+ *        (top 448 for e4m3, 127 for int8).
+ * weights [n_blocks][kv_heads][block] fp32, the tokens' accumulated attention weights, or NULL.
+ * dim 64 or 128; block 16, 32, 64 or 128 tokens.
+ *
+ * A call's batch: block_table [batch][width] (a sequence's blocks in order; entries past its
+ * last token are not read), kv_len [batch] (its tokens, the call's own rows included: row t of
+ * T is token kv_len - T + t), cu_rows [batch + 1] (its rows are [cu_rows[b], cu_rows[b+1]) of
+ * n_rows; NULL: n_rows / batch each).  All are device memory, read by the kernels: a captured
+ * call follows their values.  Rows behind the last sequence's are left alone; lengths and rows
+ * are held inside width * block and n_rows; a block id out of range is reported in err
+ * (DUPLEX_DEVERR_BLOCK) and its tokens are left out.  batch <= DUPLEX_KV_MAX_BATCH,
+ * batch * kv_heads <= 65535.
+ */
+#define DUPLEX_KV_E4M3 0
+#define DUPLEX_KV_INT8 1
+#define DUPLEX_KV_MAX_BATCH 4096
+
+typedef struct duplex_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  float* weights;
+  int32_t n_blocks, kv_heads, block, dim;
+  int32_t format;
+} duplex_kv_cache;
+
+typedef struct duplex_kv_batch {
+  const int32_t* block_table;
+  const int32_t* kv_len;
+  const int32_t* cu_rows;
+  int32_t width, batch, n_rows;
+} duplex_kv_batch;
+
+/*
+ * kv_append -- the call's rows become tokens [kv_len - T, kv_len) of their sequences.
+ * k_new, v_new: element (row, head, d) at row * row_stride + head * head_stride + d (fp16 or
+ * bf16, strides in elements and multiples of 8).  A block's scale is set by its new tokens and,
+ * where it already holds older ones of the sequence, never falls: their codes are rounded anew
+ * when it rises.  A new token's weight becomes 0.  A value that is not finite is stored as 0 and
+ * reported (DUPLEX_DEVERR_NONFINITE).  Rows before slot 0 (T > kv_len) are not stored.  No block
+ * may take new tokens of two sequences in one call.
+ */
+int duplex_kv_append(const duplex_kv_cache* cache, const duplex_kv_batch* batch, const void* k_new,
+                     const void* v_new, int act_dtype, int64_t k_row_stride, int64_t k_head_stride,
+                     int64_t v_row_stride, int64_t v_head_stride, int32_t* err, void* stream);
+
+/*
+ * kv_attend -- causal attention of the call's rows over the cache.  The row at position p sees
+ * the tokens j <= p with window == 0, j > p - window, or j < sinks.  q: (row, head, d) strided as
+ * above; heads is a multiple of kv_heads, query head i reads KV head i / (heads / kv_heads).
+ * out [n_rows][heads][dim] in q's type, lse [n_rows][heads] fp32 or NULL: the natural logarithm
+ * of the sum of exp(q.k * softmax_scale).  A row that sees nothing gets 0 and -inf.  With
+ * cache->weights, each seen token's weight grows by the sum over the call's rows and the
+ * group's heads of exp(q.k * softmax_scale - lse).  Blocks that no row sees are not read.
+ */
+int duplex_kv_attend_workspace_bytes(const duplex_kv_cache* cache, const duplex_kv_batch* batch,
+                                     int32_t heads, size_t* bytes);
+int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_batch* batch, const void* q,
+                     int act_dtype, int32_t heads, int64_t q_row_stride, int64_t q_head_stride,
+                     float softmax_scale, int32_t window, int32_t sinks, void* out, float* lse,
+                     void* workspace, size_t workspace_bytes, int32_t* err, void* stream);
+
+/*
+ * kv_evict -- keep at most `keep` tokens of each sequence and KV head: the first `sinks`, the
+ * last `recent`, and of the rest those with the largest cache->weights (ties: the earlier token;
+ * NaN counts as the largest), in their order.  They are written to the blocks of dst_table
+ * [batch][dst_width] (dst_width * block >= keep), with their weights and with scales of their
+ * own; a sequence of no more than keep tokens is copied whole.  new_len [batch] = min(kv_len,
+ * keep).  The source blocks are left as they are, so they may be shared between sequences; no
+ * destination block may be a source block of the call or appear twice.  keep >= sinks + recent.
+ * cu_rows and n_rows are not used.
+ */
+int duplex_kv_evict_workspace_bytes(const duplex_kv_cache* cache, const duplex_kv_batch* batch,
+                                    int32_t keep, size_t* bytes);
+int duplex_kv_evict(const duplex_kv_cache* cache, const duplex_kv_batch* batch,
+                    const int32_t* dst_table, int32_t dst_width, int32_t keep, int32_t sinks,
+                    int32_t recent, int32_t* new_len, void* workspace, size_t workspace_bytes,
+                    int32_t* err, void* stream);
 
 #ifdef __cplusplus
 }

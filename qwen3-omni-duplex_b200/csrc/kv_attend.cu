@@ -1,0 +1,708 @@
+// Attention over the 8-bit paged KV cache for few query rows a sequence: decode, drafted tokens,
+// short chunks (kv_prompt.cu takes long ones).
+//
+//   s_j = q . k_j * softmax_scale,  out = sum_j exp(s_j - lse) v_j,  lse = log sum_j exp(s_j)
+//
+// over the tokens that a row sees: j <= p, and inside the window (j > p - window) or a sink
+// (j < sinks).  One pass over the cache with a running maximum.
+//
+// Bound by the cache's bytes: 2 dim + a little per token and KV head, read once for all query
+// heads that share it.  A warp takes 16 tokens at a time, straight from global memory into the
+// registers that mma.sync takes (keys as A[token][dim], values transposed as A[dim][token]; the
+// query rows are the 8 columns, so 8 query heads of a group use every product), with the next 16
+// tokens' loads in flight.  No shared memory on that path: a warp's loads are whole 128-byte rows
+// (keys: halves of them), and the bytes are converted to fp16 in registers, exactly.
+//
+// The work of a launch is one list of 64-token units over (sequence, KV head, row tile); every CTA
+// takes an equal, contiguous piece of it, whatever the lengths, and reads the lengths itself (a
+// captured launch follows them).  Pieces that share a row tile leave partial results, which
+// kv_combine_kernel joins in order: no atomics, the same bits on each run.
+#include <algorithm>
+
+#include "kv.cuh"
+
+namespace duplex {
+
+constexpr int kWarps = 4;
+constexpr int kUnit = 16 * kWarps;   // tokens
+constexpr int kMaxCtas = 148 * 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// p = exp2(s - m + kShift) is what fp16 holds: the reference m may be 2^kSlack behind the true
+// maximum (so it rarely moves), p stays below 2^15, and a p of 2^-21 of the reference is still normal.
+constexpr float kShift = 7.f, kSlack = 8.f;
+
+struct AttendParams {
+  KvView c;
+  const void* q;
+  int64_t q_row, q_head;  // elements
+  int act, heads, group;
+  int window, sinks;
+  float scale_log2;       // softmax_scale * log2(e)
+  void* out;              // [n_rows][heads][dim]
+  float* lse;             // [n_rows][heads] or null
+  float* part;            // partial results, 2 slots per CTA
+  int32_t* err;
+};
+
+// The unit list of a launch: off[b] units before sequence b.  A row tile of sequence b has units(b)
+// units, the most that any of its row tiles needs.
+struct Plan {
+  int64_t total, share;
+};
+
+DEVI int tiles_of(const KvSeq& s, int group, int rows) { return (int)(((int64_t)s.rows * group + rows - 1) / rows); }
+
+DEVI int units_of(const KvSeq& s, const AttendParams& p, int rows) {
+  const int all = max((s.n + kUnit - 1) / kUnit, 1);
+  if (!p.window) return all;
+  // a row tile's window reaches over window - 1 + (its own tokens), whose ends need not be aligned
+  const int64_t span = (int64_t)p.window + (rows - 1) / p.group + 1;
+  const int64_t u = (min(p.sinks, s.n) + kUnit - 1) / kUnit + (span + kUnit - 1) / kUnit + 1;
+  return (int)min(u, (int64_t)all);
+}
+
+template <int ROWS>
+DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
+  __shared__ int64_t warp_sum[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = p.c.batch;
+  int64_t base = 0;
+  for (int b0 = 0; b0 < B; b0 += kWarps * 32) {
+    const int b = b0 + tid;
+    int64_t u = 0;
+    if (b < B) {
+      const KvSeq s = kv_seq(p.c, b);
+      u = (int64_t)p.c.heads * tiles_of(s, p.group, ROWS) * units_of(s, p, ROWS);
+    }
+    int64_t incl = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int64_t before = base, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (b < B) off[b] = before + incl - u;
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) off[B] = base;
+  __syncthreads();
+  Plan pl;
+  pl.total = base;
+  pl.share = (base + ctas - 1) / ctas;
+  if (pl.share < 1) pl.share = 1;
+  return pl;
+}
+
+// the sequence of unit u: the last b with off[b] <= u (sequences without units are passed over)
+DEVI int seq_of(const int64_t* off, int B, int64_t u) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (off[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+DEVI uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+DEVI float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// fp16 query fragments of 8 rows: row r's 16 dims at 64 cc + 16 t, scaled by a power of two that
+// brings the row's largest into [2^14, 2^15): bf16's 8 bits fit fp16's 11, and only values below
+// 2^-28 of the row's largest lose bits.  Returns the factor that undoes it.
+template <int D>
+DEVI float load_q(const AttendParams& p, int64_t row, int head, int t, bool live, uint2 (&qf)[D / 16]) {
+  uint4 raw[D / 64][2];
+  const uint8_t* src = static_cast<const uint8_t*>(p.q) + 2 * (row * p.q_row + head * p.q_head);
+  float amax = 0.f;
+#pragma unroll
+  for (int cc = 0; cc < D / 64; ++cc)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      raw[cc][j] = live ? __ldg(reinterpret_cast<const uint4*>(src + 2 * (64 * cc + 16 * t + 8 * j))) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = (&raw[cc][j].x)[i];
+        const float2 f = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(w) : act2<DUPLEX_DTYPE_BF16>(w);
+        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+    }
+  amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+  const int ex = (int)(__float_as_uint(amax) >> 23) - 127;
+  const int up = (amax == 0.f || ex == 128) ? 0 : min(14 - ex, 126);
+  const float f = pow2f(up);
+#pragma unroll
+  for (int cc = 0; cc < D / 64; ++cc)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t w0 = (&raw[cc][s >> 1].x)[(s & 1) * 2], w1 = (&raw[cc][s >> 1].x)[(s & 1) * 2 + 1];
+      const float2 a = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(w0) : act2<DUPLEX_DTYPE_BF16>(w0);
+      const float2 b = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(w1) : act2<DUPLEX_DTYPE_BF16>(w1);
+      qf[cc * 4 + s] = make_uint2(f2h(a.x * f, a.y * f), f2h(b.x * f, b.y * f));
+    }
+  return pow2f(-up);
+}
+
+// S[nt] += K (16 tokens) . Q (8 rows), both as fragments
+template <int D, int FMT, int NT>
+DEVI void qk(const uint4 (&kr)[2][D / 64], const uint2 (&qf)[NT][D / 16], float (&S)[NT][4]) {
+#pragma unroll
+  for (int cc = 0; cc < D / 64; ++cc)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t w0 = (&kr[0][cc].x)[s], w1 = (&kr[1][cc].x)[s];
+      const uint32_t a0 = KvFmt<FMT>::lo(w0), a1 = KvFmt<FMT>::lo(w1), a2 = KvFmt<FMT>::hi(w0), a3 = KvFmt<FMT>::hi(w1);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(S[nt], a0, a1, a2, a3, qf[nt][cc * 4 + s].x, qf[nt][cc * 4 + s].y);
+    }
+}
+
+// the tokens of one row tile: [0, sink_end) and [lo, end), in units
+struct Span {
+  int sink_units, lo, end, sink_end;  // lo aligned to a unit
+};
+
+DEVI Span span_of(const AttendParams& p, int first_pos, int last_pos, int n) {
+  Span s;
+  s.end = min(last_pos + 1, n);
+  s.lo = 0;
+  s.sink_units = 0;
+  s.sink_end = 0;
+  if (p.window) {
+    const int64_t w = (int64_t)first_pos - p.window + 1;
+    s.lo = w > 0 ? (int)(w / kUnit) * kUnit : 0;
+    s.sink_end = min(p.sinks, s.end);
+    s.sink_units = (s.sink_end + kUnit - 1) / kUnit;
+    if (s.sink_units * kUnit >= s.lo) s.lo = s.sink_units = s.sink_end = 0;
+  }
+  return s;
+}
+
+template <int D, int NT>
+constexpr int part_floats() { return 8 * NT * (D + 2); }  // O [rows][D], m [rows], l [rows]
+
+template <int D, int FMT, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel(AttendParams p) {
+  constexpr int ROWS = 8 * NT, VW = D / 32, LD = D + 4;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  float(*sO)[LD] = reinterpret_cast<float(*)[LD]>(dyn);  // [kWarps * ROWS]
+  int64_t* off = reinterpret_cast<int64_t*>(dyn + sizeof(float) * kWarps * ROWS * LD);
+  __shared__ float sm[kWarps][ROWS], sl[kWarps][ROWS];
+  const KvView& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  pdl_launch_dependents();
+  const Plan plan = make_plan<ROWS>(p, off, gridDim.x);
+  int64_t u = (int64_t)blockIdx.x * plan.share;
+  const int64_t u_end = min(u + plan.share, plan.total);
+  if (u >= u_end) return;
+  int b = seq_of(off, c.batch, u);
+  const int64_t u_begin = u;
+
+  while (u < u_end) {
+    while (off[b + 1] <= u) ++b;
+    const KvSeq s = kv_seq(c, b);
+    const int rt_all = tiles_of(s, p.group, ROWS), per = units_of(s, p, ROWS);
+    const int64_t r = u - off[b];
+    const int it = (int)(r / per), i0 = (int)(r - (int64_t)it * per);
+    const int i1 = (int)min((int64_t)per, i0 + (u_end - u));
+    const int h = it / rt_all, rt = it - h * rt_all;
+    const int row_base = rt * ROWS, row_all = s.rows * p.group;
+    const int first_pos = s.n - s.rows + row_base / p.group;
+    const int last_row = min(row_base + ROWS, row_all) - 1;
+    const int last_pos = s.n - s.rows + last_row / p.group;
+    const Span sp = span_of(p, first_pos, last_pos, s.n);
+
+    // query rows: as the product's columns, lane (g, t) loads row g and accumulates rows 2t, 2t + 1
+    uint2 qf[NT][D / 16];
+    float csc[NT][2];
+    int pos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int rr = row_base + nt * 8 + g;
+      const bool live = rr < row_all;
+      const float undo = load_q<D>(p, s.row0 + (live ? rr / p.group : 0), h * p.group + (live ? rr % p.group : 0), t, live, qf[nt]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        csc[nt][j] = __shfl_sync(~0u, undo, (2 * t + j) * 4) * p.scale_log2;
+        const int r2 = row_base + nt * 8 + 2 * t + j;
+        pos[nt][j] = r2 < row_all ? s.n - s.rows + r2 / p.group : -1;
+      }
+    }
+    float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) O[nt][i][j] = 0.f;
+    }
+
+    // this warp's 16 tokens of unit i; none if the base is past what the row tile sees
+    auto base_of = [&](int i) -> int {
+      const int x = i < sp.sink_units ? i * kUnit : sp.lo + (i - sp.sink_units) * kUnit;
+      const int tok = x + 16 * warp;
+      if (p.window && tok + 15 <= first_pos - p.window && tok >= p.sinks) return -1;  // between sinks and window
+      return (i < i1 && tok < (i < sp.sink_units ? sp.sink_end : sp.end)) ? tok : -1;
+    };
+    auto id_of = [&](int tok) -> int { return tok < 0 ? -1 : kv_block_at(c, b, tok / c.block, p.err); };
+    uint4 kr[2][2][D / 64], vr[2][4];
+    float ks[2], vs[2];
+    auto load = [&](int buf, int tok, int id) {
+      if (id < 0) return;
+      const int64_t bh = (int64_t)id * c.heads + h;
+      const int64_t row = bh * c.block + (tok & (c.block - 1));
+      const uint8_t* kp = c.k + row * D + 16 * t;
+      const uint8_t* vp = c.v + row * D + (D / 8) * g;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int cc = 0; cc < D / 64; ++cc)
+          kr[buf][i][cc] = __ldg(reinterpret_cast<const uint4*>(kp + (g + 8 * i) * D + 64 * cc));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* q = vp + (2 * t + (i & 1) + 8 * (i >> 1)) * D;
+        if (D == 128) vr[buf][i] = __ldg(reinterpret_cast<const uint4*>(q));
+        else {
+          const uint2 x = __ldg(reinterpret_cast<const uint2*>(q));
+          vr[buf][i] = make_uint4(x.x, x.y, 0, 0);
+        }
+      }
+      ks[buf] = __ldg(c.k_scale + bh);
+      vs[buf] = __ldg(c.v_scale + bh);
+    };
+
+    auto step = [&](int buf, int tok) {
+      float S[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) S[nt][0] = S[nt][1] = S[nt][2] = S[nt][3] = 0.f;
+      qk<D, FMT, NT>(kr[buf], qf, S);
+      const bool plain = tok + 15 <= first_pos && row_base + ROWS <= row_all &&
+                         (!p.window || tok > last_pos - p.window || tok + 15 < p.sinks);
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          S[nt][j] *= csc[nt][j & 1] * ks[buf];
+          if (!plain) {
+            const int k = tok + g + 8 * (j >> 1), q = pos[nt][j & 1];
+            if (!(k <= q && (!p.window || k > q - p.window || k < p.sinks))) S[nt][j] = -INFINITY;
+          }
+          grow |= S[nt][j] > m[nt][j & 1] + kSlack;
+        }
+      if (!plain) {  // what no row sees may hold anything: not even 0 * NaN of it
+        const int lo = p.window ? first_pos - p.window + 1 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = tok + 2 * t + (i & 1) + 8 * (i >> 1);
+          if (k >= sp.end || (k < lo && k >= p.sinks)) vr[buf][i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      const bool vgrow = vs[buf] > vref;
+      if (__any_sync(~0u, grow || vgrow)) {
+        const float vf = vgrow ? vref / vs[buf] : 1.f;
+        if (vgrow) vref = vs[buf];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float a[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float x = fmaxf(m[nt][j], fmaxf(S[nt][j], S[nt][j + 2]));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+            a[j] = x == m[nt][j] ? 1.f : ex2(m[nt][j] - x);
+            m[nt][j] = x;
+            l[nt][j] *= a[j];
+            a[j] *= vf;
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            O[nt][i][0] *= a[0];
+            O[nt][i][1] *= a[1];
+            O[nt][i][2] *= a[0];
+            O[nt][i][3] *= a[1];
+          }
+        }
+      }
+      const float vf = vs[buf] / vref;
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float ref = m[nt][j & 1] == -INFINITY ? 0.f : m[nt][j & 1];
+          x[j] = ex2(S[nt][j] - ref + kShift);
+          l[nt][j & 1] += x[j];
+          x[j] *= vf;
+        }
+        pb[nt][0] = movmatrix_trans(f2h(x[0], x[1]));
+        pb[nt][1] = movmatrix_trans(f2h(x[2], x[3]));
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t x0 = (&vr[buf][0].x)[w], x1 = (&vr[buf][1].x)[w], y0 = (&vr[buf][2].x)[w], y1 = (&vr[buf][3].x)[w];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t sel = half ? 0x7362u : 0x5140u;  // two tokens' bytes in pairs
+          const uint32_t a = __byte_perm(x0, x1, sel), e = __byte_perm(y0, y1, sel);
+          const uint32_t a0 = KvFmt<FMT>::lo(a), a1 = KvFmt<FMT>::hi(a), a2 = KvFmt<FMT>::lo(e), a3 = KvFmt<FMT>::hi(e);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(O[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        }
+      }
+    };
+
+    int tok0 = base_of(i0), id0 = id_of(tok0);
+    load(0, tok0, id0);
+    int tok1 = base_of(i0 + 1), id1 = id_of(tok1);
+    for (int i = i0; i < i1; i += 2) {
+      load(1, tok1, id1);
+      const int tok2 = base_of(i + 2), id2 = id_of(tok2);
+      if (id0 >= 0) step(0, tok0);
+      load(0, tok2, id2);
+      const int tok3 = base_of(i + 3), id3 = id_of(tok3);
+      if (id1 >= 0) step(1, tok1);
+      tok0 = tok2;
+      id0 = id2;
+      tok1 = tok3;
+      id1 = id3;
+    }
+
+    // join the four warps: rows' maxima, then scaled sums through shared memory
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x = l[nt][j];
+        x += __shfl_xor_sync(~0u, x, 4);
+        x += __shfl_xor_sync(~0u, x, 8);
+        x += __shfl_xor_sync(~0u, x, 16);
+        if (g == 0) {
+          sm[warp][nt * 8 + 2 * t + j] = m[nt][j];
+          sl[warp][nt * 8 + 2 * t + j] = x;
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int rr = nt * 8 + 2 * t + j;
+        float M = sm[0][rr];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm[w][rr]);
+        const float f = (m[nt][j] == M ? 1.f : ex2(m[nt][j] - M)) * vref;
+        float* dst = &sO[warp * ROWS + rr][(D / 8) * g];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(O[nt][i][j] * f, O[nt][i][j + 2] * f);
+      }
+    __syncthreads();
+    const bool whole = i0 == 0 && i1 == per;
+    float* part = p.part + (2 * (int64_t)blockIdx.x + (u == u_begin ? 0 : 1)) * part_floats<D, NT>();
+    for (int e = tid; e < ROWS * D / 4; e += kWarps * 32) {
+      const int rr = e / (D / 4), d = (e - rr * (D / 4)) * 4;
+      float M = sm[0][rr];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm[w][rr]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(&sO[w * ROWS + rr][d]);
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
+        L += sl[w][rr] * (sm[w][rr] == M ? 1.f : ex2(sm[w][rr] - M));
+      }
+      if (!whole) {
+        *reinterpret_cast<float4*>(part + rr * D + d) = o;
+        if (d == 0) {
+          part[ROWS * D + rr] = M;
+          part[ROWS * D + ROWS + rr] = L;
+        }
+        continue;
+      }
+      const int r2 = row_base + rr;
+      if (r2 >= row_all) continue;
+      const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      uint2 w;
+      if (p.act == DUPLEX_DTYPE_F16) w = make_uint2(f2h(o.x * inv, o.y * inv), f2h(o.z * inv, o.w * inv));
+      else {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) = w;
+      if (d == 0 && p.lse) p.lse[at] = L == 0.f ? -INFINITY : (M - kShift + log2f(L)) * kLn2;
+    }
+    __syncthreads();
+    u += i1 - i0;
+  }
+}
+
+// CTA j joins the row tile that crosses the boundary between pieces j and j + 1, if that is its first one.
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p, int ctas) {
+  constexpr int ROWS = 8 * NT;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  int64_t* off = reinterpret_cast<int64_t*>(dyn);
+  const KvView& c = p.c;
+  const int tid = threadIdx.x;
+  const Plan plan = make_plan<ROWS>(p, off, ctas);
+  const int64_t u = (int64_t)(blockIdx.x + 1) * plan.share;
+  pdl_wait();
+  if (u >= plan.total) return;
+  const int b = seq_of(off, c.batch, u);
+  const KvSeq s = kv_seq(c, b);
+  const int rt_all = tiles_of(s, p.group, ROWS), per = units_of(s, p, ROWS);
+  const int it = (int)((u - off[b]) / per);
+  const int64_t begin = off[b] + (int64_t)it * per, last = begin + per - 1;
+  if (begin == u || begin / plan.share != blockIdx.x) return;
+  const int c0 = blockIdx.x, c1 = (int)(last / plan.share);
+  const int h = it / rt_all, rt = it - h * rt_all, row_all = s.rows * p.group;
+  for (int e = tid; e < ROWS * D / 4; e += kWarps * 32) {
+    const int rr = e / (D / 4), d = (e - rr * (D / 4)) * 4, r2 = rt * ROWS + rr;
+    if (r2 >= row_all) continue;
+    // piece j > c0 begins inside the row tile: its first slot.  Piece c0's is its first too if the tile begins it.
+    auto slot = [&](int j) {
+      const int k = (j == c0 && begin != (int64_t)c0 * plan.share) ? 1 : 0;
+      return p.part + (2 * (int64_t)j + k) * part_floats<D, NT>();
+    };
+    float M = -INFINITY;
+    for (int j = c0; j <= c1; ++j) M = fmaxf(M, __ldcg(slot(j) + ROWS * D + rr));
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f;
+#pragma unroll 4
+    for (int j = c0; j <= c1; ++j) {
+      const float* ps = slot(j);
+      const float mj = __ldcg(ps + ROWS * D + rr), f = mj == M ? 1.f : ex2(mj - M);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(ps + rr * D + d));
+      L += __ldcg(ps + ROWS * D + ROWS + rr) * f;
+      o.x += x.x * f;
+      o.y += x.y * f;
+      o.z += x.z * f;
+      o.w += x.w * f;
+    }
+    const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    uint2 w;
+    if (p.act == DUPLEX_DTYPE_F16) w = make_uint2(f2h(o.x * inv, o.y * inv), f2h(o.z * inv, o.w * inv));
+    else {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+      w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) = w;
+    if (d == 0 && p.lse) p.lse[at] = L == 0.f ? -INFINITY : (M - kShift + log2f(L)) * kLn2;
+  }
+}
+
+// Accumulated attention weights: weights[token] += sum over the sequence's rows and the group's
+// heads of exp(s - lse), after the attention itself.  A warp owns 16 tokens: their keys stay in its
+// registers as fp16, the query rows come by, 32 at a time, through shared memory.
+constexpr int kRowChunk = 32;
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p) {
+  __shared__ uint2 sq[kRowChunk / 8][D / 16][32];
+  __shared__ float s_sc[kRowChunk], s_lse[kRowChunk];
+  __shared__ int s_pos[kRowChunk];
+  const KvView& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const KvSeq s = kv_seq(c, b);
+  const int tile = blockIdx.x * kUnit, start = s.n - s.rows;
+  if (tile >= s.n) return;
+  // the sequence's rows that see a token of the tile
+  int t0 = max(tile - start, 0), t1 = s.rows;
+  if (p.window && tile >= p.sinks) t1 = (int)min((int64_t)t1, (int64_t)tile + kUnit - 1 + p.window - start);
+  if (t0 >= t1) return;
+  const int tok = tile + 16 * warp;
+  const bool hidden = tok >= s.n || (p.window && tok + 15 <= start - p.window && tok >= p.sinks);
+  const int id = hidden ? -1 : kv_block_at(c, b, tok / c.block, p.err);
+  const int64_t bh = (int64_t)max(id, 0) * c.heads + h;
+  uint4 kr[2][D / 64];
+  float ks = 0.f;
+  if (id >= 0) {
+    const uint8_t* kp = c.k + (bh * c.block + (tok & (c.block - 1))) * D + 16 * t;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int cc = 0; cc < D / 64; ++cc) kr[i][cc] = __ldg(reinterpret_cast<const uint4*>(kp + (g + 8 * i) * D + 64 * cc));
+    ks = __ldg(c.k_scale + bh);
+  }
+  float sum[2] = {0.f, 0.f};
+  const int r1 = t1 * p.group;
+  for (int r0 = t0 * p.group; r0 < r1; r0 += kRowChunk) {
+    __syncthreads();
+    {  // thread 4 r + t stages row r's dims 64 cc + 16 t .. + 16
+      const int r = tid >> 2, rr = r0 + r;
+      const bool live = rr < r1;
+      uint2 qf[D / 16];
+      const int row = s.row0 + (live ? rr / p.group : 0), head = h * p.group + (live ? rr % p.group : 0);
+      const float undo = load_q<D>(p, row, head, t, live, qf);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) sq[r >> 3][i][(r & 7) * 4 + t] = qf[i];
+      if (t == 0) {
+        s_sc[r] = undo * p.scale_log2;
+        s_lse[r] = live ? p.lse[(int64_t)row * p.heads + head] * kLog2e : 0.f;
+        s_pos[r] = live ? start + rr / p.group : -1;
+      }
+    }
+    __syncthreads();
+    if (id < 0) continue;
+#pragma unroll
+    for (int nt = 0; nt < kRowChunk / 8; ++nt) {
+      if (r0 + nt * 8 >= r1) break;
+      uint2 qf[1][D / 16];
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) qf[0][i] = sq[nt][i][lane];
+      float S[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+      qk<D, FMT, 1>(kr, qf, S);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int rr = nt * 8 + 2 * t + (j & 1), k = tok + g + 8 * (j >> 1), q = s_pos[rr];
+        if (k <= q && (!p.window || k > q - p.window || k < p.sinks)) sum[j >> 1] += ex2(S[0][j] * (s_sc[rr] * ks) - s_lse[rr]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float x = sum[i];
+    x += __shfl_xor_sync(~0u, x, 1);
+    x += __shfl_xor_sync(~0u, x, 2);
+    const int k = tok + g + 8 * i;
+    // one addition to a token's sum, so its order does not matter; sequences that share a block may add to the same one
+    if (t == 0 && id >= 0 && k < s.n) atomicAdd(c.weights + bh * c.block + (k & (c.block - 1)), x);
+  }
+}
+
+int kv_check(const duplex_kv_cache* c, const duplex_kv_batch* b, KvView* out);
+
+// 16 rows a tile need half the passes over the cache of 8, at 2 CTAs an SM instead of 3
+static int nt_of(const KvView& c, int group) {
+  const int64_t rows = ((int64_t)c.n_rows * group + c.batch - 1) / c.batch;
+  return rows > 8 ? 2 : 1;
+}
+
+static size_t part_bytes(const KvView& c, int nt) {
+  return (size_t)2 * kMaxCtas * (c.dim == 128 ? (nt == 1 ? part_floats<128, 1>() : part_floats<128, 2>())
+                                              : (nt == 1 ? part_floats<64, 1>() : part_floats<64, 2>())) * 4;
+}
+
+template <int D, int FMT, int NT>
+static int run_attend(const AttendParams& p, cudaStream_t st) {
+  constexpr int ROWS = 8 * NT;
+  const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = sizeof(float) * kWarps * ROWS * (D + 4) + plan;
+  static int sms = 0;
+  if (!sms) {
+    int dev = 0;
+    if (int rc = record_cuda(cudaGetDevice(&dev))) return rc;
+    if (int rc = record_cuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev))) return rc;
+  }
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attend_kernel<D, FMT, NT>), 100 * 1024)) return rc;
+  // no more CTAs than units there can be
+  const int64_t tiles = ((int64_t)p.c.n_rows * p.group) / ROWS + p.c.batch;
+  const int64_t units = tiles * p.c.heads * (((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit);
+  const int ctas = (int)std::min(std::min((int64_t)sms * (NT == 1 ? 3 : 2), (int64_t)kMaxCtas), units);
+  kv_attend_kernel<D, FMT, NT><<<ctas, kWarps * 32, smem, st>>>(p);
+  if (int rc = record_cuda(cudaGetLastError())) return rc;
+  if (ctas > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas - 1);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = plan;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (int rc = record_cuda(cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, NT>, p, ctas))) return rc;
+  }
+  if (p.c.weights) {
+    const dim3 grid((unsigned)(((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit), p.c.heads, p.c.batch);
+    kv_weights_kernel<D, FMT><<<grid, kWarps * 32, 0, st>>>(p);
+    return record_cuda(cudaGetLastError());
+  }
+  return DUPLEX_OK;
+}
+
+template <int D, int FMT>
+static int run_attend_nt(const AttendParams& p, cudaStream_t st) {
+  return nt_of(p.c, p.group) == 1 ? run_attend<D, FMT, 1>(p, st) : run_attend<D, FMT, 2>(p, st);
+}
+
+}  // namespace duplex
+
+using namespace duplex;
+
+extern "C" int duplex_kv_attend_workspace_bytes(const duplex_kv_cache* cache, const duplex_kv_batch* batch,
+                                                int32_t heads, size_t* bytes) {
+  KvView v;
+  if (int rc = kv_check(cache, batch, &v)) return rc;
+  if (!bytes || heads < 1 || heads % cache->kv_heads) return DUPLEX_ERR_ARG;
+  *bytes = part_bytes(v, nt_of(v, heads / cache->kv_heads)) + (size_t)batch->n_rows * heads * 4;
+  return DUPLEX_OK;
+}
+
+extern "C" int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_batch* batch, const void* q,
+                                int act_dtype, int32_t heads, int64_t q_row_stride, int64_t q_head_stride,
+                                float softmax_scale, int32_t window, int32_t sinks, void* out, float* lse,
+                                void* workspace, size_t workspace_bytes, int32_t* err, void* stream) {
+  AttendParams p{};
+  if (int rc = kv_check(cache, batch, &p.c)) return rc;
+  if (act_dtype != DUPLEX_DTYPE_F16 && act_dtype != DUPLEX_DTYPE_BF16) return DUPLEX_ERR_DTYPE;
+  if (heads < 1 || heads % cache->kv_heads || window < 0 || sinks < 0) return DUPLEX_ERR_ARG;
+  if (!(softmax_scale - softmax_scale == 0.f)) return DUPLEX_ERR_ARG;
+  if (batch->n_rows == 0) return DUPLEX_OK;
+  if (!q || !out) return DUPLEX_ERR_ARG;
+  if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_row_stride | q_head_stride) & 7)) return DUPLEX_ERR_ALIGN;
+  size_t need = 0;
+  if (int rc = duplex_kv_attend_workspace_bytes(cache, batch, heads, &need)) return rc;
+  if (!workspace || workspace_bytes < need) return DUPLEX_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return DUPLEX_ERR_ALIGN;
+  p.q = q;
+  p.q_row = q_row_stride;
+  p.q_head = q_head_stride;
+  p.act = act_dtype;
+  p.heads = heads;
+  p.group = heads / cache->kv_heads;
+  // a row tile's rows are counted in 32 bits
+  if ((int64_t)batch->n_rows * p.group > 0x7FFFFFFFll - 256) return DUPLEX_ERR_UNSUPPORTED;
+  const int64_t cap = (int64_t)batch->width * cache->block;  // a window of all that can be cached is none
+  p.window = window >= cap ? 0 : window;
+  p.sinks = (int)std::min((int64_t)sinks, cap);
+  p.scale_log2 = softmax_scale * kLog2e;
+  p.out = out;
+  p.part = static_cast<float*>(workspace);
+  p.lse = lse ? lse
+              : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + need - (size_t)batch->n_rows * heads * 4);
+  p.err = err;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (cache->dim == 128)
+    return cache->format == DUPLEX_KV_E4M3 ? run_attend_nt<128, DUPLEX_KV_E4M3>(p, st) : run_attend_nt<128, DUPLEX_KV_INT8>(p, st);
+  return cache->format == DUPLEX_KV_E4M3 ? run_attend_nt<64, DUPLEX_KV_E4M3>(p, st) : run_attend_nt<64, DUPLEX_KV_INT8>(p, st);
+}

@@ -18,7 +18,8 @@ _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("DUPLEX_B200_LIB", _PKG / "libduplex_b200.so"))
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
-DEVERR_EXPERT, DEVERR_TIMEOUT = 1, 2
+DEVERR_EXPERT, DEVERR_TIMEOUT, DEVERR_NONFINITE, DEVERR_BLOCK = 1, 2, 4, 8
+KV_E4M3, KV_INT8 = 0, 1
 
 _c_int, _c_i32, _c_i64, _c_ptr, _c_size, _c_f32 = (ctypes.c_int, ctypes.c_int32, ctypes.c_int64,
                                                    ctypes.c_void_p, ctypes.c_size_t,
@@ -127,6 +128,16 @@ _SIGNATURES = {
                                   ctypes.POINTER(ctypes.c_size_t)], _c_int),
     "duplex_repack_down_slices": ([_c_ptr, _c_ptr, _c_ptr, _c_int, _c_i32, _c_i32, _c_i32, _c_i32,
                                    _c_ptr, _c_size, _c_ptr], _c_int),
+    "duplex_kv_append": ([_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_i64,
+                          _c_ptr, _c_ptr], _c_int),
+    "duplex_kv_attend_workspace_bytes": ([_c_ptr, _c_ptr, _c_i32, ctypes.POINTER(ctypes.c_size_t)],
+                                         _c_int),
+    "duplex_kv_attend": ([_c_ptr, _c_ptr, _c_ptr, _c_int, _c_i32, _c_i64, _c_i64, _c_f32, _c_i32,
+                          _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr, _c_ptr], _c_int),
+    "duplex_kv_evict_workspace_bytes": ([_c_ptr, _c_ptr, _c_i32, ctypes.POINTER(ctypes.c_size_t)],
+                                        _c_int),
+    "duplex_kv_evict": ([_c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr,
+                         _c_size, _c_ptr, _c_ptr], _c_int),
 }
 
 
@@ -135,6 +146,21 @@ class StackLayer(ctypes.Structure):
     _fields_ = [("qkv_tiles", ctypes.c_void_p), ("o_tiles", ctypes.c_void_p),
                 ("gate_w", ctypes.c_void_p), ("gate_b", ctypes.c_void_p),
                 ("gu_tiles", ctypes.c_void_p), ("dn_tiles", ctypes.c_void_p)]
+
+
+class KVCache(ctypes.Structure):
+    """duplex_kv_cache of include/duplex_b200.h."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+                ("n_blocks", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("block", ctypes.c_int32), ("dim", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+class KVBatch(ctypes.Structure):
+    """duplex_kv_batch of include/duplex_b200.h."""
+    _fields_ = [("block_table", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("cu_rows", ctypes.c_void_p), ("width", ctypes.c_int32),
+                ("batch", ctypes.c_int32), ("n_rows", ctypes.c_int32)]
 
 
 _lib = None
