@@ -20,7 +20,7 @@ struct KvView {
   uint8_t *k, *v;
   float *k_scale, *v_scale;
   float* weights;        // [n_blocks][kv_heads][block] accumulated attention weights, or null
-  int n_blocks, heads, block, dim;
+  int n_blocks, heads, block, dim, format;
   const int32_t* table;  // [batch][width] block ids
   const int32_t* kv_len; // [batch]
   const int32_t* cu;     // [batch + 1] row offsets, or null: rows split evenly

@@ -19,31 +19,14 @@
 // kv_combine_kernel joins in order: no atomics, the same bits on each run.
 #include <algorithm>
 
-#include "kv.cuh"
+#include "kv_attend.cuh"
 
 namespace duplex {
 
 constexpr int kWarps = 4;
 constexpr int kUnit = 16 * kWarps;   // tokens
 constexpr int kMaxCtas = 148 * 4;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-// p = exp2(s - m + kShift) is what fp16 holds: the reference m may be 2^kSlack behind the true
-// maximum (so it rarely moves), p stays below 2^15, and a p of 2^-21 of the reference is still normal.
-constexpr float kShift = 7.f, kSlack = 8.f;
 
-struct AttendParams {
-  KvView c;
-  const void* q;
-  int64_t q_row, q_head;  // elements
-  int act, heads, group;
-  int window, sinks;
-  float scale_log2;       // softmax_scale * log2(e)
-  void* out;              // [n_rows][heads][dim]
-  float* lse;             // [n_rows][heads] or null
-  float* part;            // partial results, 2 slots per CTA
-  int32_t* err;
-};
 
 // The unit list of a launch: off[b] units before sequence b.  A row tile of sequence b has units(b)
 // units, the most that any of its row tiles needs.
@@ -117,12 +100,6 @@ DEVI uint32_t movmatrix_trans(uint32_t a) {
   return d;
 }
 
-DEVI float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // fp16 query fragments of 8 rows: row r's 16 dims at 64 cc + 16 t, scaled by a power of two that
 // brings the row's largest into [2^14, 2^15): bf16's 8 bits fit fp16's 11, and only values below
 // 2^-28 of the row's largest lose bits.  Returns the factor that undoes it.
@@ -174,27 +151,6 @@ DEVI void qk(const uint4 (&kr)[2][D / 64], const uint2 (&qf)[NT][D / 16], float 
     }
 }
 
-// the tokens of one row tile: [0, sink_end) and [lo, end), in units
-struct Span {
-  int sink_units, lo, end, sink_end;  // lo aligned to a unit
-};
-
-DEVI Span span_of(const AttendParams& p, int first_pos, int last_pos, int n) {
-  Span s;
-  s.end = min(last_pos + 1, n);
-  s.lo = 0;
-  s.sink_units = 0;
-  s.sink_end = 0;
-  if (p.window) {
-    const int64_t w = (int64_t)first_pos - p.window + 1;
-    s.lo = w > 0 ? (int)(w / kUnit) * kUnit : 0;
-    s.sink_end = min(p.sinks, s.end);
-    s.sink_units = (s.sink_end + kUnit - 1) / kUnit;
-    if (s.sink_units * kUnit >= s.lo) s.lo = s.sink_units = s.sink_end = 0;
-  }
-  return s;
-}
-
 template <int D, int NT>
 constexpr int part_floats() { return 8 * NT * (D + 2); }  // O [rows][D], m [rows], l [rows]
 
@@ -227,7 +183,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
     const int first_pos = s.n - s.rows + row_base / p.group;
     const int last_row = min(row_base + ROWS, row_all) - 1;
     const int last_pos = s.n - s.rows + last_row / p.group;
-    const Span sp = span_of(p, first_pos, last_pos, s.n);
+    const Span sp = span_of<kUnit>(p, first_pos, last_pos, s.n);
 
     // query rows: as the product's columns, lane (g, t) loads row g and accumulates rows 2t, 2t + 1
     uint2 qf[NT][D / 16];
@@ -449,14 +405,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
       if (r2 >= row_all) continue;
       const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
       const float inv = L == 0.f ? 0.f : 1.f / L;
-      uint2 w;
-      if (p.act == DUPLEX_DTYPE_F16) w = make_uint2(f2h(o.x * inv, o.y * inv), f2h(o.z * inv, o.w * inv));
-      else {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-        w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-      }
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) = w;
-      if (d == 0 && p.lse) p.lse[at] = L == 0.f ? -INFINITY : (M - kShift + log2f(L)) * kLn2;
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
+          pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+      if (d == 0) p.lse[at] = lse_of(M, L);
     }
     __syncthreads();
     u += i1 - i0;
@@ -508,14 +459,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p,
     }
     const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    uint2 w;
-    if (p.act == DUPLEX_DTYPE_F16) w = make_uint2(f2h(o.x * inv, o.y * inv), f2h(o.z * inv, o.w * inv));
-    else {
-      const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-      w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-    }
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) = w;
-    if (d == 0 && p.lse) p.lse[at] = L == 0.f ? -INFINITY : (M - kShift + log2f(L)) * kLn2;
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
+        pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (d == 0) p.lse[at] = lse_of(M, L);
   }
 }
 
@@ -599,8 +545,6 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
   }
 }
 
-int kv_check(const duplex_kv_cache* c, const duplex_kv_batch* b, KvView* out);
-
 // 16 rows a tile need half the passes over the cache of 8, at 2 CTAs an SM instead of 3
 static int nt_of(const KvView& c, int group) {
   const int64_t rows = ((int64_t)c.n_rows * group + c.batch - 1) / c.batch;
@@ -616,12 +560,8 @@ template <int D, int FMT, int NT>
 static int run_attend(const AttendParams& p, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
   const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = sizeof(float) * kWarps * ROWS * (D + 4) + plan;
-  static int sms = 0;
-  if (!sms) {
-    int dev = 0;
-    if (int rc = record_cuda(cudaGetDevice(&dev))) return rc;
-    if (int rc = record_cuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev))) return rc;
-  }
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
   if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attend_kernel<D, FMT, NT>), 100 * 1024)) return rc;
   // no more CTAs than units there can be
   const int64_t tiles = ((int64_t)p.c.n_rows * p.group) / ROWS + p.c.batch;
@@ -642,17 +582,29 @@ static int run_attend(const AttendParams& p, cudaStream_t st) {
     cfg.numAttrs = 1;
     if (int rc = record_cuda(cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, NT>, p, ctas))) return rc;
   }
-  if (p.c.weights) {
-    const dim3 grid((unsigned)(((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit), p.c.heads, p.c.batch);
-    kv_weights_kernel<D, FMT><<<grid, kWarps * 32, 0, st>>>(p);
-    return record_cuda(cudaGetLastError());
-  }
   return DUPLEX_OK;
 }
 
 template <int D, int FMT>
-static int run_attend_nt(const AttendParams& p, cudaStream_t st) {
-  return nt_of(p.c, p.group) == 1 ? run_attend<D, FMT, 1>(p, st) : run_attend<D, FMT, 2>(p, st);
+static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
+  const int rc = kv_prompt_takes(p.c, p.group) ? kv_prompt_run(p, workspace, st)
+                 : nt_of(p.c, p.group) == 1    ? run_attend<D, FMT, 1>(p, st)
+                                               : run_attend<D, FMT, 2>(p, st);
+  if (rc || !p.c.weights) return rc;
+  const dim3 grid((unsigned)(((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit), p.c.heads, p.c.batch);
+  kv_weights_kernel<D, FMT><<<grid, kWarps * 32, 0, st>>>(p);
+  return record_cuda(cudaGetLastError());
+}
+
+// the rows' sums of exponentials lie behind the rest of the workspace
+static size_t front_bytes(const KvView& c, int group) {
+  return kv_prompt_takes(c, group) ? kv_prompt_workspace(c, group) : part_bytes(c, nt_of(c, group));
+}
+
+int device_sms(int* sms) {
+  int dev = 0;
+  if (int rc = record_cuda(cudaGetDevice(&dev))) return rc;
+  return record_cuda(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
 }
 
 }  // namespace duplex
@@ -664,7 +616,7 @@ extern "C" int duplex_kv_attend_workspace_bytes(const duplex_kv_cache* cache, co
   KvView v;
   if (int rc = kv_check(cache, batch, &v)) return rc;
   if (!bytes || heads < 1 || heads % cache->kv_heads) return DUPLEX_ERR_ARG;
-  *bytes = part_bytes(v, nt_of(v, heads / cache->kv_heads)) + (size_t)batch->n_rows * heads * 4;
+  *bytes = front_bytes(v, heads / cache->kv_heads) + (size_t)batch->n_rows * heads * 4;
   return DUPLEX_OK;
 }
 
@@ -698,11 +650,10 @@ extern "C" int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_ba
   p.scale_log2 = softmax_scale * kLog2e;
   p.out = out;
   p.part = static_cast<float*>(workspace);
-  p.lse = lse ? lse
-              : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + need - (size_t)batch->n_rows * heads * 4);
+  p.lse = lse ? lse : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + front_bytes(p.c, p.group));
   p.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cache->dim == 128)
-    return cache->format == DUPLEX_KV_E4M3 ? run_attend_nt<128, DUPLEX_KV_E4M3>(p, st) : run_attend_nt<128, DUPLEX_KV_INT8>(p, st);
-  return cache->format == DUPLEX_KV_E4M3 ? run_attend_nt<64, DUPLEX_KV_E4M3>(p, st) : run_attend_nt<64, DUPLEX_KV_INT8>(p, st);
+    return cache->format == DUPLEX_KV_E4M3 ? run_all<128, DUPLEX_KV_E4M3>(p, workspace, st) : run_all<128, DUPLEX_KV_INT8>(p, workspace, st);
+  return cache->format == DUPLEX_KV_E4M3 ? run_all<64, DUPLEX_KV_E4M3>(p, workspace, st) : run_all<64, DUPLEX_KV_INT8>(p, workspace, st);
 }

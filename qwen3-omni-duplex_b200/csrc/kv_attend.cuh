@@ -1,0 +1,73 @@
+// What the two attention kernels over the 8-bit paged KV cache share (kv_attend.cu: few query rows a
+// sequence; kv_prompt.cu: many).
+#pragma once
+
+#include "kv.cuh"
+
+namespace duplex {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// p = exp2(s - m + kShift) is what fp16 holds: the reference m may be 2^kSlack behind the true
+// maximum (so it rarely moves), p stays below 2^15, and a p of 2^-21 of the reference is still normal.
+constexpr float kShift = 7.f, kSlack = 8.f;
+
+struct AttendParams {
+  KvView c;
+  const void* q;
+  int64_t q_row, q_head;  // elements
+  int act, heads, group;
+  int window, sinks;
+  float scale_log2;       // softmax_scale * log2(e)
+  void* out;              // [n_rows][heads][dim]
+  float* lse;             // [n_rows][heads] or null
+  float* part;            // partial results, 2 slots per CTA
+  int32_t* err;
+};
+
+DEVI float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// the tokens of one row tile: [0, sink_end) and [lo, end), in units of U tokens
+struct Span {
+  int sink_units, lo, end, sink_end;  // lo aligned to a unit
+};
+
+template <int U>
+DEVI Span span_of(const AttendParams& p, int first_pos, int last_pos, int n) {
+  Span s;
+  s.end = min(last_pos + 1, n);
+  s.lo = 0;
+  s.sink_units = 0;
+  s.sink_end = 0;
+  if (p.window) {
+    const int64_t w = (int64_t)first_pos - p.window + 1;
+    s.lo = w > 0 ? (int)(w / U) * U : 0;
+    s.sink_end = min(p.sinks, s.end);
+    s.sink_units = (s.sink_end + U - 1) / U;
+    if (s.sink_units * U >= s.lo) s.lo = s.sink_units = s.sink_end = 0;
+  }
+  return s;
+}
+
+// one row's result: o / l in q's type, and the natural logarithm of the sum
+DEVI uint2 pack4(int act, float4 o) {
+  if (act == DUPLEX_DTYPE_F16) return make_uint2(f2h(o.x, o.y), f2h(o.z, o.w));
+  const __nv_bfloat162 x = __floats2bfloat162_rn(o.x, o.y), y = __floats2bfloat162_rn(o.z, o.w);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+DEVI float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * kLn2; }
+
+int kv_check(const duplex_kv_cache* c, const duplex_kv_batch* b, KvView* out);
+int device_sms(int* sms);
+
+// kv_prompt.cu
+bool kv_prompt_takes(const KvView& c, int group);
+size_t kv_prompt_workspace(const KvView& c, int group);
+int kv_prompt_run(const AttendParams& p, void* workspace, cudaStream_t st);
+
+}  // namespace duplex

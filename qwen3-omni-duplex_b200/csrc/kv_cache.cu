@@ -328,7 +328,7 @@ int kv_check(const duplex_kv_cache* c, const duplex_kv_batch* b, KvView* out) {
   if (!b->cu_rows && b->n_rows % b->batch) return DUPLEX_ERR_ARG;
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return DUPLEX_ERR_ALIGN;
   *out = KvView{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale, c->weights,
-                c->n_blocks, c->kv_heads, c->block, c->dim, b->block_table, b->kv_len, b->cu_rows,
+                c->n_blocks, c->kv_heads, c->block, c->dim, c->format, b->block_table, b->kv_len, b->cu_rows,
                 b->width, b->batch, b->n_rows};
   return DUPLEX_OK;
 }

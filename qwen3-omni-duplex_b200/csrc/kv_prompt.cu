@@ -1,0 +1,703 @@
+// Attention over the 8-bit paged KV cache for many query rows a sequence (prompts, chunks of them),
+// on the tensor cores: the formulas of kv_attend.cu over 256 query rows and 128 tokens at a time.
+//
+// Bound by products: 4 dim flops per row and token.  A CTA holds 256 rows (the heads of a KV group
+// are rows like any other) as two tiles of 128 in shared memory, and their scores and outputs in
+// tensor memory: S0, S1 [128 x 128] fp32 and O0, O1 [128 x dim] fp32, all 512 columns at dim 128.
+// The tiles take turns, so that one tile's softmax runs under the other's products:
+//
+//   warps 0-3, 4-7   softmax of tile 0, 1: a thread owns a row.  S from tensor memory, exp2, P back as
+//                    fp16 into S's own columns (the next product's A operand)
+//   warps 8-11       keys and values from the cache's codes to fp16 operands in shared memory (exact:
+//                    code times its block's scale over the row tile's largest, a power of two), two
+//                    buffers each.  Values are transposed on the way: B[dim][token]
+//   warp 12          one thread issues the products: S = Q K^T (both shared memory), O += P V
+//
+// The running maximum is a reference that may lag by 2^kSlack, so O is rescaled rarely: the exponentials
+// are taken at the old reference while the true maximum is found, and only where it has grown too far
+// is the tile's O multiplied and its exponentials taken again.
+//
+// Work is one list of (row tile, head) items, 128 tokens a unit, cut into equal contiguous pieces, one
+// per SM; kv_prompt_plan_kernel writes it (causal row tiles differ in length), kv_prompt_join_kernel
+// joins the items that a cut went through.
+#include <algorithm>
+
+#include "kv_attend.cuh"
+#include "umma.cuh"
+
+namespace duplex {
+
+constexpr int kPTok = 128, kPRows = 256, kPThreads = 13 * 32, kPMaxCtas = 160;
+
+struct PromptItem {
+  int64_t off;  // units before it (of all heads)
+  int b, rt;
+};
+
+struct PromptParams {
+  AttendParams a;
+  PromptItem* list;  // pairs (sequence, row tile), and an end
+  int* n_pairs;
+  int64_t* total;
+};
+
+DEVI void prompt_rows(const AttendParams& p, const KvSeq& s, int rt, int& row_base, int& row_all, int& first_pos, int& last_pos) {
+  row_base = rt * kPRows;
+  row_all = s.rows * p.group;
+  first_pos = s.n - s.rows + row_base / p.group;
+  last_pos = s.n - s.rows + (min(row_base + kPRows, row_all) - 1) / p.group;
+}
+
+DEVI int units_in(const Span& sp) {
+  return sp.sink_units + (sp.end > sp.lo ? (sp.end - sp.lo + kPTok - 1) / kPTok : 0);
+}
+
+// The list of (sequence, row tile) pairs with their units, by one CTA.
+constexpr int kPlanThreads = 1024;
+
+__global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptParams pp) {
+  extern __shared__ int tiles[];  // [batch + 1] row tiles before each sequence
+  __shared__ int64_t warp_sum[kPlanThreads / 32];
+  const AttendParams& p = pp.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = p.c.batch;
+  pdl_launch_dependents();
+  auto scan = [&](int64_t x, int64_t& all) {  // exclusive, over the block
+    int64_t incl = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int64_t before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    return before + incl - x;
+  };
+  int64_t base = 0, all = 0;
+  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int t = 0;
+    if (b < B) t = (int)(((int64_t)kv_seq(p.c, b).rows * p.group + kPRows - 1) / kPRows);
+    const int64_t at = scan(t, all);
+    if (b < B) tiles[b] = (int)(base + at);
+    base += all;
+  }
+  if (tid == 0) tiles[B] = (int)base;
+  __syncthreads();
+  const int pairs = tiles[B];
+  base = 0;
+  for (int i0 = 0; i0 < pairs; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int64_t u = 0;
+    int b = 0, rt = 0;
+    if (i < pairs) {
+      int lo = 0, hi = B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tiles[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      b = lo;
+      rt = i - tiles[b];
+      const KvSeq s = kv_seq(p.c, b);
+      int row_base, row_all, first_pos, last_pos;
+      prompt_rows(p, s, rt, row_base, row_all, first_pos, last_pos);
+      u = (int64_t)max(units_in(span_of<kPTok>(p, first_pos, last_pos, s.n)), 1) * p.c.heads;
+    }
+    const int64_t at = base + scan(u, all);
+    if (i < pairs) pp.list[i] = PromptItem{at, b, rt};
+    base += all;
+  }
+  if (tid == 0) {
+    pp.list[pairs] = PromptItem{base, 0, 0};
+    *pp.n_pairs = pairs;
+    *pp.total = base;
+  }
+}
+
+// the last pair whose first unit is <= u
+DEVI int pair_of(const PromptItem* list, int pairs, int64_t u) {
+  int lo = 0, hi = pairs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (list[mid].off <= u) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// shared memory, from a 128-byte boundary.  Operands are core matrices of 8 rows x 16 bytes (umma.cuh):
+// Q and K [dim / 8][row][8 dims]; V [token / 8][dim][8 tokens] with 16 bytes between its 8-dim groups,
+// so that the lanes that write it (4 dims apart) meet no bank twice.
+template <int D> struct PromptSmem {
+  static constexpr uint32_t kQTile = 128 * D * 2, kK = kPTok * D * 2;
+  static constexpr uint32_t kVGroup = 144, kVLbo = D / 8 * kVGroup, kV = kPTok / 8 * kVLbo;
+  static constexpr uint32_t q = 0, k = 2 * kQTile, v = k + 2 * kK, bars = v + 2 * kV;
+  static constexpr uint32_t bytes = bars + 256;
+};
+
+template <int D> constexpr int prompt_part() { return kPRows * (D + 2); }
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(PromptParams pp) {
+  using L = PromptSmem<D>;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ uint32_t s_tmem;
+  __shared__ uint32_t s_ref[2];  // largest key / value scale of the item, as bits
+  __shared__ int s_bad;
+  __shared__ volatile int s_abort;
+  const AttendParams& p = pp.a;
+  const KvView& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::bars);
+  uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *s_full = bar + 8, *p_ready = bar + 10,
+           *o_full = bar + 12, *drain = bar + 13;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + i, 4);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 4);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_ready + i, 4);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
+    fence_mbar_init();
+    s_abort = 0;
+  }
+  if (warp == 12) tmem_alloc<512>(&s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = s_tmem;
+  auto t_s = [&](int mt) { return tm + mt * 128; };
+  auto t_o = [&](int mt) { return tm + 256 + mt * D; };
+  pdl_wait();
+  pdl_launch_dependents();
+
+  auto wait = [&](uint64_t* b, uint32_t n) -> bool {  // the n-th completion (from 0) of a barrier
+    if (mbar_wait_bounded(b, n & 1, &s_abort)) return true;
+    set_error(p.err, DUPLEX_DEVERR_TIMEOUT);
+    return false;
+  };
+
+  const int pairs = *pp.n_pairs;
+  const int64_t total = *pp.total, share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1);
+  const int64_t u_begin = (int64_t)blockIdx.x * share, u_end = min(u_begin + share, total);
+  int64_t u = u_begin;
+  int pi = u < u_end ? pair_of(pp.list, pairs, u) : 0;
+  uint32_t n_tile = 0, n_s = 0, n_item = 0;  // tiles so far, this warp's tile's scores so far, items so far
+
+  while (u < u_end) {
+    while (pp.list[pi + 1].off <= u) ++pi;
+    const PromptItem item = pp.list[pi];
+    const KvSeq s = kv_seq(c, item.b);
+    int row_base, row_all, first_pos, last_pos;
+    prompt_rows(p, s, item.rt, row_base, row_all, first_pos, last_pos);
+    const Span sp = span_of<kPTok>(p, first_pos, last_pos, s.n);
+    const int units = units_in(sp), per = max(units, 1);
+    const int64_t r = u - item.off;
+    const int h = (int)(r / per), i0 = (int)(r - (int64_t)h * per);
+    const int i1 = (int)min((int64_t)per, i0 + (u_end - u));
+    const int n = min(i1, units) - i0;  // tiles of this piece (0: rows that see nothing)
+    const bool two = row_base + 128 < row_all;
+    const int lo_x = p.window ? first_pos - p.window + 1 : 0;  // the first token past the sinks that a row sees
+    auto base_of = [&](int i) { return i < sp.sink_units ? i * kPTok : sp.lo + (i - sp.sink_units) * kPTok; };
+    auto seen = [&](int k) { return k < sp.end && (k >= lo_x || k < p.sinks); };
+
+    // ---- the piece's largest scales, and whether all its block ids are good
+    if (tid < 2) s_ref[tid] = 0;
+    if (tid == 2) s_bad = 0;
+    __syncthreads();
+    {
+      const int per_tile = kPTok / c.block, cnt = n * per_tile;
+      float mk = 0.f, mv = 0.f;
+      for (int e = tid; e < cnt; e += kPThreads) {
+        const int i = e / per_tile, tok = base_of(i0 + i) + (e - i * per_tile) * c.block;
+        if (tok >= sp.end || (tok + c.block <= lo_x && tok >= p.sinks)) continue;
+        const int id = kv_block_at(c, item.b, tok / c.block, p.err);
+        if (id < 0) {
+          s_bad = 1;
+          continue;
+        }
+        mk = fmaxf(mk, __ldg(c.k_scale + (int64_t)id * c.heads + h));
+        mv = fmaxf(mv, __ldg(c.v_scale + (int64_t)id * c.heads + h));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        mk = fmaxf(mk, __shfl_xor_sync(~0u, mk, o));
+        mv = fmaxf(mv, __shfl_xor_sync(~0u, mv, o));
+      }
+      if (lane == 0) {
+        atomicMax(&s_ref[0], __float_as_uint(mk));
+        atomicMax(&s_ref[1], __float_as_uint(mv));
+      }
+    }
+    // ---- query rows to shared memory, as fp16 scaled by a power of two (kv_attend.cu: load_q)
+    float undo = 1.f;
+    if (warp < 8) {
+      const int rr = row_base + tid;
+      const bool live = rr < row_all;
+      const uint8_t* src = static_cast<const uint8_t*>(p.q) +
+                           2 * ((int64_t)(s.row0 + (live ? rr / p.group : 0)) * p.q_row +
+                                (int64_t)(h * p.group + (live ? rr % p.group : 0)) * p.q_head);
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = (&x.x)[j];
+          const float2 f = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(w) : act2<DUPLEX_DTYPE_BF16>(w);
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      const int ex = (int)(__float_as_uint(amax) >> 23) - 127;
+      const int up = (amax == 0.f || ex == 128) ? 0 : min(14 - ex, 126);
+      const float f = pow2f(up);
+      undo = pow2f(-up);
+      uint8_t* dst = sm + L::q + (tid >> 7) * L::kQTile + (tid & 127) * 16;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+        uint4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = (&x.x)[j];
+          const float2 a = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(w) : act2<DUPLEX_DTYPE_BF16>(w);
+          (&y.x)[j] = f2h(a.x * f, a.y * f);
+        }
+        *reinterpret_cast<uint4*>(dst + i * 128 * 16) = y;
+      }
+      fence_proxy_async_shared();
+    }
+    __syncthreads();
+    const float kref = fmaxf(__uint_as_float(s_ref[0]), pow2f(-126)), vref = fmaxf(__uint_as_float(s_ref[1]), pow2f(-126));
+    const bool bad = s_bad != 0;
+
+    if (warp >= 8 && warp < 12) {
+      // ------------------------------------------------ keys and values
+      constexpr int KC = D / 64, VG = D == 128 ? 4 : 2;  // 16-byte chunks a lane takes of a key; 8-token groups a lane takes
+      const int cw = warp - 8;
+      const int kt = lane & 7, kc = lane >> 3;                    // key: token of 8, chunk of 4
+      const int vl = D == 128 ? lane : lane & 15, vh = D == 128 ? 0 : lane >> 4;  // value: dims 4 vl .. + 3, group's half
+      uint4 kx[4][KC];
+      uint32_t vx[VG][8];
+      float kr[2], vr[2];  // scale ratios of the warp's two 16-token parts
+      int id[2], id_next[2];
+      auto ids = [&](int i, int (&to)[2]) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tok = base_of(i) + 32 * cw + 16 * e;
+          to[e] = -1;
+          if (i < i0 + n && tok < sp.end && !(tok + 15 < lo_x && tok >= p.sinks))
+            to[e] = kv_block_at(c, item.b, tok / c.block, nullptr);
+        }
+      };
+      auto row_at = [&](int e, int tok) {
+        return (((int64_t)id[e] * c.heads + h) * c.block + (tok & (c.block - 1))) * D;
+      };
+      auto load_k = [&](int i) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int tok = base_of(i) + 32 * cw + 8 * q + kt;
+#pragma unroll
+          for (int cc = 0; cc < KC; ++cc)
+            kx[q][cc] = id[q >> 1] < 0 ? make_uint4(0, 0, 0, 0)
+                                       : __ldg(reinterpret_cast<const uint4*>(c.k + row_at(q >> 1, tok) + 64 * cc + 16 * kc));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) kr[e] = id[e] < 0 ? 0.f : __ldg(c.k_scale + (int64_t)id[e] * c.heads + h);
+      };
+      auto load_v = [&](int i) {
+#pragma unroll
+        for (int q = 0; q < VG; ++q) {
+          const int e = D == 128 ? q >> 1 : q;
+          const int tok = base_of(i) + 32 * cw + (D == 128 ? 8 * q : 16 * q + 8 * vh);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            vx[q][j] = id[e] < 0 ? 0u : __ldg(reinterpret_cast<const uint32_t*>(c.v + row_at(e, tok + j)) + vl);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) vr[e] = id[e] < 0 ? 0.f : __ldg(c.v_scale + (int64_t)id[e] * c.heads + h);
+      };
+      auto mul = [](uint32_t x, __half2 f) {
+        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), f);
+        return *reinterpret_cast<const uint32_t*>(&y);
+      };
+      if (n > 0) {
+        ids(i0, id);
+        load_k(i0);
+        load_v(i0);
+      }
+      for (int j = 0; j < n; ++j) {
+        const uint32_t cnt = n_tile + j, slot = cnt & 1, use = cnt >> 1;
+        const int i = i0 + j, base = base_of(i);
+        const bool clean = base + kPTok <= sp.end && (base >= lo_x || base + kPTok <= p.sinks);
+        ids(i + 1, id_next);
+        if (use > 0 && !wait(k_empty + slot, use - 1)) break;
+        uint8_t* ks = sm + L::k + slot * L::kK;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int t = 32 * cw + 8 * q + kt;
+          const __half2 f = __float2half2_rn(kr[q >> 1] / kref);
+          const bool zero = !clean && !seen(base + t);
+#pragma unroll
+          for (int cc = 0; cc < KC; ++cc) {
+            uint4 x = kx[q][cc];
+            if (zero) x = make_uint4(0, 0, 0, 0);
+            uint8_t* dst = ks + (8 * cc + 2 * kc) * kPTok * 16 + t * 16;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(mul(KvFmt<FMT>::lo(x.x), f), mul(KvFmt<FMT>::hi(x.x), f),
+                                                        mul(KvFmt<FMT>::lo(x.y), f), mul(KvFmt<FMT>::hi(x.y), f));
+            *reinterpret_cast<uint4*>(dst + kPTok * 16) = make_uint4(mul(KvFmt<FMT>::lo(x.z), f), mul(KvFmt<FMT>::hi(x.z), f),
+                                                                     mul(KvFmt<FMT>::lo(x.w), f), mul(KvFmt<FMT>::hi(x.w), f));
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full + slot);
+        id[0] = id_next[0];
+        id[1] = id_next[1];
+        if (j + 1 < n) load_k(i + 1);
+        if (use > 0 && !wait(v_empty + slot, use - 1)) break;
+        uint8_t* vs = sm + L::v + slot * L::kV;
+#pragma unroll
+        for (int q = 0; q < VG; ++q) {
+          const int t0 = 32 * cw + (D == 128 ? 8 * q : 16 * q + 8 * vh);
+          const __half2 f = __float2half2_rn(vr[D == 128 ? q >> 1 : q] / vref);
+          if (!clean) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (!seen(base + t0 + k)) vx[q][k] = 0;
+          }
+          uint4 o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // token pairs: their bytes interleaved, then fp16 pairs per dim
+            const uint32_t a = __byte_perm(vx[q][2 * k], vx[q][2 * k + 1], 0x5140u);
+            const uint32_t b = __byte_perm(vx[q][2 * k], vx[q][2 * k + 1], 0x7362u);
+            (&o[0].x)[k] = mul(KvFmt<FMT>::lo(a), f);
+            (&o[1].x)[k] = mul(KvFmt<FMT>::hi(a), f);
+            (&o[2].x)[k] = mul(KvFmt<FMT>::lo(b), f);
+            (&o[3].x)[k] = mul(KvFmt<FMT>::hi(b), f);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int d = 4 * vl + k;
+            *reinterpret_cast<uint4*>(vs + (t0 >> 3) * L::kVLbo + (d >> 3) * L::kVGroup + (d & 7) * 16) = o[k];
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full + slot);
+        if (j + 1 < n) load_v(i + 1);
+      }
+    } else if (warp == 12) {
+      // ------------------------------------------------ products
+      if (lane == 0 && n > 0) {
+        constexpr uint32_t id_qk = idesc_f16(0, 128, kPTok), id_pv = idesc_f16(0, 128, D);
+        const uint32_t sq = smem_u32(sm + L::q), sk = smem_u32(sm + L::k), sv = smem_u32(sm + L::v);
+        auto qk = [&](int mt, uint32_t slot) {
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+            umma_ss(t_s(mt), smem_desc_kmajor(sq + mt * L::kQTile + x * 4096, 2048, 128),
+                    smem_desc_kmajor(sk + slot * L::kK + x * 4096, 2048, 128), id_qk, x != 0);
+          umma_commit(s_full + mt);
+        };
+        auto pv = [&](int mt, uint32_t slot, bool more) {
+#pragma unroll
+          for (int x = 0; x < kPTok / 16; ++x)
+            umma_ts(t_o(mt), t_s(mt) + 8 * x, smem_desc_kmajor(sv + slot * L::kV + 2 * x * L::kVLbo, L::kVLbo, L::kVGroup),
+                    id_pv, more || x != 0);
+        };
+        uint32_t n0 = n_s;
+        bool ok = wait(k_full + (n_tile & 1), n_tile >> 1);
+        if (ok) {
+          tc_fence_after();
+          qk(0, n_tile & 1);
+          if (two) qk(1, n_tile & 1);
+          umma_commit(k_empty + (n_tile & 1));
+        }
+        for (int j = 0; ok && j < n; ++j) {
+          const uint32_t cnt = n_tile + j, slot = cnt & 1, nslot = slot ^ 1;
+          if (!(ok = wait(v_full + slot, cnt >> 1) && wait(p_ready, n0 + j))) break;
+          tc_fence_after();
+          pv(0, slot, j > 0);
+          if (j + 1 < n) {
+            if (!(ok = wait(k_full + nslot, (cnt + 1) >> 1))) break;
+            tc_fence_after();
+            qk(0, nslot);
+          }
+          if (two) {
+            if (!(ok = wait(p_ready + 1, n_item + j))) break;  // n_item counts tile 1's scores here
+            tc_fence_after();
+            pv(1, slot, j > 0);
+          }
+          umma_commit(v_empty + slot);
+          if (j + 1 < n) {
+            if (two) qk(1, nslot);
+            umma_commit(k_empty + nslot);
+          }
+        }
+        if (ok) umma_commit(o_full);
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------ softmax: this thread's row
+      const int mt = warp >> 2, rr = row_base + tid;
+      const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
+      const bool live = rr < row_all;
+      const int pos = live ? s.n - s.rows + rr / p.group : -1;
+      const int wlo = p.window ? pos - p.window : -1;  // tokens k > wlo, or k < sinks
+      const int t_first = s.n - s.rows + min(row_base + mt * 128, row_all - 1) / p.group;  // positions of the tile's rows
+      const int t_last = s.n - s.rows + (min(row_base + mt * 128 + 128, row_all) - 1) / p.group;
+      const bool ragged = row_base + mt * 128 + 128 > row_all;
+      const float cs = undo * p.scale_log2 * kref;
+      float m = -INFINITY, l = 0.f;
+      bool ok = mt == 0 || two;
+      const uint32_t ts = t_s(mt) + lane_at, to = t_o(mt) + lane_at;
+      for (int j = 0; ok && j < n; ++j) {
+        const int base = base_of(i0 + j);
+        const bool masked = bad || ragged || base + kPTok - 1 > t_first ||
+                            (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
+        if (!(ok = __all_sync(~0u, wait(s_full + mt, n_s + j)))) break;
+        tc_fence_after();
+        uint32_t P[64];
+        float ls, mx;
+        for (int pass = 0; pass < 2; ++pass) {
+          const float from = m == -INFINITY ? 0.f : m, add = kShift - from;
+          ls = 0.f;
+          mx = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[32];
+            __syncwarp();
+            tmem_ld32(ts + 32 * q, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), cs, add));
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const int k = base + 32 * q + e;
+                bool see = k <= pos && (k > wlo || k < p.sinks);
+                if (bad && see) see = (unsigned)c.table[(int64_t)item.b * c.width + k / c.block] < (unsigned)c.n_blocks;
+                if (!see) v[e] = __float_as_uint(-INFINITY);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float a = __uint_as_float(v[e]), b = __uint_as_float(v[e + 1]);
+              mx = fmaxf(mx, fmaxf(a, b));
+              const float x = ex2(a), y = ex2(b);
+              ls += x;
+              ls += y;
+              P[16 * q + e / 2] = f2h(x, y);
+            }
+          }
+          const bool grow = mx > (m == -INFINITY ? -INFINITY : kShift + kSlack);
+          if (pass || !__any_sync(~0u, grow)) break;
+          const float to_m = grow ? mx - kShift + from : m;
+          const float f = to_m == m ? 1.f : ex2(m - to_m);
+          m = to_m;
+          l *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t v[32];
+              tmem_ld32(to + 32 * q, v);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              tmem_st32(to + 32 * q, v);
+            }
+          }
+        }
+        __syncwarp();
+        l += ls;
+        tmem_st32(ts, P);
+        tmem_st32(ts + 32, P + 32);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready + mt);
+      }
+      // ---- the row's result
+      const bool have = ok && n > 0 && __all_sync(~0u, wait(o_full, n_item));
+      if (have) tc_fence_after();
+      if (ok && (have || n <= 0)) {
+        const bool whole = i0 == 0 && i1 == per;
+        const float inv = whole ? (l == 0.f ? 0.f : vref / l) : vref;
+        float* part = p.part + (2 * (int64_t)blockIdx.x + (u == u_begin ? 0 : 1)) * prompt_part<D>();
+        const int64_t at = live ? (int64_t)(s.row0 + rr / p.group) * p.heads + h * p.group + rr % p.group : 0;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t v[32];
+          __syncwarp();
+          if (have) {
+            tmem_ld32(to + 32 * q, v);
+            tc_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            if (!live) break;
+            const float4 o = make_float4(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv,
+                                         __uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
+            if (whole) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + 32 * q + e)) = pack4(p.act, o);
+            else *reinterpret_cast<float4*>(part + tid * D + 32 * q + e) = o;
+          }
+        }
+        if (live) {
+          if (whole) p.lse[at] = lse_of(m, l);
+          else {
+            part[kPRows * D + tid] = m;
+            part[kPRows * D + kPRows + tid] = l;
+          }
+        }
+        tc_fence_before();
+      }
+    }
+    __syncthreads();
+    if (s_abort) break;
+    tc_fence_after();
+    // counters of the barriers' completions: each role keeps the ones it waits on
+    n_tile += n;
+    if (warp < 4) n_s += n;
+    else if (warp < 8) n_s += two ? n : 0;
+    else if (warp == 12) {
+      n_s += n;                   // p_ready[0]
+      n_item += two ? n : 0;      // p_ready[1]
+    }
+    if (warp < 8) n_item += n > 0 ? 1 : 0;  // o_full
+    u += i1 - i0;
+  }
+
+  // no product may still be running when tensor memory goes
+  if (warp == 12) {
+    if (lane == 0) {
+      umma_commit(drain);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(drain, 0))
+        if (clock64() - t0 > 200000000LL) {
+          set_error(p.err, DUPLEX_DEVERR_TIMEOUT);
+          break;
+        }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == 12) tmem_dealloc<512>(tm);
+}
+
+// CTA j joins the item that crosses the boundary between pieces j and j + 1, if that is its first one.
+constexpr int kJoinThreads = 512;
+
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptParams pp, int ctas) {
+  const AttendParams& p = pp.a;
+  pdl_wait();
+  const int64_t total = *pp.total, share = max((total + ctas - 1) / ctas, (int64_t)1);
+  const int64_t u = (int64_t)(blockIdx.x + 1) * share;
+  if (u >= total) return;
+  const int pi = pair_of(pp.list, *pp.n_pairs, u);
+  const PromptItem item = pp.list[pi];
+  const int64_t per = (pp.list[pi + 1].off - item.off) / p.c.heads;
+  const int h = (int)((u - item.off) / per);
+  const int64_t begin = item.off + h * per, last = begin + per - 1;
+  if (begin == u || begin / share != blockIdx.x) return;
+  const int c0 = blockIdx.x, c1 = (int)(last / share);
+  const KvSeq s = kv_seq(p.c, item.b);
+  const int row_all = s.rows * p.group;
+  for (int e = threadIdx.x; e < kPRows * D / 4; e += kJoinThreads) {
+    const int rr = e / (D / 4), d = (e - rr * (D / 4)) * 4, r2 = item.rt * kPRows + rr;
+    if (r2 >= row_all) continue;
+    auto slot = [&](int j) {
+      const int k = (j == c0 && begin != (int64_t)c0 * share) ? 1 : 0;
+      return p.part + (2 * (int64_t)j + k) * prompt_part<D>();
+    };
+    float M = -INFINITY;
+    for (int j = c0; j <= c1; ++j) M = fmaxf(M, __ldcg(slot(j) + kPRows * D + rr));
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int j = c0; j <= c1; ++j) {
+      const float* ps = slot(j);
+      const float mj = __ldcg(ps + kPRows * D + rr), f = mj == M ? 1.f : ex2(mj - M);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(ps + rr * D + d));
+      l += __ldcg(ps + kPRows * D + kPRows + rr) * f;
+      o.x += x.x * f;
+      o.y += x.y * f;
+      o.z += x.z * f;
+      o.w += x.w * f;
+    }
+    const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
+        pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (d == 0) p.lse[at] = lse_of(M, l);
+  }
+}
+
+bool kv_prompt_takes(const KvView& c, int group) { return (int64_t)c.n_rows * group >= 128ll * c.batch; }
+
+static int64_t max_pairs(const KvView& c, int group) { return (int64_t)c.n_rows * group / kPRows + c.batch; }
+
+static size_t list_bytes(const KvView& c, int group) {
+  return (size_t)((max_pairs(c, group) + 2) * (int64_t)sizeof(PromptItem) + 127) / 128 * 128;
+}
+
+size_t kv_prompt_workspace(const KvView& c, int group) {
+  return list_bytes(c, group) + (size_t)2 * kPMaxCtas * (c.dim == 128 ? prompt_part<128>() : prompt_part<64>()) * 4;
+}
+
+template <int D, int FMT>
+static int run(const PromptParams& pp, int ctas, cudaStream_t st) {
+  constexpr size_t smem = PromptSmem<D>::bytes;
+  const KvView& c = pp.a.c;
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_prompt_kernel<D, FMT>), (int)smem)) return rc;
+  kv_prompt_plan_kernel<<<1, kPlanThreads, sizeof(int) * (c.batch + 1), st>>>(pp);
+  if (int rc = record_cuda(cudaGetLastError())) return rc;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kPThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (int rc = record_cuda(cudaLaunchKernelEx(&cfg, kv_prompt_kernel<D, FMT>, pp))) return rc;
+  if (ctas < 2) return DUPLEX_OK;
+  cfg.gridDim = dim3(ctas - 1);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  return record_cuda(cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<D>, pp, ctas));
+}
+
+int kv_prompt_run(const AttendParams& a, void* workspace, cudaStream_t st) {
+  PromptParams pp{a, nullptr, nullptr, nullptr};
+  const size_t list = list_bytes(a.c, a.group);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  pp.list = reinterpret_cast<PromptItem*>(ws + sizeof(PromptItem));
+  pp.total = reinterpret_cast<int64_t*>(ws);
+  pp.n_pairs = reinterpret_cast<int*>(ws + 8);
+  pp.a.part = reinterpret_cast<float*>(ws + list);
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  const int64_t units = max_pairs(a.c, a.group) * a.c.heads * (((int64_t)a.c.width * a.c.block + kPTok - 1) / kPTok);
+  const int ctas = (int)std::min({(int64_t)sms, (int64_t)kPMaxCtas, units});
+  if (a.c.dim == 128)
+    return a.c.format == DUPLEX_KV_E4M3 ? run<128, DUPLEX_KV_E4M3>(pp, ctas, st) : run<128, DUPLEX_KV_INT8>(pp, ctas, st);
+  return a.c.format == DUPLEX_KV_E4M3 ? run<64, DUPLEX_KV_E4M3>(pp, ctas, st) : run<64, DUPLEX_KV_INT8>(pp, ctas, st);
+}
+
+}  // namespace duplex
