@@ -27,7 +27,7 @@
 
 namespace duplex {
 
-constexpr int kPTok = 128, kPRows = 256, kPThreads = 13 * 32, kPMaxCtas = 160;
+constexpr int kPTok = 128, kPRows = 256, kPThreads = 512, kPMaxCtas = 160;
 
 struct PromptItem {
   int64_t off;  // units before it (of all heads)
@@ -51,6 +51,9 @@ DEVI void prompt_rows(const AttendParams& p, const KvSeq& s, int rt, int& row_ba
 DEVI int units_in(const Span& sp) {
   return sp.sink_units + (sp.end > sp.lo ? (sp.end - sp.lo + kPTok - 1) / kPTok : 0);
 }
+
+// An item costs as much as its tiles and kPOver more (query rows in, results out, the pipeline's ends).
+constexpr int kPOver = 2;
 
 // The list of (sequence, row tile) pairs with their units, by one CTA.
 constexpr int kPlanThreads = 1024;
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
       const KvSeq s = kv_seq(p.c, b);
       int row_base, row_all, first_pos, last_pos;
       prompt_rows(p, s, rt, row_base, row_all, first_pos, last_pos);
-      u = (int64_t)max(units_in(span_of<kPTok>(p, first_pos, last_pos, s.n)), 1) * p.c.heads;
+      u = (int64_t)(units_in(span_of<kPTok>(p, first_pos, last_pos, s.n)) + kPOver) * p.c.heads;
     }
     const int64_t at = base + scan(u, all);
     if (i < pairs) pp.list[i] = PromptItem{at, b, rt};
@@ -131,24 +134,65 @@ DEVI int pair_of(const PromptItem* list, int pairs, int64_t u) {
   return lo;
 }
 
-// shared memory, from a 128-byte boundary.  Operands are core matrices of 8 rows x 16 bytes (umma.cuh):
-// Q and K [dim / 8][row][8 dims]; V [token / 8][dim][8 tokens] with 16 bytes between its 8-dim groups,
-// so that the lanes that write it (4 dims apart) meet no bank twice.
+// shared memory, from a 1024-byte boundary: operands in the 128-byte swizzle (umma.cuh).  Q and K
+// [dim / 64][row][64 dims] are K-major; V [dim / 64][token][64 dims], the same layout, is MN-major.
 template <int D> struct PromptSmem {
-  static constexpr uint32_t kQTile = 128 * D * 2, kK = kPTok * D * 2;
-  static constexpr uint32_t kVGroup = 144, kVLbo = D / 8 * kVGroup, kV = kPTok / 8 * kVLbo;
-  static constexpr uint32_t q = 0, k = 2 * kQTile, v = k + 2 * kK, bars = v + 2 * kV;
-  static constexpr uint32_t bytes = bars + 256;
+  static constexpr uint32_t kHalf = 128 * 128, kTile = D / 64 * kHalf;
+  static constexpr uint32_t q = 0, k = 2 * kTile, v = k + 2 * kTile, undo = v + 2 * kTile, bars = undo + kPRows * 4;
+  static constexpr uint32_t bytes = bars + 256 + 1024;
 };
+
+// 16-byte chunk c of a row
+DEVI uint32_t sw128(int row, int c) { return (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)); }
 
 template <int D> constexpr int prompt_part() { return kPRows * (D + 2); }
 
+// The piece of an item that a CTA works on next: its list position and what follows from it, found
+// alike by every warp.
+struct Piece {
+  KvSeq s;
+  Span sp;
+  int b, h, row_base, row_all, first_pos, last_pos, lo_x;
+  int i0, n, len;    // its first tile, its tiles (0: rows that see nothing), its units
+  bool whole, two;   // the item's only piece; rows in the second tile
+
+  DEVI int base_of(int i) const { return i < sp.sink_units ? i * kPTok : sp.lo + (i - sp.sink_units) * kPTok; }
+  DEVI bool seen(const AttendParams& p, int k) const { return k < sp.end && (k >= lo_x || k < p.sinks); }
+};
+
+DEVI void find_piece(const PromptParams& pp, int64_t u, int64_t u_end, int& pi, Piece& x) {
+  const AttendParams& p = pp.a;
+  while (pp.list[pi + 1].off <= u) ++pi;
+  const PromptItem item = pp.list[pi];
+  x.b = item.b;
+  x.s = kv_seq(p.c, item.b);
+  prompt_rows(p, x.s, item.rt, x.row_base, x.row_all, x.first_pos, x.last_pos);
+  x.sp = span_of<kPTok>(p, x.first_pos, x.last_pos, x.s.n);
+  const int per = units_in(x.sp) + kPOver;
+  const int64_t r = u - item.off;
+  x.h = (int)(r / per);
+  const int u0 = (int)(r - (int64_t)x.h * per), u1 = (int)min((int64_t)per, u0 + (u_end - u));
+  x.len = u1 - u0;
+  x.whole = u0 == 0 && u1 == per;
+  x.i0 = max(u0 - kPOver, 0);
+  x.n = max(u1 - kPOver, 0) - x.i0;
+  x.two = x.row_base + 128 < x.row_all;
+  x.lo_x = p.window ? x.first_pos - p.window + 1 : 0;  // the first token past the sinks that a row sees
+}
+
+// Registers: 512 threads start with 128 each; the softmax warps take what the others leave
+// (256 * 160 + 128 * 112 + 128 * 72 < 512 * 128).
+constexpr int kRegSoftmax = 160, kRegConvert = 112, kRegMma = 72;
+constexpr int kWorkers = 13 * 32;  // the fourth warp group's other warps only give their registers
+
 template <int D, int FMT>
-__global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(PromptParams pp) {
+__global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_constant__ PromptParams pp) {
   using L = PromptSmem<D>;
-  extern __shared__ __align__(128) uint8_t sm[];
+  extern __shared__ uint8_t dyn[];
+  uint8_t* const sm = dyn + (1024 - smem_u32(dyn) % 1024) % 1024;
+  float* const s_undo = reinterpret_cast<float*>(sm + L::undo);
   __shared__ uint32_t s_tmem;
-  __shared__ uint32_t s_ref[2];  // largest key / value scale of the item, as bits
+  __shared__ uint32_t s_ref[2];  // largest key / value scale of the piece, as bits
   __shared__ int s_bad;
   __shared__ volatile int s_abort;
   const AttendParams& p = pp.a;
@@ -170,6 +214,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(PromptParams pp
     mbar_init(drain, 1);
     fence_mbar_init();
     s_abort = 0;
+    s_ref[0] = s_ref[1] = 0;
+    s_bad = 0;
   }
   if (warp == 12) tmem_alloc<512>(&s_tmem);
   tc_fence_before();
@@ -192,36 +238,30 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(PromptParams pp
   const int64_t u_begin = (int64_t)blockIdx.x * share, u_end = min(u_begin + share, total);
   int64_t u = u_begin;
   int pi = u < u_end ? pair_of(pp.list, pairs, u) : 0;
-  uint32_t n_tile = 0, n_s = 0, n_item = 0;  // tiles so far, this warp's tile's scores so far, items so far
+  Piece x;
+  // each role walks the pieces, between the same two barriers a piece: query rows and scales are
+  // there; the piece is done
 
-  while (u < u_end) {
-    while (pp.list[pi + 1].off <= u) ++pi;
-    const PromptItem item = pp.list[pi];
-    const KvSeq s = kv_seq(c, item.b);
-    int row_base, row_all, first_pos, last_pos;
-    prompt_rows(p, s, item.rt, row_base, row_all, first_pos, last_pos);
-    const Span sp = span_of<kPTok>(p, first_pos, last_pos, s.n);
-    const int units = units_in(sp), per = max(units, 1);
-    const int64_t r = u - item.off;
-    const int h = (int)(r / per), i0 = (int)(r - (int64_t)h * per);
-    const int i1 = (int)min((int64_t)per, i0 + (u_end - u));
-    const int n = min(i1, units) - i0;  // tiles of this piece (0: rows that see nothing)
-    const bool two = row_base + 128 < row_all;
-    const int lo_x = p.window ? first_pos - p.window + 1 : 0;  // the first token past the sinks that a row sees
-    auto base_of = [&](int i) { return i < sp.sink_units ? i * kPTok : sp.lo + (i - sp.sink_units) * kPTok; };
-    auto seen = [&](int k) { return k < sp.end && (k >= lo_x || k < p.sinks); };
-
-    // ---- the piece's largest scales, and whether all its block ids are good
-    if (tid < 2) s_ref[tid] = 0;
-    if (tid == 2) s_bad = 0;
-    __syncthreads();
-    {
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax: a thread's row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegSoftmax));
+    const int mt = warp >> 2;
+    const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
+    const uint32_t ts = t_s(mt) + lane_at, to = t_o(mt) + lane_at;
+    uint32_t n_s = 0, n_o = 0;  // completions of s_full[mt], o_full so far
+    while (u < u_end) {
+      find_piece(pp, u, u_end, pi, x);
+      const int n = x.n, h = x.h, row_base = x.row_base, row_all = x.row_all;
+      const KvSeq& s = x.s;
+      const Span& sp = x.sp;
+      // the piece's largest scales, and whether all its block ids are good
+      {
       const int per_tile = kPTok / c.block, cnt = n * per_tile;
       float mk = 0.f, mv = 0.f;
-      for (int e = tid; e < cnt; e += kPThreads) {
-        const int i = e / per_tile, tok = base_of(i0 + i) + (e - i * per_tile) * c.block;
-        if (tok >= sp.end || (tok + c.block <= lo_x && tok >= p.sinks)) continue;
-        const int id = kv_block_at(c, item.b, tok / c.block, p.err);
+      for (int e = tid; e < cnt; e += 256) {
+        const int i = e / per_tile, tok = x.base_of(x.i0 + i) + (e - i * per_tile) * c.block;
+        if (tok >= sp.end || (tok + c.block <= x.lo_x && tok >= p.sinks)) continue;
+        const int id = kv_block_at(c, x.b, tok / c.block, p.err);
         if (id < 0) {
           s_bad = 1;
           continue;
@@ -239,302 +279,147 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(PromptParams pp
         atomicMax(&s_ref[1], __float_as_uint(mv));
       }
     }
-    // ---- query rows to shared memory, as fp16 scaled by a power of two (kv_attend.cu: load_q)
-    float undo = 1.f;
-    if (warp < 8) {
+      // query rows to shared memory, as fp16 scaled by a power of two (kv_attend.cu: load_q): a warp
+      // takes 8 rows at a time, 4 lanes a row
+      {
+        uint4 raw[4][D / 32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r2 = row_base + 32 * warp + 8 * i + (lane & 7);
+          const uint8_t* src = static_cast<const uint8_t*>(p.q) + 16 * (lane >> 3);
+          const bool in = r2 < row_all;
+          if (in) src += 2 * ((int64_t)(s.row0 + r2 / p.group) * p.q_row + (int64_t)(h * p.group + r2 % p.group) * p.q_head);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e)
+            raw[i][e] = in ? __ldg(reinterpret_cast<const uint4*>(src + 64 * e)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = (32 * warp + 8 * i + (lane & 7)) & 127;
+          float amax = 0.f;
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t y = (&raw[i][e].x)[w];
+              const float2 f = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(y) : act2<DUPLEX_DTYPE_BF16>(y);
+              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 8));
+          amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 16));
+          const int ex = (int)(__float_as_uint(amax) >> 23) - 127;
+          const int up = (amax == 0.f || ex == 128) ? 0 : min(14 - ex, 126);
+          const float f = p.scale_log2 < 0.f ? -pow2f(up) : pow2f(up);  // its sign goes with the row
+          if (lane < 8) s_undo[32 * warp + 8 * i + lane] = pow2f(-up);
+          uint8_t* dst = sm + L::q + (warp >> 2) * L::kTile;
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) {
+            uint4 y;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t z = (&raw[i][e].x)[w];
+              const float2 a = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(z) : act2<DUPLEX_DTYPE_BF16>(z);
+              (&y.x)[w] = f2h(a.x * f, a.y * f);
+            }
+            const int ch = 4 * e + (lane >> 3);  // of the row's D / 8
+            *reinterpret_cast<uint4*>(dst + (ch >> 3) * L::kHalf + sw128(row, ch & 7)) = y;
+          }
+        }
+      }
       const int rr = row_base + tid;
       const bool live = rr < row_all;
-      const uint8_t* src = static_cast<const uint8_t*>(p.q) +
-                           2 * ((int64_t)(s.row0 + (live ? rr / p.group : 0)) * p.q_row +
-                                (int64_t)(h * p.group + (live ? rr % p.group : 0)) * p.q_head);
-      float amax = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w = (&x.x)[j];
-          const float2 f = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(w) : act2<DUPLEX_DTYPE_BF16>(w);
-          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-      }
-      const int ex = (int)(__float_as_uint(amax) >> 23) - 127;
-      const int up = (amax == 0.f || ex == 128) ? 0 : min(14 - ex, 126);
-      const float f = pow2f(up);
-      undo = pow2f(-up);
-      uint8_t* dst = sm + L::q + (tid >> 7) * L::kQTile + (tid & 127) * 16;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-        uint4 y;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w = (&x.x)[j];
-          const float2 a = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(w) : act2<DUPLEX_DTYPE_BF16>(w);
-          (&y.x)[j] = f2h(a.x * f, a.y * f);
-        }
-        *reinterpret_cast<uint4*>(dst + i * 128 * 16) = y;
-      }
       fence_proxy_async_shared();
-    }
-    __syncthreads();
-    const float kref = fmaxf(__uint_as_float(s_ref[0]), pow2f(-126)), vref = fmaxf(__uint_as_float(s_ref[1]), pow2f(-126));
-    const bool bad = s_bad != 0;
-
-    if (warp >= 8 && warp < 12) {
-      // ------------------------------------------------ keys and values
-      constexpr int KC = D / 64, VG = D == 128 ? 4 : 2;  // 16-byte chunks a lane takes of a key; 8-token groups a lane takes
-      const int cw = warp - 8;
-      const int kt = lane & 7, kc = lane >> 3;                    // key: token of 8, chunk of 4
-      const int vl = D == 128 ? lane : lane & 15, vh = D == 128 ? 0 : lane >> 4;  // value: dims 4 vl .. + 3, group's half
-      uint4 kx[4][KC];
-      uint32_t vx[VG][8];
-      float kr[2], vr[2];  // scale ratios of the warp's two 16-token parts
-      int id[2], id_next[2];
-      auto ids = [&](int i, int (&to)[2]) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int tok = base_of(i) + 32 * cw + 16 * e;
-          to[e] = -1;
-          if (i < i0 + n && tok < sp.end && !(tok + 15 < lo_x && tok >= p.sinks))
-            to[e] = kv_block_at(c, item.b, tok / c.block, nullptr);
-        }
-      };
-      auto row_at = [&](int e, int tok) {
-        return (((int64_t)id[e] * c.heads + h) * c.block + (tok & (c.block - 1))) * D;
-      };
-      auto load_k = [&](int i) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int tok = base_of(i) + 32 * cw + 8 * q + kt;
-#pragma unroll
-          for (int cc = 0; cc < KC; ++cc)
-            kx[q][cc] = id[q >> 1] < 0 ? make_uint4(0, 0, 0, 0)
-                                       : __ldg(reinterpret_cast<const uint4*>(c.k + row_at(q >> 1, tok) + 64 * cc + 16 * kc));
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) kr[e] = id[e] < 0 ? 0.f : __ldg(c.k_scale + (int64_t)id[e] * c.heads + h);
-      };
-      auto load_v = [&](int i) {
-#pragma unroll
-        for (int q = 0; q < VG; ++q) {
-          const int e = D == 128 ? q >> 1 : q;
-          const int tok = base_of(i) + 32 * cw + (D == 128 ? 8 * q : 16 * q + 8 * vh);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            vx[q][j] = id[e] < 0 ? 0u : __ldg(reinterpret_cast<const uint32_t*>(c.v + row_at(e, tok + j)) + vl);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) vr[e] = id[e] < 0 ? 0.f : __ldg(c.v_scale + (int64_t)id[e] * c.heads + h);
-      };
-      auto mul = [](uint32_t x, __half2 f) {
-        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), f);
-        return *reinterpret_cast<const uint32_t*>(&y);
-      };
-      if (n > 0) {
-        ids(i0, id);
-        load_k(i0);
-        load_v(i0);
-      }
-      for (int j = 0; j < n; ++j) {
-        const uint32_t cnt = n_tile + j, slot = cnt & 1, use = cnt >> 1;
-        const int i = i0 + j, base = base_of(i);
-        const bool clean = base + kPTok <= sp.end && (base >= lo_x || base + kPTok <= p.sinks);
-        ids(i + 1, id_next);
-        if (use > 0 && !wait(k_empty + slot, use - 1)) break;
-        uint8_t* ks = sm + L::k + slot * L::kK;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int t = 32 * cw + 8 * q + kt;
-          const __half2 f = __float2half2_rn(kr[q >> 1] / kref);
-          const bool zero = !clean && !seen(base + t);
-#pragma unroll
-          for (int cc = 0; cc < KC; ++cc) {
-            uint4 x = kx[q][cc];
-            if (zero) x = make_uint4(0, 0, 0, 0);
-            uint8_t* dst = ks + (8 * cc + 2 * kc) * kPTok * 16 + t * 16;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(mul(KvFmt<FMT>::lo(x.x), f), mul(KvFmt<FMT>::hi(x.x), f),
-                                                        mul(KvFmt<FMT>::lo(x.y), f), mul(KvFmt<FMT>::hi(x.y), f));
-            *reinterpret_cast<uint4*>(dst + kPTok * 16) = make_uint4(mul(KvFmt<FMT>::lo(x.z), f), mul(KvFmt<FMT>::hi(x.z), f),
-                                                                     mul(KvFmt<FMT>::lo(x.w), f), mul(KvFmt<FMT>::hi(x.w), f));
-          }
-        }
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(k_full + slot);
-        id[0] = id_next[0];
-        id[1] = id_next[1];
-        if (j + 1 < n) load_k(i + 1);
-        if (use > 0 && !wait(v_empty + slot, use - 1)) break;
-        uint8_t* vs = sm + L::v + slot * L::kV;
-#pragma unroll
-        for (int q = 0; q < VG; ++q) {
-          const int t0 = 32 * cw + (D == 128 ? 8 * q : 16 * q + 8 * vh);
-          const __half2 f = __float2half2_rn(vr[D == 128 ? q >> 1 : q] / vref);
-          if (!clean) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (!seen(base + t0 + k)) vx[q][k] = 0;
-          }
-          uint4 o[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {  // token pairs: their bytes interleaved, then fp16 pairs per dim
-            const uint32_t a = __byte_perm(vx[q][2 * k], vx[q][2 * k + 1], 0x5140u);
-            const uint32_t b = __byte_perm(vx[q][2 * k], vx[q][2 * k + 1], 0x7362u);
-            (&o[0].x)[k] = mul(KvFmt<FMT>::lo(a), f);
-            (&o[1].x)[k] = mul(KvFmt<FMT>::hi(a), f);
-            (&o[2].x)[k] = mul(KvFmt<FMT>::lo(b), f);
-            (&o[3].x)[k] = mul(KvFmt<FMT>::hi(b), f);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int d = 4 * vl + k;
-            *reinterpret_cast<uint4*>(vs + (t0 >> 3) * L::kVLbo + (d >> 3) * L::kVGroup + (d & 7) * 16) = o[k];
-          }
-        }
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(v_full + slot);
-        if (j + 1 < n) load_v(i + 1);
-      }
-    } else if (warp == 12) {
-      // ------------------------------------------------ products
-      if (lane == 0 && n > 0) {
-        constexpr uint32_t id_qk = idesc_f16(0, 128, kPTok), id_pv = idesc_f16(0, 128, D);
-        const uint32_t sq = smem_u32(sm + L::q), sk = smem_u32(sm + L::k), sv = smem_u32(sm + L::v);
-        auto qk = [&](int mt, uint32_t slot) {
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x)
-            umma_ss(t_s(mt), smem_desc_kmajor(sq + mt * L::kQTile + x * 4096, 2048, 128),
-                    smem_desc_kmajor(sk + slot * L::kK + x * 4096, 2048, 128), id_qk, x != 0);
-          umma_commit(s_full + mt);
-        };
-        auto pv = [&](int mt, uint32_t slot, bool more) {
-#pragma unroll
-          for (int x = 0; x < kPTok / 16; ++x)
-            umma_ts(t_o(mt), t_s(mt) + 8 * x, smem_desc_kmajor(sv + slot * L::kV + 2 * x * L::kVLbo, L::kVLbo, L::kVGroup),
-                    id_pv, more || x != 0);
-        };
-        uint32_t n0 = n_s;
-        bool ok = wait(k_full + (n_tile & 1), n_tile >> 1);
-        if (ok) {
-          tc_fence_after();
-          qk(0, n_tile & 1);
-          if (two) qk(1, n_tile & 1);
-          umma_commit(k_empty + (n_tile & 1));
-        }
-        for (int j = 0; ok && j < n; ++j) {
-          const uint32_t cnt = n_tile + j, slot = cnt & 1, nslot = slot ^ 1;
-          if (!(ok = wait(v_full + slot, cnt >> 1) && wait(p_ready, n0 + j))) break;
-          tc_fence_after();
-          pv(0, slot, j > 0);
-          if (j + 1 < n) {
-            if (!(ok = wait(k_full + nslot, (cnt + 1) >> 1))) break;
-            tc_fence_after();
-            qk(0, nslot);
-          }
-          if (two) {
-            if (!(ok = wait(p_ready + 1, n_item + j))) break;  // n_item counts tile 1's scores here
-            tc_fence_after();
-            pv(1, slot, j > 0);
-          }
-          umma_commit(v_empty + slot);
-          if (j + 1 < n) {
-            if (two) qk(1, nslot);
-            umma_commit(k_empty + nslot);
-          }
-        }
-        if (ok) umma_commit(o_full);
-      }
-      __syncwarp();
-    } else {
-      // ------------------------------------------------ softmax: this thread's row
-      const int mt = warp >> 2, rr = row_base + tid;
-      const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
-      const bool live = rr < row_all;
+      named_bar_sync(1, kWorkers);
+      const float kref = fmaxf(__uint_as_float(s_ref[0]), pow2f(-126)), vref = fmaxf(__uint_as_float(s_ref[1]), pow2f(-126));
+      const bool bad = s_bad != 0;
       const int pos = live ? s.n - s.rows + rr / p.group : -1;
       const int wlo = p.window ? pos - p.window : -1;  // tokens k > wlo, or k < sinks
       const int t_first = s.n - s.rows + min(row_base + mt * 128, row_all - 1) / p.group;  // positions of the tile's rows
       const int t_last = s.n - s.rows + (min(row_base + mt * 128 + 128, row_all) - 1) / p.group;
       const bool ragged = row_base + mt * 128 + 128 > row_all;
-      const float cs = undo * p.scale_log2 * kref;
+      const float cs = fmaxf(s_undo[tid] * fabsf(p.scale_log2) * kref, 1.2e-38f);  // not 0: hidden scores are -inf
       float m = -INFINITY, l = 0.f;
-      bool ok = mt == 0 || two;
-      const uint32_t ts = t_s(mt) + lane_at, to = t_o(mt) + lane_at;
+      bool ok = mt == 0 || x.two;
       for (int j = 0; ok && j < n; ++j) {
-        const int base = base_of(i0 + j);
+        const int base = x.base_of(x.i0 + j);
         const bool masked = bad || ragged || base + kPTok - 1 > t_first ||
                             (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
         if (!(ok = __all_sync(~0u, wait(s_full + mt, n_s + j)))) break;
         tc_fence_after();
-        uint32_t P[64];
-        float ls, mx;
-        for (int pass = 0; pass < 2; ++pass) {
-          const float from = m == -INFINITY ? 0.f : m, add = kShift - from;
-          ls = 0.f;
-          mx = -INFINITY;
+        auto load = [&](int q, uint32_t (&v)[32]) {  // 32 scores, -inf where the row does not look
+          __syncwarp();
+          tmem_ld32(ts + 32 * q, v);
+          tc_wait_ld();
+          if (masked) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t v[32];
-            __syncwarp();
-            tmem_ld32(ts + 32 * q, v);
-            tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), cs, add));
-            if (masked) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int k = base + 32 * q + e;
-                bool see = k <= pos && (k > wlo || k < p.sinks);
-                if (bad && see) see = (unsigned)c.table[(int64_t)item.b * c.width + k / c.block] < (unsigned)c.n_blocks;
-                if (!see) v[e] = __float_as_uint(-INFINITY);
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float a = __uint_as_float(v[e]), b = __uint_as_float(v[e + 1]);
-              mx = fmaxf(mx, fmaxf(a, b));
-              const float x = ex2(a), y = ex2(b);
-              ls += x;
-              ls += y;
-              P[16 * q + e / 2] = f2h(x, y);
+            for (int e = 0; e < 32; ++e) {
+              const int k = base + 32 * q + e;
+              bool see = k <= pos && (k > wlo || k < p.sinks);
+              if (bad && see) see = (unsigned)c.table[(int64_t)x.b * c.width + k / c.block] < (unsigned)c.n_blocks;
+              if (!see) v[e] = __float_as_uint(-INFINITY);
             }
           }
-          const bool grow = mx > (m == -INFINITY ? -INFINITY : kShift + kSlack);
-          if (pass || !__any_sync(~0u, grow)) break;
-          const float to_m = grow ? mx - kShift + from : m;
+        };
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          uint32_t v[32];
+          load(q, v);
+          float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[e & 3] = fmaxf(y[e & 3], __uint_as_float(v[e]));
+          mx = fmaxf(mx, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+        }
+        mx *= cs;
+        if (__any_sync(~0u, mx > m + kSlack)) {
+          const float to_m = mx > m + kSlack ? mx : m;
           const float f = to_m == m ? 1.f : ex2(m - to_m);
           m = to_m;
           l *= f;
           if (j > 0) {
-#pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              uint32_t v[32];
-              tmem_ld32(to + 32 * q, v);
+#pragma unroll 1
+            for (int q = 0; q < D / 16; ++q) {
+              uint32_t v[16];
+              tmem_ld16(to + 16 * q, v);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-              tmem_st32(to + 32 * q, v);
+              for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              tmem_st16(to + 16 * q, v);
             }
           }
         }
-        __syncwarp();
-        l += ls;
-        tmem_st32(ts, P);
-        tmem_st32(ts + 32, P + 32);
+        const float add = kShift - (m == -INFINITY ? 0.f : m);
+        float ls[2] = {0.f, 0.f};
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {  // P's columns 16 q .. + 15 lie over scores that are already read
+          uint32_t v[32], P[16];
+          load(q, v);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float ea = ex2(fmaf(__uint_as_float(v[e]), cs, add)), eb = ex2(fmaf(__uint_as_float(v[e + 1]), cs, add));
+            ls[0] += ea;
+            ls[1] += eb;
+            P[e / 2] = f2h(ea, eb);
+          }
+          tmem_st16(ts + 16 * q, P);
+        }
+        l += ls[0] + ls[1];
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready + mt);
       }
       // ---- the row's result
-      const bool have = ok && n > 0 && __all_sync(~0u, wait(o_full, n_item));
+      const bool have = ok && n > 0 && __all_sync(~0u, wait(o_full, n_o));
       if (have) tc_fence_after();
       if (ok && (have || n <= 0)) {
-        const bool whole = i0 == 0 && i1 == per;
+        const bool whole = x.whole;
         const float inv = whole ? (l == 0.f ? 0.f : vref / l) : vref;
         float* part = p.part + (2 * (int64_t)blockIdx.x + (u == u_begin ? 0 : 1)) * prompt_part<D>();
         const int64_t at = live ? (int64_t)(s.row0 + rr / p.group) * p.heads + h * p.group + rr % p.group : 0;
+        // a whole item's rows go through the query rows' place (all products are done), to be written
+        // 16 lanes a row; a piece's [dim / 4][row] as they come
+        uint8_t* stage = sm + L::q + warp * 32 * D * 2;
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
           uint32_t v[32];
@@ -547,12 +432,32 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(PromptParams pp
             for (int e = 0; e < 32; ++e) v[e] = 0;
           }
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            if (!live) break;
-            const float4 o = make_float4(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv,
-                                         __uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
-            if (whole) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + 32 * q + e)) = pack4(p.act, o);
-            else *reinterpret_cast<float4*>(part + tid * D + 32 * q + e) = o;
+          for (int e = 0; e < 32; e += 8) {
+            float o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[e + k]) * inv;
+            if (whole) {
+              const uint2 y = pack4(p.act, make_float4(o[0], o[1], o[2], o[3])), z = pack4(p.act, make_float4(o[4], o[5], o[6], o[7]));
+              const int ch = 4 * q + e / 8;
+              *reinterpret_cast<uint4*>(stage + lane * D * 2 + ((ch ^ (lane & 7)) << 4)) = make_uint4(y.x, y.y, z.x, z.y);
+            } else {
+              float4* to4 = reinterpret_cast<float4*>(part) + (8 * q + e / 4) * kPRows + tid;
+              to4[0] = make_float4(o[0], o[1], o[2], o[3]);
+              to4[kPRows] = make_float4(o[4], o[5], o[6], o[7]);
+            }
+          }
+        }
+        __syncwarp();
+        if (whole) {
+          constexpr int LR = D / 8, RI = 32 / LR;  // lanes a row, rows a store
+#pragma unroll 4
+          for (int i = 0; i < 32; i += RI) {
+            const int row = i + lane / LR, ch = lane % LR, r2 = row_base + 32 * warp + row;
+            if (r2 < row_all) {
+              const int64_t o = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
+              *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + 2 * (o * D + 8 * ch)) =
+                  *reinterpret_cast<const uint4*>(stage + row * D * 2 + ((ch ^ (row & 7)) << 4));
+            }
           }
         }
         if (live) {
@@ -564,34 +469,182 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(PromptParams pp
         }
         tc_fence_before();
       }
+      if (tid == 0) {  // everyone has read them: the converters, before this piece's last tile
+        s_ref[0] = s_ref[1] = 0;
+        s_bad = 0;
+      }
+      named_bar_sync(1, kWorkers);
+      if (s_abort) break;
+      tc_fence_after();
+      if (mt == 0 || x.two) n_s += n;
+      if (n > 0) ++n_o;
+      u += x.len;
     }
-    __syncthreads();
-    if (s_abort) break;
-    tc_fence_after();
-    // counters of the barriers' completions: each role keeps the ones it waits on
-    n_tile += n;
-    if (warp < 4) n_s += n;
-    else if (warp < 8) n_s += two ? n : 0;
-    else if (warp == 12) {
-      n_s += n;                   // p_ready[0]
-      n_item += two ? n : 0;      // p_ready[1]
-    }
-    if (warp < 8) n_item += n > 0 ? 1 : 0;  // o_full
-    u += i1 - i0;
-  }
-
-  // no product may still be running when tensor memory goes
-  if (warp == 12) {
-    if (lane == 0) {
-      umma_commit(drain);
-      const long long t0 = clock64();
-      while (!mbar_try_wait(drain, 0))
-        if (clock64() - t0 > 200000000LL) {
-          set_error(p.err, DUPLEX_DEVERR_TIMEOUT);
-          break;
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------- keys and values
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegConvert));
+    uint32_t n_tile = 0;
+    while (u < u_end) {
+      find_piece(pp, u, u_end, pi, x);
+      const int n = x.n, h = x.h, i0 = x.i0, lo_x = x.lo_x;
+      const Span& sp = x.sp;
+      constexpr int KC = D / 64;  // 16-byte chunks a lane takes of a token
+      const int cw = warp - 8, kt = lane & 7, kc = lane >> 3;  // token of 8, chunk of 4 (of 64 dims)
+      uint4 kx[4][KC], vx[4][KC];
+      float kr[2], vr[2];  // scales of the warp's two 16-token parts
+      int id[2], id_next[2];
+      auto ids = [&](int i, int (&to)[2]) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tok = x.base_of(i) + 32 * cw + 16 * e;
+          to[e] = -1;
+          if (i < i0 + n && tok < sp.end && !(tok + 15 < lo_x && tok >= p.sinks))
+            to[e] = kv_block_at(c, x.b, tok / c.block, nullptr);
         }
+      };
+      auto load = [&](int i, const uint8_t* codes, const float* scales, uint4 (&to)[4][KC], float (&sc)[2]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int e = q >> 1, tok = x.base_of(i) + 32 * cw + 8 * q + kt;
+          const uint8_t* src = codes + ((((int64_t)id[e] * c.heads + h) * c.block + (tok & (c.block - 1))) * D + 16 * kc);
+#pragma unroll
+          for (int cc = 0; cc < KC; ++cc)
+            to[q][cc] = id[e] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(src + 64 * cc));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sc[e] = id[e] < 0 ? 0.f : __ldg(scales + (int64_t)id[e] * c.heads + h);
+      };
+      auto mul = [](uint32_t w, __half2 f) {
+        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&w), f);
+        return *reinterpret_cast<const uint32_t*>(&y);
+      };
+      auto put = [&](uint8_t* dst, int base, bool clean, const uint4 (&from)[4][KC], const float (&sc)[2], float ref) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int t = 32 * cw + 8 * q + kt;
+          const __half2 f = __float2half2_rn(sc[q >> 1] / ref);
+          const bool zero = !clean && !x.seen(p, base + t);
+#pragma unroll
+          for (int cc = 0; cc < KC; ++cc) {
+            uint4 y = from[q][cc];
+            if (zero) y = make_uint4(0, 0, 0, 0);
+            uint8_t* at = dst + cc * L::kHalf;
+            *reinterpret_cast<uint4*>(at + sw128(t, 2 * kc)) = make_uint4(mul(KvFmt<FMT>::lo(y.x), f), mul(KvFmt<FMT>::hi(y.x), f),
+                                                                          mul(KvFmt<FMT>::lo(y.y), f), mul(KvFmt<FMT>::hi(y.y), f));
+            *reinterpret_cast<uint4*>(at + sw128(t, 2 * kc + 1)) =
+                make_uint4(mul(KvFmt<FMT>::lo(y.z), f), mul(KvFmt<FMT>::hi(y.z), f), mul(KvFmt<FMT>::lo(y.w), f),
+                           mul(KvFmt<FMT>::hi(y.w), f));
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+      };
+      ids(i0, id);
+      if (n > 0) {
+        load(i0, c.k, c.k_scale, kx, kr);
+        load(i0, c.v, c.v_scale, vx, vr);
+      }
+      named_bar_sync(1, kWorkers);
+      const float kref = fmaxf(__uint_as_float(s_ref[0]), pow2f(-126)), vref = fmaxf(__uint_as_float(s_ref[1]), pow2f(-126));
+      for (int j = 0; j < n; ++j) {
+        const uint32_t cnt = n_tile + j, slot = cnt & 1, use = cnt >> 1;
+        const int i = i0 + j, base = x.base_of(i);
+        const bool clean = base + kPTok <= sp.end && (base >= lo_x || base + kPTok <= p.sinks);
+        ids(i + 1, id_next);
+        if (use > 0 && !wait(k_empty + slot, use - 1)) break;
+        put(sm + L::k + slot * L::kTile, base, clean, kx, kr, kref);
+        if (lane == 0) mbar_arrive(k_full + slot);
+        id[0] = id_next[0];
+        id[1] = id_next[1];
+        if (j + 1 < n) load(i + 1, c.k, c.k_scale, kx, kr);
+        if (use > 0 && !wait(v_empty + slot, use - 1)) break;
+        put(sm + L::v + slot * L::kTile, base, clean, vx, vr, vref);
+        if (lane == 0) mbar_arrive(v_full + slot);
+        if (j + 1 < n) load(i + 1, c.v, c.v_scale, vx, vr);
+      }
+      named_bar_sync(1, kWorkers);
+      if (s_abort) break;
+      n_tile += n;
+      u += x.len;
     }
-    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegMma));
+    if (warp == 12) {
+      // -------------------------------------------------------------- products
+      constexpr uint32_t id_qk = idesc_f16(0, 128, kPTok), id_pv = idesc_f16(0, 128, D) | kIdescBMnMajor;
+      uint32_t n_tile = 0, n1 = 0;  // tiles so far (p_ready[0], the rings); completions of p_ready[1]
+      while (u < u_end) {
+        find_piece(pp, u, u_end, pi, x);
+        const int n = x.n;
+        const bool two = x.two;
+        named_bar_sync(1, kWorkers);
+        if (lane == 0 && n > 0) {
+          const uint32_t sq = smem_u32(sm + L::q), sk = smem_u32(sm + L::k), sv = smem_u32(sm + L::v);
+          auto qk = [&](int mt, uint32_t slot) {
+            const uint64_t dq = smem_desc_sw128(sq + mt * L::kTile, 16), dk = smem_desc_sw128(sk + slot * L::kTile, 16);
+#pragma unroll 2
+            for (int y = 0; y < D / 16; ++y) {
+              const uint32_t at = (y >> 2) * (L::kHalf >> 4) + (y & 3) * 2;
+              umma_ss(t_s(mt), dq + at, dk + at, id_qk, y != 0);
+            }
+            umma_commit(s_full + mt);
+          };
+          auto pv = [&](int mt, uint32_t slot, bool more) {
+            const uint64_t dv = smem_desc_sw128(sv + slot * L::kTile, L::kHalf);
+#pragma unroll 2
+            for (int y = 0; y < kPTok / 16; ++y)
+              umma_ts(t_o(mt), t_s(mt) + 8 * y, dv + y * (2048 >> 4), id_pv, more || y != 0);
+          };
+          bool ok = wait(k_full + (n_tile & 1), n_tile >> 1);
+          if (ok) {
+            tc_fence_after();
+            qk(0, n_tile & 1);
+            if (two) qk(1, n_tile & 1);
+            umma_commit(k_empty + (n_tile & 1));
+          }
+          for (int j = 0; ok && j < n; ++j) {
+            const uint32_t cnt = n_tile + j, slot = cnt & 1, nslot = slot ^ 1;
+            if (!(ok = wait(v_full + slot, cnt >> 1) && wait(p_ready, n_tile + j))) break;
+            tc_fence_after();
+            pv(0, slot, j > 0);
+            if (j + 1 < n) {
+              if (!(ok = wait(k_full + nslot, (cnt + 1) >> 1))) break;
+              tc_fence_after();
+              qk(0, nslot);
+            }
+            if (two) {
+              if (!(ok = wait(p_ready + 1, n1 + j))) break;
+              tc_fence_after();
+              pv(1, slot, j > 0);
+            }
+            umma_commit(v_empty + slot);
+            if (j + 1 < n) {
+              if (two) qk(1, nslot);
+              umma_commit(k_empty + nslot);
+            }
+          }
+          if (ok) umma_commit(o_full);
+        }
+        __syncwarp();
+        named_bar_sync(1, kWorkers);
+        if (s_abort) break;
+        tc_fence_after();
+        n_tile += n;
+        if (two) n1 += n;
+        u += x.len;
+      }
+      // no product may still be running when tensor memory goes
+      if (lane == 0) {
+        umma_commit(drain);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(drain, 0))
+          if (clock64() - t0 > 200000000LL) {
+            set_error(p.err, DUPLEX_DEVERR_TIMEOUT);
+            break;
+          }
+      }
+      __syncwarp();
+    }
   }
   __syncthreads();
   if (warp == 12) tmem_dealloc<512>(tm);
@@ -617,7 +670,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
   const KvSeq s = kv_seq(p.c, item.b);
   const int row_all = s.rows * p.group;
   for (int e = threadIdx.x; e < kPRows * D / 4; e += kJoinThreads) {
-    const int rr = e / (D / 4), d = (e - rr * (D / 4)) * 4, r2 = item.rt * kPRows + rr;
+    const int rr = e % kPRows, d = e / kPRows * 4, r2 = item.rt * kPRows + rr;
     if (r2 >= row_all) continue;
     auto slot = [&](int j) {
       const int k = (j == c0 && begin != (int64_t)c0 * share) ? 1 : 0;
@@ -631,7 +684,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
     for (int j = c0; j <= c1; ++j) {
       const float* ps = slot(j);
       const float mj = __ldcg(ps + kPRows * D + rr), f = mj == M ? 1.f : ex2(mj - M);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(ps + rr * D + d));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(ps) + d / 4 * kPRows + rr);
       l += __ldcg(ps + kPRows * D + kPRows + rr) * f;
       o.x += x.x * f;
       o.y += x.y * f;
@@ -693,7 +746,7 @@ int kv_prompt_run(const AttendParams& a, void* workspace, cudaStream_t st) {
   pp.a.part = reinterpret_cast<float*>(ws + list);
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  const int64_t units = max_pairs(a.c, a.group) * a.c.heads * (((int64_t)a.c.width * a.c.block + kPTok - 1) / kPTok);
+  const int64_t units = max_pairs(a.c, a.group) * a.c.heads * (((int64_t)a.c.width * a.c.block + kPTok - 1) / kPTok + kPOver);
   const int ctas = (int)std::min({(int64_t)sms, (int64_t)kPMaxCtas, units});
   if (a.c.dim == 128)
     return a.c.format == DUPLEX_KV_E4M3 ? run<128, DUPLEX_KV_E4M3>(pp, ctas, st) : run<128, DUPLEX_KV_INT8>(pp, ctas, st);
