@@ -53,7 +53,7 @@ DEVI int units_in(const Span& sp) {
 }
 
 // An item costs as much as its tiles and kPOver more (query rows in, results out, the pipeline's ends).
-constexpr int kPOver = 2;
+constexpr int kPOver = 4;
 
 // The list of (sequence, row tile) pairs with their units, by one CTA.
 constexpr int kPlanThreads = 1024;
@@ -145,6 +145,27 @@ template <int D> struct PromptSmem {
 // 16-byte chunk c of a row
 DEVI uint32_t sw128(int row, int c) { return (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)); }
 
+DEVI float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// two fp32 operations in one instruction
+DEVI float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+DEVI float2 add2f(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\t"
+      "mov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 template <int D> constexpr int prompt_part() { return kPRows * (D + 2); }
 
 // The piece of an item that a CTA works on next: its list position and what follows from it, found
@@ -221,7 +242,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = s_tmem;
+  constexpr uint32_t tm = 0;  // all 512 columns: they start at column 0
   auto t_s = [&](int mt) { return tm + mt * 128; };
   auto t_o = [&](int mt) { return tm + 256 + mt * D; };
   pdl_wait();
@@ -346,64 +367,93 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
                             (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
         if (!(ok = __all_sync(~0u, wait(s_full + mt, n_s + j)))) break;
         tc_fence_after();
-        auto load = [&](int q, uint32_t (&v)[32]) {  // 32 scores, -inf where the row does not look
-          __syncwarp();
-          tmem_ld32(ts + 32 * q, v);
-          tc_wait_ld();
-          if (masked) {
+        const int k_max = pos - base, k_min = wlo - base, k_sink = p.sinks - base;  // columns k <= k_max, k > k_min or k < k_sink
+        auto hide = [&](uint32_t (&w)[16], int q) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int k = base + 32 * q + e;
-              bool see = k <= pos && (k > wlo || k < p.sinks);
-              if (bad && see) see = (unsigned)c.table[(int64_t)x.b * c.width + k / c.block] < (unsigned)c.n_blocks;
-              if (!see) v[e] = __float_as_uint(-INFINITY);
-            }
+          for (int e = 0; e < 16; ++e) {
+            bool see = 16 * q + e <= k_max && (16 * q + e > k_min || 16 * q + e < k_sink);
+            if (bad && see)
+              see = (unsigned)c.table[(int64_t)x.b * c.width + (base + 16 * q + e) / c.block] < (unsigned)c.n_blocks;
+            if (!see) w[e] = __float_as_uint(-INFINITY);
           }
         };
+        // The loops are short on purpose: unrolled over the row they outgrow the instruction caches, and
+        // the tile takes 1.8 times as long.
         float mx = -INFINITY;
+        if (masked) {
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          uint32_t v[32];
-          load(q, v);
-          float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int q = 0; q < 8; ++q) {
+            uint32_t w[16];
+            __syncwarp();
+            tmem_ld16(ts + 16 * q, w);
+            tc_wait_ld();
+            hide(w, q);
+            tmem_st16(ts + 16 * q, w);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y[e & 3] = fmaxf(y[e & 3], __uint_as_float(v[e]));
-          mx = fmaxf(mx, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(w[e]));
+          }
+          tc_wait_st();
+        } else {
+          __syncwarp();
+#pragma unroll 1
+          for (int q = 0; q < 2; ++q) {
+            uint32_t w[2][32];
+            tmem_ld32(ts + 64 * q, w[0]);
+            tmem_ld32(ts + 64 * q + 32, w[1]);
+            tc_wait_ld();
+            float y[4] = {mx, mx, mx, mx};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) y[e & 3] = max3(y[e & 3], __uint_as_float(w[0][e]), __uint_as_float(w[1][e]));
+            mx = max3(y[0], y[1], fmaxf(y[2], y[3]));
+          }
         }
         mx *= cs;
         if (__any_sync(~0u, mx > m + kSlack)) {
-          const float to_m = mx > m + kSlack ? mx : m;
-          const float f = to_m == m ? 1.f : ex2(m - to_m);
-          m = to_m;
+          const float top = mx > m + kSlack ? mx : m;
+          const float f = top == m ? 1.f : ex2(m - top);
+          m = top;
           l *= f;
           if (j > 0) {
 #pragma unroll 1
             for (int q = 0; q < D / 16; ++q) {
-              uint32_t v[16];
-              tmem_ld16(to + 16 * q, v);
+              uint32_t o[16];
+              tmem_ld16(to + 16 * q, o);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-              tmem_st16(to + 16 * q, v);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(to + 16 * q, o);
             }
           }
         }
         const float add = kShift - (m == -INFINITY ? 0.f : m);
-        float ls[2] = {0.f, 0.f};
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {  // P's columns 16 q .. + 15 lie over scores that are already read
-          uint32_t v[32], P[16];
-          load(q, v);
+        const float2 cs2 = make_float2(cs, cs), add2 = make_float2(add, add);
+        float2 ls = make_float2(0.f, 0.f);
+        {
+          uint32_t va[32], vb[32];
+          auto part = [&](const uint32_t (&w)[32], int q) {  // P's columns 16 q .. + 15 lie over scores that are already read
+            uint32_t P[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float ea = ex2(fmaf(__uint_as_float(v[e]), cs, add)), eb = ex2(fmaf(__uint_as_float(v[e + 1]), cs, add));
-            ls[0] += ea;
-            ls[1] += eb;
-            P[e / 2] = f2h(ea, eb);
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])), cs2, add2);
+              const float2 z = make_float2(ex2(y.x), ex2(y.y));
+              ls = add2f(ls, z);
+              P[e / 2] = f2h(z.x, z.y);
+            }
+            tmem_st16(ts + 16 * q, P);
+          };
+          __syncwarp();
+          tmem_ld32(ts, va);
+#pragma unroll 1
+          for (int q = 0; q < 4; q += 2) {
+            tc_wait_ld();
+            tmem_ld32(ts + 32 * q + 32, vb);
+            part(va, q);
+            tc_wait_ld();
+            if (q == 0) tmem_ld32(ts + 64, va);
+            part(vb, q + 1);
           }
-          tmem_st16(ts + 16 * q, P);
         }
-        l += ls[0] + ls[1];
+        l += ls.x + ls.y;
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -578,52 +628,56 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         const int n = x.n;
         const bool two = x.two;
         named_bar_sync(1, kWorkers);
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
           const uint32_t sq = smem_u32(sm + L::q), sk = smem_u32(sm + L::k), sv = smem_u32(sm + L::v);
+          auto done = [&](uint64_t* b) {
+            if (elect_one()) umma_commit(b);
+          };
           auto qk = [&](int mt, uint32_t slot) {
             const uint64_t dq = smem_desc_sw128(sq + mt * L::kTile, 16), dk = smem_desc_sw128(sk + slot * L::kTile, 16);
-#pragma unroll 2
+#pragma unroll
             for (int y = 0; y < D / 16; ++y) {
               const uint32_t at = (y >> 2) * (L::kHalf >> 4) + (y & 3) * 2;
-              umma_ss(t_s(mt), dq + at, dk + at, id_qk, y != 0);
+              if (elect_one()) umma_ss(t_s(mt), dq + at, dk + at, id_qk, y != 0);
             }
-            umma_commit(s_full + mt);
+            done(s_full + mt);
           };
           auto pv = [&](int mt, uint32_t slot, bool more) {
             const uint64_t dv = smem_desc_sw128(sv + slot * L::kTile, L::kHalf);
-#pragma unroll 2
+#pragma unroll
             for (int y = 0; y < kPTok / 16; ++y)
-              umma_ts(t_o(mt), t_s(mt) + 8 * y, dv + y * (2048 >> 4), id_pv, more || y != 0);
+              if (elect_one()) umma_ts(t_o(mt), t_s(mt) + 8 * y, dv + y * (2048 >> 4), id_pv, more || y != 0);
           };
-          bool ok = wait(k_full + (n_tile & 1), n_tile >> 1);
+          auto all = [&](uint64_t* b, uint32_t k) { return __all_sync(~0u, wait(b, k)) != 0; };
+          bool ok = all(k_full + (n_tile & 1), n_tile >> 1);
           if (ok) {
             tc_fence_after();
             qk(0, n_tile & 1);
             if (two) qk(1, n_tile & 1);
-            umma_commit(k_empty + (n_tile & 1));
+            done(k_empty + (n_tile & 1));
           }
           for (int j = 0; ok && j < n; ++j) {
             const uint32_t cnt = n_tile + j, slot = cnt & 1, nslot = slot ^ 1;
-            if (!(ok = wait(v_full + slot, cnt >> 1) && wait(p_ready, n_tile + j))) break;
+            if (!(ok = all(v_full + slot, cnt >> 1) && all(p_ready, cnt))) break;
             tc_fence_after();
             pv(0, slot, j > 0);
             if (j + 1 < n) {
-              if (!(ok = wait(k_full + nslot, (cnt + 1) >> 1))) break;
+              if (!(ok = all(k_full + nslot, (cnt + 1) >> 1))) break;
               tc_fence_after();
               qk(0, nslot);
             }
             if (two) {
-              if (!(ok = wait(p_ready + 1, n1 + j))) break;
+              if (!(ok = all(p_ready + 1, n1 + j))) break;
               tc_fence_after();
               pv(1, slot, j > 0);
             }
-            umma_commit(v_empty + slot);
+            done(v_empty + slot);
             if (j + 1 < n) {
               if (two) qk(1, nslot);
-              umma_commit(k_empty + nslot);
+              done(k_empty + nslot);
             }
           }
-          if (ok) umma_commit(o_full);
+          if (ok) done(o_full);
         }
         __syncwarp();
         named_bar_sync(1, kWorkers);
@@ -634,15 +688,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         u += x.len;
       }
       // no product may still be running when tensor memory goes
-      if (lane == 0) {
-        umma_commit(drain);
-        const long long t0 = clock64();
-        while (!mbar_try_wait(drain, 0))
-          if (clock64() - t0 > 200000000LL) {
-            set_error(p.err, DUPLEX_DEVERR_TIMEOUT);
-            break;
-          }
-      }
+      if (elect_one()) umma_commit(drain);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(drain, 0))
+        if (clock64() - t0 > 200000000LL) {
+          set_error(p.err, DUPLEX_DEVERR_TIMEOUT);
+          break;
+        }
       __syncwarp();
     }
   }

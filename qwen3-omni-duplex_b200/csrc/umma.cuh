@@ -132,6 +132,15 @@ DEVI void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t id
       : "memory");
 }
 
+// True in one lane of a converged warp.  A role whose whole warp walks the loop and elects a lane for
+// each instruction keeps its descriptors in uniform registers; one lane in a branch of its own moves
+// every operand there first, which costs more than the MMA.
+DEVI bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+
 // This thread's generic shared-memory writes before later async-proxy reads of them (the
 // MMA's operands), once a barrier has ordered the threads.
 DEVI void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
