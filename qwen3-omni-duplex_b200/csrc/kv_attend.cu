@@ -641,7 +641,7 @@ extern "C" int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_ba
   p.q_head = q_head_stride;
   p.act = act_dtype;
   p.heads = heads;
-  p.group = heads / cache->kv_heads;
+  p.set_group(heads / cache->kv_heads);
   // a row tile's rows are counted in 32 bits
   if ((int64_t)batch->n_rows * p.group > 0x7FFFFFFFll - 256) return DUPLEX_ERR_UNSUPPORTED;
   const int64_t cap = (int64_t)batch->width * cache->block;  // a window of all that can be cached is none

@@ -23,6 +23,15 @@ struct AttendParams {
   float* lse;             // [n_rows][heads] or null
   float* part;            // partial results, 2 slots per CTA
   int32_t* err;
+  uint32_t group_mul, group_shift;  // r / group = (mulhi(r, mul) + r) >> shift for 0 <= r < 2^31
+
+  DEVI int by_group(int r) const { return (int)((__umulhi((uint32_t)r, group_mul) + (uint32_t)r) >> group_shift); }
+  void set_group(int g) {
+    group = g;
+    group_shift = 0;
+    while ((1ull << group_shift) < (uint64_t)g) ++group_shift;
+    group_mul = (uint32_t)((((1ull << group_shift) - (uint64_t)g) << 32) / (uint64_t)g + 1);
+  }
 };
 
 DEVI float ex2(float x) {
