@@ -414,14 +414,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
   }
 }
 
-// CTA j joins the row tile that crosses the boundary between pieces j and j + 1, if that is its first one.
+// CTA (j, y) joins the row tile that crosses the boundary between pieces j and j + 1, if that is its first
+// one: 128 float4s of it (4 rows of 128 dims, 8 of 64).  The pieces' factors first, a warp a row, then
+// sums with all pieces' loads independent of one another.
 template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p, int ctas) {
-  constexpr int ROWS = 8 * NT;
+  constexpr int ROWS = 8 * NT, RC = 512 / D;  // rows of a CTA
   extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ float s_m[RC], s_l[RC];
   int64_t* off = reinterpret_cast<int64_t*>(dyn);
   const KvView& c = p.c;
-  const int tid = threadIdx.x;
+  float* s_f = reinterpret_cast<float*>(off + c.batch + 1);  // [pieces][RC]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Plan plan = make_plan<ROWS>(p, off, ctas);
   const int64_t u = (int64_t)(blockIdx.x + 1) * plan.share;
   pdl_wait();
@@ -432,37 +436,54 @@ __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p,
   const int it = (int)((u - off[b]) / per);
   const int64_t begin = off[b] + (int64_t)it * per, last = begin + per - 1;
   if (begin == u || begin / plan.share != blockIdx.x) return;
-  const int c0 = blockIdx.x, c1 = (int)(last / plan.share);
+  const int c0 = blockIdx.x, n = (int)(last / plan.share) - c0 + 1;
   const int h = it / rt_all, rt = it - h * rt_all, row_all = s.rows * p.group;
-  for (int e = tid; e < ROWS * D / 4; e += kWarps * 32) {
-    const int rr = e / (D / 4), d = (e - rr * (D / 4)) * 4, r2 = rt * ROWS + rr;
-    if (r2 >= row_all) continue;
-    // piece j > c0 begins inside the row tile: its first slot.  Piece c0's is its first too if the tile begins it.
-    auto slot = [&](int j) {
-      const int k = (j == c0 && begin != (int64_t)c0 * plan.share) ? 1 : 0;
-      return p.part + (2 * (int64_t)j + k) * part_floats<D, NT>();
-    };
-    float M = -INFINITY;
-    for (int j = c0; j <= c1; ++j) M = fmaxf(M, __ldcg(slot(j) + ROWS * D + rr));
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
-#pragma unroll 4
-    for (int j = c0; j <= c1; ++j) {
-      const float* ps = slot(j);
-      const float mj = __ldcg(ps + ROWS * D + rr), f = mj == M ? 1.f : ex2(mj - M);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(ps + rr * D + d));
-      L += __ldcg(ps + ROWS * D + ROWS + rr) * f;
-      o.x += x.x * f;
-      o.y += x.y * f;
-      o.z += x.z * f;
-      o.w += x.w * f;
+  // piece j > 0 begins inside the row tile: its first slot.  Piece 0's is its first too if the tile begins it.
+  auto slot = [&](int j) {
+    const int k = (j == 0 && begin != (int64_t)c0 * plan.share) ? 1 : 0;
+    return p.part + (2 * (int64_t)(c0 + j) + k) * part_floats<D, NT>();
+  };
+  for (int r = warp; r < RC; r += kWarps) {
+    const int rr = blockIdx.y * RC + r;
+    float M = -INFINITY, L = 0.f;
+    for (int j = lane; j < n; j += 32) {
+      const float m = __ldcg(slot(j) + ROWS * D + rr);
+      s_f[j * RC + r] = m;
+      M = fmaxf(M, m);
     }
-    const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
-        pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-    if (d == 0) p.lse[at] = lse_of(M, L);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+    for (int j = lane; j < n; j += 32) {
+      const float m = s_f[j * RC + r], f = m == M ? 1.f : ex2(m - M);
+      s_f[j * RC + r] = f;
+      L += f * __ldcg(slot(j) + ROWS * D + ROWS + rr);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
+    if (lane == 0) {
+      s_m[r] = M;
+      s_l[r] = L;
+    }
   }
+  __syncthreads();
+  const int r = tid / (D / 4), d = (tid - r * (D / 4)) * 4, rr = blockIdx.y * RC + r, r2 = rt * ROWS + rr;
+  if (r2 >= row_all) return;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) {
+    const float f = s_f[j * RC + r];
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(slot(j) + rr * D + d));
+    o.x += x.x * f;
+    o.y += x.y * f;
+    o.z += x.z * f;
+    o.w += x.w * f;
+  }
+  const float M = s_m[r], L = s_l[r];
+  const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
+      pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+  if (d == 0) p.lse[at] = lse_of(M, L);
 }
 
 // Accumulated attention weights: weights[token] += sum over the sequence's rows and the group's
@@ -470,7 +491,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p,
 // registers as fp16, the query rows come by, 32 at a time, through shared memory.
 constexpr int kRowChunk = 32;
 
-template <int D, int FMT>
+// U units a CTA: where all rows are one chunk (decode) the chunk is staged once for several; otherwise
+// one unit, whose keys stay in registers while the chunks go by.
+template <int D, int FMT, int U>
 __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p) {
   __shared__ uint2 sq[kRowChunk / 8][D / 16][32];
   __shared__ float s_sc[kRowChunk], s_lse[kRowChunk];
@@ -479,27 +502,32 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
   const KvSeq s = kv_seq(c, b);
-  const int tile = blockIdx.x * kUnit, start = s.n - s.rows;
+  const int tile = blockIdx.x * (U * kUnit), start = s.n - s.rows;
   if (tile >= s.n) return;
   // the sequence's rows that see a token of the tile
   int t0 = max(tile - start, 0), t1 = s.rows;
-  if (p.window && tile >= p.sinks) t1 = (int)min((int64_t)t1, (int64_t)tile + kUnit - 1 + p.window - start);
+  if (p.window && tile >= p.sinks) t1 = (int)min((int64_t)t1, (int64_t)tile + U * kUnit - 1 + p.window - start);
   if (t0 >= t1) return;
-  const int tok = tile + 16 * warp;
-  const bool hidden = tok >= s.n || (p.window && tok + 15 <= start - p.window && tok >= p.sinks);
-  const int id = hidden ? -1 : kv_block_at(c, b, tok / c.block, p.err);
-  const int64_t bh = (int64_t)max(id, 0) * c.heads + h;
-  uint4 kr[2][D / 64];
-  float ks = 0.f;
-  if (id >= 0) {
-    const uint8_t* kp = c.k + (bh * c.block + (tok & (c.block - 1))) * D + 16 * t;
+  uint4 kr[U][2][D / 64];
+  float ks[U], sum[U][2];
+  int64_t at[U];  // the warp's 16 tokens' slot, or -1
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int x = 0; x < U; ++x) {
+    const int tok = tile + x * kUnit + 16 * warp;
+    const bool hidden = tok >= s.n || (p.window && tok + 15 <= start - p.window && tok >= p.sinks);
+    const int id = hidden ? -1 : kv_block_at(c, b, tok / c.block, p.err);
+    const int64_t bh = (int64_t)max(id, 0) * c.heads + h;
+    at[x] = id < 0 ? -1 : bh * c.block + (tok & (c.block - 1));
+    sum[x][0] = sum[x][1] = ks[x] = 0.f;
+    if (id >= 0) {
+      const uint8_t* kp = c.k + at[x] * D + 16 * t;
 #pragma unroll
-      for (int cc = 0; cc < D / 64; ++cc) kr[i][cc] = __ldg(reinterpret_cast<const uint4*>(kp + (g + 8 * i) * D + 64 * cc));
-    ks = __ldg(c.k_scale + bh);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int cc = 0; cc < D / 64; ++cc) kr[x][i][cc] = __ldg(reinterpret_cast<const uint4*>(kp + (g + 8 * i) * D + 64 * cc));
+      ks[x] = __ldg(c.k_scale + bh);
+    }
   }
-  float sum[2] = {0.f, 0.f};
   const int r1 = t1 * p.group;
   for (int r0 = t0 * p.group; r0 < r1; r0 += kRowChunk) {
     __syncthreads();
@@ -518,31 +546,39 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
       }
     }
     __syncthreads();
-    if (id < 0) continue;
 #pragma unroll
     for (int nt = 0; nt < kRowChunk / 8; ++nt) {
       if (r0 + nt * 8 >= r1) break;
       uint2 qf[1][D / 16];
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) qf[0][i] = sq[nt][i][lane];
-      float S[1][4] = {{0.f, 0.f, 0.f, 0.f}};
-      qk<D, FMT, 1>(kr, qf, S);
+      const float sc[2] = {s_sc[nt * 8 + 2 * t], s_sc[nt * 8 + 2 * t + 1]}, ls[2] = {s_lse[nt * 8 + 2 * t], s_lse[nt * 8 + 2 * t + 1]};
+      const int pos[2] = {s_pos[nt * 8 + 2 * t], s_pos[nt * 8 + 2 * t + 1]};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int rr = nt * 8 + 2 * t + (j & 1), k = tok + g + 8 * (j >> 1), q = s_pos[rr];
-        if (k <= q && (!p.window || k > q - p.window || k < p.sinks)) sum[j >> 1] += ex2(S[0][j] * (s_sc[rr] * ks) - s_lse[rr]);
+      for (int x = 0; x < U; ++x) {
+        if (at[x] < 0) continue;
+        float S[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+        qk<D, FMT, 1>(kr[x], qf, S);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = tile + x * kUnit + 16 * warp + g + 8 * (j >> 1), q = pos[j & 1];
+          if (k <= q && (!p.window || k > q - p.window || k < p.sinks))
+            sum[x][j >> 1] += ex2(S[0][j] * (sc[j & 1] * ks[x]) - ls[j & 1]);
+        }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float x = sum[i];
-    x += __shfl_xor_sync(~0u, x, 1);
-    x += __shfl_xor_sync(~0u, x, 2);
-    const int k = tok + g + 8 * i;
-    // one addition to a token's sum, so its order does not matter; sequences that share a block may add to the same one
-    if (t == 0 && id >= 0 && k < s.n) atomicAdd(c.weights + bh * c.block + (k & (c.block - 1)), x);
-  }
+  for (int x = 0; x < U; ++x)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float y = sum[x][i];
+      y += __shfl_xor_sync(~0u, y, 1);
+      y += __shfl_xor_sync(~0u, y, 2);
+      const int k = tile + x * kUnit + 16 * warp + g + 8 * i;
+      // one addition to a token's sum, so its order does not matter; sequences that share a block may add to the same one
+      if (t == 0 && at[x] >= 0 && k < s.n) atomicAdd(c.weights + at[x] + g + 8 * i, y);
+    }
 }
 
 // 16 rows a tile need half the passes over the cache of 8, at 2 CTAs an SM instead of 3
@@ -570,10 +606,11 @@ static int run_attend(const AttendParams& p, cudaStream_t st) {
   kv_attend_kernel<D, FMT, NT><<<ctas, kWarps * 32, smem, st>>>(p);
   if (int rc = record_cuda(cudaGetLastError())) return rc;
   if (ctas > 1) {
+    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_combine_kernel<D, NT>), 100 * 1024)) return rc;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas - 1);
+    cfg.gridDim = dim3(ctas - 1, ROWS * D / 512);
     cfg.blockDim = dim3(kWarps * 32);
-    cfg.dynamicSmemBytes = plan;
+    cfg.dynamicSmemBytes = plan + sizeof(float) * ctas * (512 / D);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -591,8 +628,11 @@ static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
                  : nt_of(p.c, p.group) == 1    ? run_attend<D, FMT, 1>(p, st)
                                                : run_attend<D, FMT, 2>(p, st);
   if (rc || !p.c.weights) return rc;
-  const dim3 grid((unsigned)(((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit), p.c.heads, p.c.batch);
-  kv_weights_kernel<D, FMT><<<grid, kWarps * 32, 0, st>>>(p);
+  const bool few = (int64_t)p.c.n_rows * p.group <= (int64_t)p.c.batch * kRowChunk;
+  const int tokens = few ? 2 * kUnit : kUnit;
+  const dim3 grid((unsigned)(((int64_t)p.c.width * p.c.block + tokens - 1) / tokens), p.c.heads, p.c.batch);
+  if (few) kv_weights_kernel<D, FMT, 2><<<grid, kWarps * 32, 0, st>>>(p);
+  else kv_weights_kernel<D, FMT, 1><<<grid, kWarps * 32, 0, st>>>(p);
   return record_cuda(cudaGetLastError());
 }
 

@@ -6,12 +6,13 @@
 // bound by their bytes (append reads 2 bytes and writes 1 per element, eviction reads 1 and
 // writes 1): the block's values stay in registers between the search for the largest and the
 // rounding, so each is read once.
+#include <type_traits>
+
 #include "kv.cuh"
 
 namespace duplex {
 
-constexpr int kThreads = 256;  // 16 elements each, so 128 x 128 values are 4 rounds
-constexpr int kRounds = 4;
+constexpr int kThreads = 256;  // 16 elements each: R = 1, 2 or 4 rounds for a block's values
 
 DEVI float block_max(float x, float* red) {
 #pragma unroll
@@ -39,17 +40,22 @@ struct AppendParams {
 
 // Work item w of a sequence's touched blocks: sequence b owns items [cu[b]/P + 2b, cu[b+1]/P + 2(b+1)),
 // which is never fewer than the blocks that its rows touch.
-template <int FMT, int ACT>
+template <int FMT, int ACT, int kRounds>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams p) {
   __shared__ float red[kThreads / 32];
   const KvView& c = p.c;
   const int P = c.block, D = c.dim, h = blockIdx.y, tid = threadIdx.x;
   const bool val = blockIdx.z != 0;
   const int64_t w = blockIdx.x;
-  int lo = 0, hi = c.batch - 1;
-  while (lo < hi) {  // the last b whose first item is <= w
-    const int mid = (lo + hi + 1) >> 1;
-    if (kv_seq(c, mid).row0 / P + 2ll * mid <= w) lo = mid; else hi = mid - 1;
+  // the last b whose first item is <= w, 32 sequences a look
+  int lo = 0, left = c.batch;
+  const int lane = tid & 31;
+  while (left > 1) {
+    const int step = (left + 31) / 32, at = lo + lane * step;
+    const bool before = at < lo + left && kv_seq(c, at).row0 / P + 2ll * at <= w;
+    const int i = 31 - __clz(__ballot_sync(~0u, before) | 1u);
+    left = min(step, lo + left - (lo + i * step));
+    lo += i * step;
   }
   const int b = lo;
   const KvSeq s = kv_seq(c, b);
@@ -140,7 +146,7 @@ struct EvictParams {
   KvView c;
   const int32_t* dst;  // [batch][dst_width]
   int dst_width, keep, sinks, recent;
-  int32_t* index;      // [batch][heads][keep] kept tokens in order (sequences with more than keep)
+  int32_t* index;      // [batch][heads][keep] kept tokens in order, as block * P + place in it
   int32_t* new_len;
   int32_t* err;
 };
@@ -156,27 +162,48 @@ DEVI uint32_t order_key(float x) {
 constexpr int kSelThreads = 1024;
 
 // One CTA per (sequence, head).  The R = keep - sinks - recent largest keys of the tokens between
-// sinks and recent: four passes of 8 bits find the R-th largest key (per-warp histograms in shared
-// memory), a last pass writes the kept tokens in order: all above it, and the first of those equal.
+// sinks and recent: four passes of 8 bits find the R-th largest key (per-warp histograms), then each
+// warp counts and writes its own stretch of the tokens in order: all above that key, and the first of
+// those equal.  Keys stay in shared memory (SM_KEYS: up to kMaxKeys tokens), so weights and block ids
+// are read once; longer sequences read them anew in each pass.
+constexpr int kMaxKeys = 40 * 1024;
+
+template <bool SM_KEYS>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
-  __shared__ int hist[kSelThreads / 32][256];
-  __shared__ int warp_sum[2][kSelThreads / 32];
+  constexpr int W = kSelThreads / 32;
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[W][256];
+  __shared__ int total[256];
+  __shared__ int s_held[W], s_equal[W];
   __shared__ int s_digit, s_above;
   const KvView& c = p.c;
   const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = kv_seq(c, b).n;
   if (h == 0 && tid == 0) p.new_len[b] = min(n, p.keep);
-  if (n <= p.keep) return;
-  const int lo = p.sinks, hi = n - p.recent;  // keep >= sinks + recent and n > keep, so lo < hi
-  int want = p.keep - p.sinks - p.recent;
   int32_t* out = p.index + ((int64_t)b * c.heads + h) * p.keep;
-  auto key_of = [&](int j) -> uint32_t {
+  auto slot_of = [&](int j) -> int {  // a token's place among all blocks' tokens, or -1
     const int id = kv_block_at(c, b, j / c.block, p.err);
-    return id < 0 ? 0u : order_key(c.weights[((int64_t)id * c.heads + h) * c.block + j % c.block]);
+    return id < 0 ? -1 : id * c.block + (j & (c.block - 1));
   };
+  if (n <= p.keep) {
+    for (int j = tid; j < n; j += kSelThreads) out[j] = slot_of(j);
+    return;
+  }
+  auto read_key = [&](int j) -> uint32_t {
+    const int s = slot_of(j);
+    return s < 0 ? 0u : order_key(c.weights[((int64_t)(s / c.block) * c.heads + h) * c.block + (s & (c.block - 1))]);
+  };
+  const int lo = p.sinks, hi = n - p.recent;  // keep >= sinks + recent and n > keep, so lo < hi
+  if (SM_KEYS) {
+#pragma unroll 4
+    for (int j = lo + tid; j < hi; j += kSelThreads) keys[j] = read_key(j);
+  }
+  auto key_of = [&](int j) -> uint32_t { return SM_KEYS ? keys[j] : read_key(j); };
+  int want = p.keep - p.sinks - p.recent;
+  const bool none = want == 0;
   uint32_t prefix = 0, mask = 0;
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    for (int i = tid; i < 256 * (kSelThreads / 32); i += kSelThreads) (&hist[0][0])[i] = 0;
+  for (int shift = 24; shift >= 0 && !none; shift -= 8) {
+    for (int i = tid; i < 256 * W; i += kSelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
     for (int j = lo + tid; j < hi; j += kSelThreads) {
       const uint32_t u = key_of(j);
@@ -185,15 +212,29 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
     __syncthreads();
     if (tid < 256) {
       int sum = 0;
-      for (int w = 0; w < kSelThreads / 32; ++w) sum += hist[w][tid];
-      hist[0][tid] = sum;
+#pragma unroll 8
+      for (int w = 0; w < W; ++w) sum += hist[w][tid];
+      total[tid] = sum;
     }
     __syncthreads();
-    if (tid == 0) {
-      int above = 0, d = 255;
-      while (d > 0 && above + hist[0][d] < want) above += hist[0][d--];
-      s_digit = d;
-      s_above = above;
+    if (warp == 0) {  // the largest digit with `want` keys at it and above: lane i has digits 255 - 8 i down
+      int mine = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mine += total[255 - 8 * lane - e];
+      int above = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(~0u, above, o);
+        if (lane >= o) above += v;
+      }
+      const int first = __ffs(__ballot_sync(~0u, above >= want)) - 1;  // there are at least `want` keys
+      if (lane == first) {
+        above -= mine;
+        int d = 255 - 8 * lane;
+        while (above + total[d] < want) above += total[d--];
+        s_digit = d;
+        s_above = above;
+      }
     }
     __syncthreads();
     prefix |= (uint32_t)s_digit << shift;
@@ -201,55 +242,58 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
     want -= s_above;
     __syncthreads();
   }
-  // now `want` of the keys equal to prefix are kept, the first ones
-  const bool none = p.keep == p.sinks + p.recent;
-  int kept = 0, equal = 0;  // kept tokens and equal keys before this round's
-  for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    bool held = false, eq = false;
-    if (j < n) {
-      if (j < lo || j >= hi) held = true;
-      else if (!none) {
-        const uint32_t u = key_of(j);
-        held = u > prefix;
-        eq = u == prefix;
-      }
+  // `want` of the keys equal to prefix are kept, the first ones
+  const int stretch = ((n + W - 1) / W + 31) / 32 * 32, j0 = min(warp * stretch, n), j1 = min(j0 + stretch, n);
+  auto look = [&](int j, bool& held, bool& eq) {
+    held = eq = false;
+    if (j >= j1) return;
+    if (j < lo || j >= hi) held = true;
+    else if (!none) {
+      const uint32_t u = key_of(j);
+      held = u > prefix;
+      eq = u == prefix;
     }
-    const uint32_t be = __ballot_sync(~0u, eq);
-    if (lane == 0) warp_sum[0][warp] = __popc(be);
-    __syncthreads();
-    int e_before = 0, e_all = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) e_before += warp_sum[0][w];
-      e_all += warp_sum[0][w];
-    }
-    if (eq && equal + e_before + __popc(be & ((1u << lane) - 1)) < want) held = true;
+  };
+  if (SM_KEYS) __syncthreads();
+  int held_n = 0, equal_n = 0;
+  for (int j = j0; j < j1; j += 32) {
+    bool held, eq;
+    look(j + lane, held, eq);
+    held_n += __popc(__ballot_sync(~0u, held));
+    equal_n += __popc(__ballot_sync(~0u, eq));
+  }
+  if (lane == 0) {
+    s_held[warp] = held_n;
+    s_equal[warp] = equal_n;
+  }
+  __syncthreads();
+  int to = 0, equal = 0;  // kept tokens and equal keys before the warp's
+  for (int w = 0; w < warp; ++w) {
+    to += s_held[w] + min(s_equal[w], max(want - equal, 0));
+    equal += s_equal[w];
+  }
+  for (int j = j0; j < j1; j += 32) {
+    bool held, eq;
+    look(j + lane, held, eq);
+    const uint32_t be = __ballot_sync(~0u, eq), below = (1u << lane) - 1;
+    if (eq && equal + __popc(be & below) < want) held = true;
     const uint32_t bh = __ballot_sync(~0u, held);
-    if (lane == 0) warp_sum[1][warp] = __popc(bh);
-    __syncthreads();
-    int h_before = 0, h_all = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) h_before += warp_sum[1][w];
-      h_all += warp_sum[1][w];
-    }
-    const int to = kept + h_before + __popc(bh & ((1u << lane) - 1));
-    if (held && to < p.keep) out[to] = j;
-    kept += h_all;
-    equal += e_all;
-    __syncthreads();
+    const int i = to + __popc(bh & below);
+    if (held && i < p.keep) out[i] = slot_of(j + lane);
+    to += __popc(bh);
+    equal += __popc(be);
   }
 }
 
-// One CTA per (destination block, sequence and head, keys or values): its tokens' codes are read
-// where they are, brought to the largest source scale's value, and rounded at the new scale.
-template <int FMT>
+// One CTA per (destination block, sequence and head): its tokens' codes, keys and values, are read
+// where they are, and rounded at the new block's scale.
+template <int FMT, int R>
 __global__ void __launch_bounds__(kThreads) kv_gather_kernel(EvictParams p) {
-  __shared__ float red[kThreads / 32];
+  __shared__ float red[2][kThreads / 32];
   const KvView& c = p.c;
   const int P = c.block, D = c.dim, tid = threadIdx.x;
-  const bool val = blockIdx.z != 0;
   const int b = blockIdx.y / c.heads, h = blockIdx.y - b * c.heads;
-  const int n = kv_seq(c, b).n, kept = min(n, p.keep);
+  const int kept = min(kv_seq(c, b).n, p.keep);
   const int base = blockIdx.x * P;
   if (base >= kept) return;
   const int id = p.dst[(int64_t)b * p.dst_width + blockIdx.x];
@@ -258,60 +302,71 @@ __global__ void __launch_bounds__(kThreads) kv_gather_kernel(EvictParams p) {
     return;
   }
   const int count = min(kept - base, P);
-  const int32_t* index = n > p.keep ? p.index + ((int64_t)b * c.heads + h) * p.keep : nullptr;
-  const uint8_t* codes = val ? c.v : c.k;
-  const float* scales = val ? c.v_scale : c.k_scale;
+  const int32_t* index = p.index + ((int64_t)b * c.heads + h) * p.keep + base;
   const int per = D / 16;
-  uint4 x[kRounds];
-  float sc[kRounds];
-  float amax = 0.f;
+  int src[R];
 #pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const int e = tid + i * kThreads, tok = e / per, d = (e - tok * per) * 16;
-    x[i] = make_uint4(0, 0, 0, 0);
-    sc[i] = 0.f;
-    if (tok < count) {
-      const int j = index ? index[base + tok] : base + tok;
-      const int src = kv_block_at(c, b, j / P, p.err);
-      if (src >= 0) {
-        const int64_t row = ((int64_t)src * c.heads + h) * P + j % P;
-        x[i] = __ldg(reinterpret_cast<const uint4*>(codes + row * D + d));
-        sc[i] = scales[(int64_t)src * c.heads + h];
-      }
-    }
-    float m = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 a = h2f(KvFmt<FMT>::lo((&x[i].x)[j])), q = h2f(KvFmt<FMT>::hi((&x[i].x)[j]));
-      m = fmaxf(m, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(q.x), fabsf(q.y))));
-    }
-    amax = fmaxf(amax, m * sc[i]);
+  for (int i = 0; i < R; ++i) {
+    const int tok = (tid + i * kThreads) / per;
+    src[i] = tok < count ? __ldg(index + tok) : -1;
   }
-  amax = block_max(amax, red);
-  const int e2 = KvFmt<FMT>::exponent(amax);
-  const float inv = e2 >= 127 ? 0.5f * pow2f(-126) : pow2f(-e2);
+  uint4 x[2][R];
+  float sc[2][R], amax[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int e = tid + i * kThreads, d = (e % per) * 16;
+    const int64_t bh = (int64_t)(max(src[i], 0) / P) * c.heads + h, row = bh * P + (src[i] & (P - 1));
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      x[y][i] = src[i] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>((y ? c.v : c.k) + row * D + d));
+      sc[y][i] = src[i] < 0 ? 0.f : __ldg((y ? c.v_scale : c.k_scale) + bh);
+    }
+  }
   const int64_t at = ((int64_t)id * c.heads + h) * P;
-  uint8_t* to = (val ? c.v : c.k) + at * D;
-#pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const int e = tid + i * kThreads, tok = e / per;
-    if (tok >= count) continue;
-    const float f = sc[i] * inv;
-    uint4 q;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 a = h2f(KvFmt<FMT>::lo((&x[i].x)[j])), d = h2f(KvFmt<FMT>::hi((&x[i].x)[j]));
-      (&q.x)[j] = KvFmt<FMT>::encode4(a.x * f, a.y * f, d.x * f, d.y * f);
-    }
-    *reinterpret_cast<uint4*>(to + e * 16) = q;
+  for (int i = tid; i < count; i += kThreads) {
+    const int s = __ldg(index + i);
+    c.weights[at + i] = s < 0 ? 0.f : c.weights[((int64_t)(s / P) * c.heads + h) * P + (s & (P - 1))];
   }
-  if (tid == 0) ((val ? c.v_scale : c.k_scale))[(int64_t)id * c.heads + h] = pow2f(min(e2, 127));
-  if (!val)
-    for (int i = tid; i < count; i += kThreads) {
-      const int j = index ? index[base + i] : base + i;
-      const int src = kv_block_at(c, b, j / P, nullptr);
-      c.weights[at + i] = src < 0 ? 0.f : c.weights[((int64_t)src * c.heads + h) * P + j % P];
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = h2f(KvFmt<FMT>::lo((&x[y][i].x)[j])), q = h2f(KvFmt<FMT>::hi((&x[y][i].x)[j]));
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(q.x), fabsf(q.y))));
+      }
+      amax[y] = fmaxf(amax[y], m * sc[y][i]);
     }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax[y] = fmaxf(amax[y], __shfl_xor_sync(~0u, amax[y], o));
+    if ((tid & 31) == 0) red[y][tid >> 5] = amax[y];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    float m = red[y][0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) m = fmaxf(m, red[y][w]);
+    const int e2 = min(KvFmt<FMT>::exponent(m), 127);
+    const float inv = e2 == 127 ? 0.5f * pow2f(-126) : pow2f(-e2);
+    uint8_t* to = (y ? c.v : c.k) + at * D;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int e = tid + i * kThreads;
+      if (e / per >= count) continue;
+      const float f = sc[y][i] * inv;
+      uint4 q;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = h2f(KvFmt<FMT>::lo((&x[y][i].x)[j])), d = h2f(KvFmt<FMT>::hi((&x[y][i].x)[j]));
+        (&q.x)[j] = KvFmt<FMT>::encode4(a.x * f, a.y * f, d.x * f, d.y * f);
+      }
+      *reinterpret_cast<uint4*>(to + e * 16) = q;
+    }
+    if (tid == 0) (y ? c.v_scale : c.k_scale)[(int64_t)id * c.heads + h] = pow2f(e2);
+  }
 }
 
 // ----------------------------------------------------------------- checks
@@ -357,14 +412,20 @@ extern "C" int duplex_kv_append(const duplex_kv_cache* cache, const duplex_kv_ba
   const int64_t items = batch->n_rows / cache->block + 2ll * batch->batch;
   const dim3 grid((unsigned)items, cache->kv_heads, 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rounds = (cache->block * cache->dim / 16 + kThreads - 1) / kThreads;
+  auto go = [&](auto fmt, auto act) {
+    constexpr int F = decltype(fmt)::value, A = decltype(act)::value;
+    if (rounds == 1) kv_append_kernel<F, A, 1><<<grid, kThreads, 0, st>>>(p);
+    else if (rounds == 2) kv_append_kernel<F, A, 2><<<grid, kThreads, 0, st>>>(p);
+    else kv_append_kernel<F, A, 4><<<grid, kThreads, 0, st>>>(p);
+  };
+  using E4 = std::integral_constant<int, DUPLEX_KV_E4M3>;
+  using I8 = std::integral_constant<int, DUPLEX_KV_INT8>;
+  using F16 = std::integral_constant<int, DUPLEX_DTYPE_F16>;
+  using B16 = std::integral_constant<int, DUPLEX_DTYPE_BF16>;
   const bool f16 = act_dtype == DUPLEX_DTYPE_F16;
-  if (cache->format == DUPLEX_KV_E4M3) {
-    if (f16) kv_append_kernel<DUPLEX_KV_E4M3, DUPLEX_DTYPE_F16><<<grid, kThreads, 0, st>>>(p);
-    else kv_append_kernel<DUPLEX_KV_E4M3, DUPLEX_DTYPE_BF16><<<grid, kThreads, 0, st>>>(p);
-  } else {
-    if (f16) kv_append_kernel<DUPLEX_KV_INT8, DUPLEX_DTYPE_F16><<<grid, kThreads, 0, st>>>(p);
-    else kv_append_kernel<DUPLEX_KV_INT8, DUPLEX_DTYPE_BF16><<<grid, kThreads, 0, st>>>(p);
-  }
+  if (cache->format == DUPLEX_KV_E4M3) f16 ? go(E4{}, F16{}) : go(E4{}, B16{});
+  else f16 ? go(I8{}, F16{}) : go(I8{}, B16{});
   return record_cuda(cudaGetLastError());
 }
 
@@ -383,6 +444,7 @@ extern "C" int duplex_kv_evict(const duplex_kv_cache* cache, const duplex_kv_bat
   EvictParams p{};
   if (int rc = kv_check(cache, batch, &p.c)) return rc;
   if (!cache->weights || !dst_table || !new_len || keep < 1 || sinks < 0 || recent < 0) return DUPLEX_ERR_ARG;
+  if ((int64_t)cache->n_blocks * cache->block > 0x7FFFFFFFll) return DUPLEX_ERR_UNSUPPORTED;  // a token's place is 32 bits
   if ((int64_t)sinks + recent > keep || (int64_t)dst_width * cache->block < keep) return DUPLEX_ERR_ARG;
   size_t need = 0;
   duplex_kv_evict_workspace_bytes(cache, batch, keep, &need);
@@ -397,10 +459,24 @@ extern "C" int duplex_kv_evict(const duplex_kv_cache* cache, const duplex_kv_bat
   p.new_len = new_len;
   p.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  kv_select_kernel<<<dim3(cache->kv_heads, batch->batch), kSelThreads, 0, st>>>(p);
+  const dim3 heads(cache->kv_heads, batch->batch);
+  const int64_t cap = (int64_t)batch->width * cache->block;
+  if (cap <= kMaxKeys) {
+    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_select_kernel<true>), kMaxKeys * 4)) return rc;
+    kv_select_kernel<true><<<heads, kSelThreads, (size_t)cap * 4, st>>>(p);
+  } else {
+    kv_select_kernel<false><<<heads, kSelThreads, 0, st>>>(p);
+  }
   if (int rc = record_cuda(cudaGetLastError())) return rc;
-  const dim3 grid((keep + cache->block - 1) / cache->block, batch->batch * cache->kv_heads, 2);
-  if (cache->format == DUPLEX_KV_E4M3) kv_gather_kernel<DUPLEX_KV_E4M3><<<grid, kThreads, 0, st>>>(p);
-  else kv_gather_kernel<DUPLEX_KV_INT8><<<grid, kThreads, 0, st>>>(p);
+  const dim3 grid((keep + cache->block - 1) / cache->block, batch->batch * cache->kv_heads);
+  const int rounds = (cache->block * cache->dim / 16 + kThreads - 1) / kThreads;
+  auto go = [&](auto fmt) {
+    constexpr int F = decltype(fmt)::value;
+    if (rounds == 1) kv_gather_kernel<F, 1><<<grid, kThreads, 0, st>>>(p);
+    else if (rounds == 2) kv_gather_kernel<F, 2><<<grid, kThreads, 0, st>>>(p);
+    else kv_gather_kernel<F, 4><<<grid, kThreads, 0, st>>>(p);
+  };
+  if (cache->format == DUPLEX_KV_E4M3) go(std::integral_constant<int, DUPLEX_KV_E4M3>{});
+  else go(std::integral_constant<int, DUPLEX_KV_INT8>{});
   return record_cuda(cudaGetLastError());
 }
