@@ -7,11 +7,12 @@
 // (j < sinks).  One pass over the cache with a running maximum.
 //
 // Bound by the cache's bytes: 2 dim + a little per token and KV head, read once for all query
-// heads that share it.  A warp takes 16 tokens at a time, straight from global memory into the
+// heads that share it.  A warp takes 16 tokens at a time into the
 // registers that mma.sync takes (keys as A[token][dim], values transposed as A[dim][token]; the
-// query rows are the 8 columns, so 8 query heads of a group use every product), with the next 16
-// tokens' loads in flight.  No shared memory on that path: a warp's loads are whole 128-byte rows
-// (keys: halves of them), and the bytes are converted to fp16 in registers, exactly.
+// query rows are the 8 columns, so 8 query heads of a group use every product), out of a ring of its own
+// in shared memory that asynchronous copies fill two steps ahead.  The codes are converted to fp16 in
+// registers, exactly.  (With the next 16 tokens in registers instead, 12 warps an SM and 48 KB in
+// flight, 64 sequences of 12,288 tokens took 172 us.)
 //
 // The work of a launch is one list of 64-token units over (sequence, KV head, row tile); every CTA
 // takes an equal, contiguous piece of it, whatever the lengths, and reads the lengths itself (a
@@ -154,15 +155,42 @@ DEVI void qk(const uint4 (&kr)[2][D / 64], const uint2 (&qf)[NT][D / 16], float 
 template <int D, int NT>
 constexpr int part_floats() { return 8 * NT * (D + 2); }  // O [rows][D], m [rows], l [rows]
 
+// A warp's ring: slots of 16 tokens' keys, values and their two scales.
+template <int D> constexpr int stage_bytes() { return 32 * D + 128; }
+template <int D> constexpr int ring_slots() { return D == 128 ? 3 : 5; }
+
+template <int D, int NT>
+constexpr int front_smem() {
+  const int rings = kWarps * ring_slots<D>() * stage_bytes<D>(), meet = 4 * kWarps * 8 * NT * (D + 4);
+  return rings > meet ? rings : meet;
+}
+
+// A slot's bytes in lines of 128 (8 chunks of 16): the chunks are turned so that the lanes that read
+// together, 2 tokens x 4 chunks of the keys, 4 even tokens x 2 chunks of the values, meet no bank twice.
+template <int D> DEVI int swz_k(int o) { return D == 128 ? o ^ ((o & 128) >> 1) : o; }
+template <int D> DEVI int swz_v(int o) { return o ^ (((o >> (D == 128 ? 8 : 7)) & 3) << 5); }
+
+DEVI void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+DEVI void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+DEVI void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> DEVI void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int D, int NT> constexpr int attend_ctas() { return NT == 1 ? 4 : 3; }  // an SM
+
 template <int D, int FMT, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel(AttendParams p) {
-  constexpr int ROWS = 8 * NT, VW = D / 32, LD = D + 4;
-  extern __shared__ __align__(16) uint8_t dyn[];
-  float(*sO)[LD] = reinterpret_cast<float(*)[LD]>(dyn);  // [kWarps * ROWS]
-  int64_t* off = reinterpret_cast<int64_t*>(dyn + sizeof(float) * kWarps * ROWS * LD);
+__global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_kernel(AttendParams p) {
+  constexpr int ROWS = 8 * NT, VW = D / 32, LD = D + 4, ST = ring_slots<D>(), kStage = stage_bytes<D>();
+  extern __shared__ __align__(128) uint8_t dyn[];
+  float(*sO)[LD] = reinterpret_cast<float(*)[LD]>(dyn);  // [kWarps * ROWS], over the rings
+  int64_t* off = reinterpret_cast<int64_t*>(dyn + front_smem<D, NT>());
   __shared__ float sm[kWarps][ROWS], sl[kWarps][ROWS];
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t* const ring = dyn + warp * (ST * kStage);
   pdl_launch_dependents();
   const Plan plan = make_plan<ROWS>(p, off, gridDim.x);
   int64_t u = (int64_t)blockIdx.x * plan.share;
@@ -220,37 +248,55 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
       return (i < i1 && tok < (i < sp.sink_units ? sp.sink_end : sp.end)) ? tok : -1;
     };
     auto id_of = [&](int tok) -> int { return tok < 0 ? -1 : kv_block_at(c, b, tok / c.block, p.err); };
-    uint4 kr[2][2][D / 64], vr[2][4];
-    float ks[2], vs[2];
-    auto load = [&](int buf, int tok, int id) {
-      if (id < 0) return;
-      const int64_t bh = (int64_t)id * c.heads + h;
-      const int64_t row = bh * c.block + (tok & (c.block - 1));
-      const uint8_t* kp = c.k + row * D + 16 * t;
-      const uint8_t* vp = c.v + row * D + (D / 8) * g;
+    // step i's copies into its ring slot, and the scales beside them (a value scale of -1: nothing here)
+    auto issue = [&](int i, int id) {
+      uint8_t* st = ring + (i % ST) * kStage;
+      if (id >= 0) {
+        const int tok = base_of(i);
+        const int64_t bh = (int64_t)id * c.heads + h;
+        const int64_t row = (bh * c.block + (tok & (c.block - 1))) * D;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const int o = (32 * e + lane) * 16;  // of the 16 tokens' bytes
+          cp_async16(st + swz_k<D>(o), c.k + row + o);
+          cp_async16(st + 16 * D + swz_v<D>(o), c.v + row + o);
+        }
+        if (lane < 2) cp_async4(st + 32 * D + 4 * lane, (lane ? c.v_scale : c.k_scale) + bh);
+      } else if (lane == 0) {
+        *reinterpret_cast<float*>(st + 32 * D + 4) = -1.f;
+      }
+      cp_async_commit();
+    };
+
+    auto step = [&](const uint8_t* st, int tok) {
+      const float ks = *reinterpret_cast<const float*>(st + 32 * D), vs = *reinterpret_cast<const float*>(st + 32 * D + 4);
+      if (vs < 0.f) return;
+      uint4 kr[2][D / 64];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int cc = 0; cc < D / 64; ++cc)
-          kr[buf][i][cc] = __ldg(reinterpret_cast<const uint4*>(kp + (g + 8 * i) * D + 64 * cc));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* q = vp + (2 * t + (i & 1) + 8 * (i >> 1)) * D;
-        if (D == 128) vr[buf][i] = __ldg(reinterpret_cast<const uint4*>(q));
-        else {
-          const uint2 x = __ldg(reinterpret_cast<const uint2*>(q));
-          vr[buf][i] = make_uint4(x.x, x.y, 0, 0);
-        }
-      }
-      ks[buf] = __ldg(c.k_scale + bh);
-      vs[buf] = __ldg(c.v_scale + bh);
-    };
-
-    auto step = [&](int buf, int tok) {
+          kr[i][cc] = *reinterpret_cast<const uint4*>(st + swz_k<D>((g + 8 * i) * D + 64 * cc + 16 * t));
       float S[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) S[nt][0] = S[nt][1] = S[nt][2] = S[nt][3] = 0.f;
-      qk<D, FMT, NT>(kr[buf], qf, S);
+      qk<D, FMT, NT>(kr, qf, S);
+      uint32_t vr[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* q = st + 16 * D + swz_v<D>((2 * t + (i & 1) + 8 * (i >> 1)) * D + (D / 8) * g);
+        if constexpr (D == 128) {
+          const uint4 x = *reinterpret_cast<const uint4*>(q);
+          vr[i][0] = x.x;
+          vr[i][1] = x.y;
+          vr[i][2] = x.z;
+          vr[i][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(q);
+          vr[i][0] = x.x;
+          vr[i][1] = x.y;
+        }
+      }
       const bool plain = tok + 15 <= first_pos && row_base + ROWS <= row_all &&
                          (!p.window || tok > last_pos - p.window || tok + 15 < p.sinks);
       bool grow = false;
@@ -258,7 +304,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          S[nt][j] *= csc[nt][j & 1] * ks[buf];
+          S[nt][j] *= csc[nt][j & 1] * ks;
           if (!plain) {
             const int k = tok + g + 8 * (j >> 1), q = pos[nt][j & 1];
             if (!(k <= q && (!p.window || k > q - p.window || k < p.sinks))) S[nt][j] = -INFINITY;
@@ -270,13 +316,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int k = tok + 2 * t + (i & 1) + 8 * (i >> 1);
-          if (k >= sp.end || (k < lo && k >= p.sinks)) vr[buf][i] = make_uint4(0, 0, 0, 0);
+          if (k >= sp.end || (k < lo && k >= p.sinks)) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[i][w] = 0;
+          }
         }
       }
-      const bool vgrow = vs[buf] > vref;
+      const bool vgrow = vs > vref;
       if (__any_sync(~0u, grow || vgrow)) {
-        const float vf = vgrow ? vref / vs[buf] : 1.f;
-        if (vgrow) vref = vs[buf];
+        const float vf = vgrow ? vref / vs : 1.f;
+        if (vgrow) vref = vs;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float a[2];
@@ -300,7 +349,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
           }
         }
       }
-      const float vf = vs[buf] / vref;
+      const float vf = vs == vref ? 1.f : vs / vref;
       uint32_t pb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -317,7 +366,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
       }
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
-        const uint32_t x0 = (&vr[buf][0].x)[w], x1 = (&vr[buf][1].x)[w], y0 = (&vr[buf][2].x)[w], y1 = (&vr[buf][3].x)[w];
+        const uint32_t x0 = vr[0][w], x1 = vr[1][w], y0 = vr[2][w], y1 = vr[3][w];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t sel = half ? 0x7362u : 0x5140u;  // two tokens' bytes in pairs
@@ -329,21 +378,20 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv_attend_kernel
       }
     };
 
-    int tok0 = base_of(i0), id0 = id_of(tok0);
-    load(0, tok0, id0);
-    int tok1 = base_of(i0 + 1), id1 = id_of(tok1);
-    for (int i = i0; i < i1; i += 2) {
-      load(1, tok1, id1);
-      const int tok2 = base_of(i + 2), id2 = id_of(tok2);
-      if (id0 >= 0) step(0, tok0);
-      load(0, tok2, id2);
-      const int tok3 = base_of(i + 3), id3 = id_of(tok3);
-      if (id1 >= 0) step(1, tok1);
-      tok0 = tok2;
-      id0 = id2;
-      tok1 = tok3;
-      id1 = id3;
+    // ST - 1 steps' copies in flight, one block id further ahead
+#pragma unroll
+    for (int e = 0; e < ST - 1; ++e) issue(i0 + e, id_of(base_of(i0 + e)));
+    int id = id_of(base_of(i0 + ST - 1));
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+      cp_async_wait<ST - 2>();
+      __syncwarp();  // everyone's copies of step i are there, and step i - 1's slot is read
+      issue(i + ST - 1, id);
+      id = id_of(base_of(i + ST));
+      step(ring + (i % ST) * kStage, base_of(i));
     }
+    cp_async_wait<0>();
+    __syncthreads();  // the ring becomes the place where the warps meet
 
     // join the four warps: rows' maxima, then scaled sums through shared memory
 #pragma unroll
@@ -595,14 +643,14 @@ static size_t part_bytes(const KvView& c, int nt) {
 template <int D, int FMT, int NT>
 static int run_attend(const AttendParams& p, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
-  const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = sizeof(float) * kWarps * ROWS * (D + 4) + plan;
+  const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = front_smem<D, NT>() + plan;
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attend_kernel<D, FMT, NT>), 100 * 1024)) return rc;
   // no more CTAs than units there can be
   const int64_t tiles = ((int64_t)p.c.n_rows * p.group) / ROWS + p.c.batch;
   const int64_t units = tiles * p.c.heads * (((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit);
-  const int ctas = (int)std::min(std::min((int64_t)sms * (NT == 1 ? 3 : 2), (int64_t)kMaxCtas), units);
+  const int ctas = (int)std::min(std::min((int64_t)sms * attend_ctas<D, NT>(), (int64_t)kMaxCtas), units);
   kv_attend_kernel<D, FMT, NT><<<ctas, kWarps * 32, smem, st>>>(p);
   if (int rc = record_cuda(cudaGetLastError())) return rc;
   if (ctas > 1) {
