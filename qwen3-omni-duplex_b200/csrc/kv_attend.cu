@@ -14,7 +14,7 @@
 // registers, exactly.  (With the next 16 tokens in registers instead, 12 warps an SM and 48 KB in
 // flight, 64 sequences of 12,288 tokens took 172 us.)
 //
-// The work of a launch is one list of 64-token units over (sequence, KV head, row tile); every CTA
+// The work of a launch is one list of 128-token units over (sequence, KV head, row tile); every CTA
 // takes an equal, contiguous piece of it, whatever the lengths, and reads the lengths itself (a
 // captured launch follows them).  Pieces that share a row tile leave partial results, which
 // kv_combine_kernel joins in order: no atomics, the same bits on each run.
@@ -25,7 +25,8 @@
 namespace duplex {
 
 constexpr int kWarps = 4;
-constexpr int kUnit = 16 * kWarps;   // tokens
+constexpr int kUnit = 32 * kWarps;   // tokens
+constexpr int kWUnit = 16 * kWarps;  // of kv_weights_kernel
 constexpr int kMaxCtas = 148 * 4;
 
 
@@ -155,13 +156,13 @@ DEVI void qk(const uint4 (&kr)[2][D / 64], const uint2 (&qf)[NT][D / 16], float 
 template <int D, int NT>
 constexpr int part_floats() { return 8 * NT * (D + 2); }  // O [rows][D], m [rows], l [rows]
 
-// A warp's ring: slots of 16 tokens' keys, values and their two scales.
-template <int D> constexpr int stage_bytes() { return 32 * D + 128; }
-template <int D> constexpr int ring_slots() { return D == 128 ? 3 : 5; }
+// A warp's ring: slots of 32 tokens' keys, values and their scales.
+template <int D> constexpr int stage_bytes() { return 64 * D + 128; }
+template <int D, int NT> constexpr int ring_slots() { return D == 128 && NT == 1 ? 2 : 3; }
 
 template <int D, int NT>
 constexpr int front_smem() {
-  const int rings = kWarps * ring_slots<D>() * stage_bytes<D>(), meet = 4 * kWarps * 8 * NT * (D + 4);
+  const int rings = kWarps * ring_slots<D, NT>() * stage_bytes<D>(), meet = 4 * kWarps * 8 * NT * (D + 4);
   return rings > meet ? rings : meet;
 }
 
@@ -179,11 +180,11 @@ DEVI void cp_async4(void* dst, const void* src) {
 DEVI void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> DEVI void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int D, int NT> constexpr int attend_ctas() { return NT == 1 ? 4 : 3; }  // an SM
+template <int D, int NT> constexpr int attend_ctas() { return NT == 1 ? 3 : 2; }  // an SM
 
 template <int D, int FMT, int NT>
 __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_kernel(AttendParams p) {
-  constexpr int ROWS = 8 * NT, VW = D / 32, LD = D + 4, ST = ring_slots<D>(), kStage = stage_bytes<D>();
+  constexpr int ROWS = 8 * NT, VW = D / 32, LD = D + 4, ST = ring_slots<D, NT>(), kStage = stage_bytes<D>();
   extern __shared__ __align__(128) uint8_t dyn[];
   float(*sO)[LD] = reinterpret_cast<float(*)[LD]>(dyn);  // [kWarps * ROWS], over the rings
   int64_t* off = reinterpret_cast<int64_t*>(dyn + front_smem<D, NT>());
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* const ring = dyn + warp * (ST * kStage);
+  const int psh = __ffs(c.block) - 1;
   pdl_launch_dependents();
   const Plan plan = make_plan<ROWS>(p, off, gridDim.x);
   int64_t u = (int64_t)blockIdx.x * plan.share;
@@ -230,113 +232,117 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       }
     }
     float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126);
+    float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
+      ad[nt][0] = ad[nt][1] = kShift;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) O[nt][i][j] = 0.f;
     }
 
-    // this warp's 16 tokens of unit i; none if the base is past what the row tile sees
+    // this warp's 32 tokens of unit i, as two parts of 16 (a block holds whole parts): the blocks' ids, or
+    // -1 where no row of the tile looks
     auto base_of = [&](int i) -> int {
-      const int x = i < sp.sink_units ? i * kUnit : sp.lo + (i - sp.sink_units) * kUnit;
-      const int tok = x + 16 * warp;
-      if (p.window && tok + 15 <= first_pos - p.window && tok >= p.sinks) return -1;  // between sinks and window
-      return (i < i1 && tok < (i < sp.sink_units ? sp.sink_end : sp.end)) ? tok : -1;
+      return (i < sp.sink_units ? i * kUnit : sp.lo + (i - sp.sink_units) * kUnit) + 32 * warp;
     };
-    auto id_of = [&](int tok) -> int { return tok < 0 ? -1 : kv_block_at(c, b, tok / c.block, p.err); };
-    // step i's copies into its ring slot, and the scales beside them (a value scale of -1: nothing here)
-    auto issue = [&](int i, int id) {
+    auto ids_of = [&](int i) -> int2 {
+      const int tok = base_of(i), lim = i < i1 ? (i < sp.sink_units ? sp.sink_end : sp.end) : 0;
+      auto id = [&](int k) {
+        const bool gap = p.window && k + 15 <= first_pos - p.window && k >= p.sinks;  // between sinks and window
+        return k < lim && !gap ? kv_block_at(c, b, k >> psh, p.err) : -1;
+      };
+      return make_int2(id(tok), id(tok + 16));
+    };
+    // step i's copies into its ring slot, and the parts' scales beside them (a value scale of -1: nothing here)
+    auto issue = [&](int i, int2 id) {
       uint8_t* st = ring + (i % ST) * kStage;
-      if (id >= 0) {
-        const int tok = base_of(i);
-        const int64_t bh = (int64_t)id * c.heads + h;
-        const int64_t row = (bh * c.block + (tok & (c.block - 1))) * D;
+      const int tok = base_of(i);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          const int o = (32 * e + lane) * 16;  // of the 16 tokens' bytes
-          cp_async16(st + swz_k<D>(o), c.k + row + o);
-          cp_async16(st + 16 * D + swz_v<D>(o), c.v + row + o);
+      for (int x = 0; x < 2; ++x) {
+        const int y = x ? id.y : id.x;
+        if (y >= 0) {
+          const int64_t bh = (int64_t)y * c.heads + h;
+          const int64_t row = (bh * c.block + ((tok + 16 * x) & (c.block - 1))) * D + 16 * lane;
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) {
+            const int o = 16 * D * x + 512 * e + 16 * lane;
+            cp_async16(st + swz_k<D>(o), c.k + row + 512 * e);
+            cp_async16(st + 32 * D + swz_v<D>(o), c.v + row + 512 * e);
+          }
+          if (lane < 2) cp_async4(st + 64 * D + 8 * x + 4 * lane, (lane ? c.v_scale : c.k_scale) + bh);
+        } else if (lane == 0) {
+          *reinterpret_cast<float*>(st + 64 * D + 8 * x + 4) = -1.f;
         }
-        if (lane < 2) cp_async4(st + 32 * D + 4 * lane, (lane ? c.v_scale : c.k_scale) + bh);
-      } else if (lane == 0) {
-        *reinterpret_cast<float*>(st + 32 * D + 4) = -1.f;
       }
       cp_async_commit();
     };
 
     auto step = [&](const uint8_t* st, int tok) {
-      const float ks = *reinterpret_cast<const float*>(st + 32 * D), vs = *reinterpret_cast<const float*>(st + 32 * D + 4);
-      if (vs < 0.f) return;
-      uint4 kr[2][D / 64];
+      const float4 sc = *reinterpret_cast<const float4*>(st + 64 * D);
+      const float ks[2] = {sc.x, sc.z}, vs[2] = {sc.y, sc.w};
+      if (fmaxf(vs[0], vs[1]) < 0.f) return;
+      float S[2][NT][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int x = 0; x < 2; ++x) {
+        uint4 kr[2][D / 64];
 #pragma unroll
-        for (int cc = 0; cc < D / 64; ++cc)
-          kr[i][cc] = *reinterpret_cast<const uint4*>(st + swz_k<D>((g + 8 * i) * D + 64 * cc + 16 * t));
-      float S[NT][4];
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) S[nt][0] = S[nt][1] = S[nt][2] = S[nt][3] = 0.f;
-      qk<D, FMT, NT>(kr, qf, S);
-      uint32_t vr[4][VW];
+          for (int cc = 0; cc < D / 64; ++cc)
+            kr[i][cc] = *reinterpret_cast<const uint4*>(st + swz_k<D>((16 * x + g + 8 * i) * D + 64 * cc + 16 * t));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* q = st + 16 * D + swz_v<D>((2 * t + (i & 1) + 8 * (i >> 1)) * D + (D / 8) * g);
-        if constexpr (D == 128) {
-          const uint4 x = *reinterpret_cast<const uint4*>(q);
-          vr[i][0] = x.x;
-          vr[i][1] = x.y;
-          vr[i][2] = x.z;
-          vr[i][3] = x.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(q);
-          vr[i][0] = x.x;
-          vr[i][1] = x.y;
-        }
+        for (int nt = 0; nt < NT; ++nt) S[x][nt][0] = S[x][nt][1] = S[x][nt][2] = S[x][nt][3] = 0.f;
+        qk<D, FMT, NT>(kr, qf, S[x]);
       }
-      const bool plain = tok + 15 <= first_pos && row_base + ROWS <= row_all &&
-                         (!p.window || tok > last_pos - p.window || tok + 15 < p.sinks);
+      // rows past the last have zeros for a query and are not written: they need no mask
+      const bool plain = tok + 31 <= first_pos && (!p.window || tok > last_pos - p.window || tok + 31 < p.sinks) &&
+                         fminf(vs[0], vs[1]) >= 0.f;
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          S[nt][j] *= csc[nt][j & 1] * ks;
-          if (!plain) {
-            const int k = tok + g + 8 * (j >> 1), q = pos[nt][j & 1];
-            if (!(k <= q && (!p.window || k > q - p.window || k < p.sinks))) S[nt][j] = -INFINITY;
-          }
-          grow |= S[nt][j] > m[nt][j & 1] + kSlack;
-        }
-      if (!plain) {  // what no row sees may hold anything: not even 0 * NaN of it
-        const int lo = p.window ? first_pos - p.window + 1 : 0;
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = tok + 2 * t + (i & 1) + 8 * (i >> 1);
-          if (k >= sp.end || (k < lo && k >= p.sinks)) {
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vr[i][w] = 0;
-          }
+            for (int i = 0; i < 2; ++i) {
+              float& y = S[x][nt][j + 2 * i];
+              y = fmaf(y, csc[nt][j] * ks[x], ad[nt][j]);
+              if (!plain) {
+                const int k = tok + 16 * x + g + 8 * i, q = pos[nt][j];
+                if (!(k <= q && (!p.window || k > q - p.window || k < p.sinks)) || vs[x] < 0.f) y = -INFINITY;
+              }
+            }
+          grow |= fmaxf(fmaxf(S[0][nt][j], S[0][nt][j + 2]), fmaxf(S[1][nt][j], S[1][nt][j + 2])) > lim[nt][j];
         }
-      }
-      const bool vgrow = vs > vref;
-      if (__any_sync(~0u, grow || vgrow)) {
-        const float vf = vgrow ? vref / vs : 1.f;
-        if (vgrow) vref = vs;
+      const float vmax = fmaxf(vs[0], vs[1]);
+      if (__any_sync(~0u, grow || vmax > vref)) {
+        const float vf = vmax > vref ? vref / vmax : 1.f;
+        if (vmax > vref) vref = vmax;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float a[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float x = fmaxf(m[nt][j], fmaxf(S[nt][j], S[nt][j + 2]));
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
-            a[j] = x == m[nt][j] ? 1.f : ex2(m[nt][j] - x);
-            m[nt][j] = x;
+            float y = fmaxf(fmaxf(S[0][nt][j], S[0][nt][j + 2]), fmaxf(S[1][nt][j], S[1][nt][j + 2]));
+            y = fmaxf(y, __shfl_xor_sync(~0u, y, 4));
+            y = fmaxf(y, __shfl_xor_sync(~0u, y, 8));
+            y = fmaxf(y, __shfl_xor_sync(~0u, y, 16));
+            const float top = fmaxf(m[nt][j], y - ad[nt][j]);
+            a[j] = top == m[nt][j] ? 1.f : ex2(m[nt][j] - top);
+            m[nt][j] = top;
+            const float to = kShift - (top == -INFINITY ? 0.f : top), by = to - ad[nt][j];
+            ad[nt][j] = to;
+            lim[nt][j] = top == -INFINITY ? -INFINITY : kShift + kSlack;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              S[x][nt][j] += by;
+              S[x][nt][j + 2] += by;
+            }
             l[nt][j] *= a[j];
             a[j] *= vf;
           }
@@ -349,45 +355,74 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           }
         }
       }
-      const float vf = vs == vref ? 1.f : vs / vref;
-      uint32_t pb[NT][2];
+      const bool same = vs[0] == vref && vs[1] == vref;
+      const float vf[2] = {same ? 1.f : vs[0] / vref, same ? 1.f : vs[1] / vref};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float x[4];
+      for (int x = 0; x < 2; ++x) {
+        uint32_t pb[NT][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float ref = m[nt][j & 1] == -INFINITY ? 0.f : m[nt][j & 1];
-          x[j] = ex2(S[nt][j] - ref + kShift);
-          l[nt][j & 1] += x[j];
-          x[j] *= vf;
+        for (int nt = 0; nt < NT; ++nt) {
+          float y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            y[j] = ex2(S[x][nt][j]);
+            l[nt][j & 1] += y[j];
+            if (!same) y[j] *= vf[x];
+          }
+          pb[nt][0] = movmatrix_trans(f2h(y[0], y[1]));
+          pb[nt][1] = movmatrix_trans(f2h(y[2], y[3]));
         }
-        pb[nt][0] = movmatrix_trans(f2h(x[0], x[1]));
-        pb[nt][1] = movmatrix_trans(f2h(x[2], x[3]));
-      }
+        uint32_t vr[4][VW];
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const uint32_t x0 = vr[0][w], x1 = vr[1][w], y0 = vr[2][w], y1 = vr[3][w];
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* q = st + 32 * D + swz_v<D>((16 * x + 2 * t + (i & 1) + 8 * (i >> 1)) * D + (D / 8) * g);
+          if constexpr (D == 128) {
+            const uint4 y = *reinterpret_cast<const uint4*>(q);
+            vr[i][0] = y.x;
+            vr[i][1] = y.y;
+            vr[i][2] = y.z;
+            vr[i][3] = y.w;
+          } else {
+            const uint2 y = *reinterpret_cast<const uint2*>(q);
+            vr[i][0] = y.x;
+            vr[i][1] = y.y;
+          }
+        }
+        if (!plain) {  // what no row sees may hold anything: not even 0 * NaN of it
+          const int lo = p.window ? first_pos - p.window + 1 : 0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362u : 0x5140u;  // two tokens' bytes in pairs
-          const uint32_t a = __byte_perm(x0, x1, sel), e = __byte_perm(y0, y1, sel);
-          const uint32_t a0 = KvFmt<FMT>::lo(a), a1 = KvFmt<FMT>::hi(a), a2 = KvFmt<FMT>::lo(e), a3 = KvFmt<FMT>::hi(e);
+          for (int i = 0; i < 4; ++i) {
+            const int k = tok + 16 * x + 2 * t + (i & 1) + 8 * (i >> 1);
+            if (k >= sp.end || (k < lo && k >= p.sinks) || vs[x] < 0.f) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(O[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+              for (int w = 0; w < VW; ++w) vr[i][w] = 0;
+            }
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362u : 0x5140u;  // two tokens' bytes in pairs
+            const uint32_t a = __byte_perm(vr[0][w], vr[1][w], sel), e = __byte_perm(vr[2][w], vr[3][w], sel);
+            const uint32_t a0 = KvFmt<FMT>::lo(a), a1 = KvFmt<FMT>::hi(a), a2 = KvFmt<FMT>::lo(e), a3 = KvFmt<FMT>::hi(e);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(O[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+          }
         }
       }
     };
 
-    // ST - 1 steps' copies in flight, one block id further ahead
+    // ST - 1 steps' copies in flight, the block ids one step further ahead
 #pragma unroll
-    for (int e = 0; e < ST - 1; ++e) issue(i0 + e, id_of(base_of(i0 + e)));
-    int id = id_of(base_of(i0 + ST - 1));
+    for (int e = 0; e < ST - 1; ++e) issue(i0 + e, ids_of(i0 + e));
+    int2 id = ids_of(i0 + ST - 1);
 #pragma unroll 1
     for (int i = i0; i < i1; ++i) {
       cp_async_wait<ST - 2>();
       __syncwarp();  // everyone's copies of step i are there, and step i - 1's slot is read
       issue(i + ST - 1, id);
-      id = id_of(base_of(i + ST));
+      id = ids_of(i + ST);
       step(ring + (i % ST) * kStage, base_of(i));
     }
     cp_async_wait<0>();
@@ -550,18 +585,18 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
   const KvSeq s = kv_seq(c, b);
-  const int tile = blockIdx.x * (U * kUnit), start = s.n - s.rows;
+  const int tile = blockIdx.x * (U * kWUnit), start = s.n - s.rows;
   if (tile >= s.n) return;
   // the sequence's rows that see a token of the tile
   int t0 = max(tile - start, 0), t1 = s.rows;
-  if (p.window && tile >= p.sinks) t1 = (int)min((int64_t)t1, (int64_t)tile + U * kUnit - 1 + p.window - start);
+  if (p.window && tile >= p.sinks) t1 = (int)min((int64_t)t1, (int64_t)tile + U * kWUnit - 1 + p.window - start);
   if (t0 >= t1) return;
   uint4 kr[U][2][D / 64];
   float ks[U], sum[U][2];
   int64_t at[U];  // the warp's 16 tokens' slot, or -1
 #pragma unroll
   for (int x = 0; x < U; ++x) {
-    const int tok = tile + x * kUnit + 16 * warp;
+    const int tok = tile + x * kWUnit + 16 * warp;
     const bool hidden = tok >= s.n || (p.window && tok + 15 <= start - p.window && tok >= p.sinks);
     const int id = hidden ? -1 : kv_block_at(c, b, tok / c.block, p.err);
     const int64_t bh = (int64_t)max(id, 0) * c.heads + h;
@@ -609,7 +644,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
         qk<D, FMT, 1>(kr[x], qf, S);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int k = tile + x * kUnit + 16 * warp + g + 8 * (j >> 1), q = pos[j & 1];
+          const int k = tile + x * kWUnit + 16 * warp + g + 8 * (j >> 1), q = pos[j & 1];
           if (k <= q && (!p.window || k > q - p.window || k < p.sinks))
             sum[x][j >> 1] += ex2(S[0][j] * (sc[j & 1] * ks[x]) - ls[j & 1]);
         }
@@ -623,7 +658,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
       float y = sum[x][i];
       y += __shfl_xor_sync(~0u, y, 1);
       y += __shfl_xor_sync(~0u, y, 2);
-      const int k = tile + x * kUnit + 16 * warp + g + 8 * i;
+      const int k = tile + x * kWUnit + 16 * warp + g + 8 * i;
       // one addition to a token's sum, so its order does not matter; sequences that share a block may add to the same one
       if (t == 0 && at[x] >= 0 && k < s.n) atomicAdd(c.weights + at[x] + g + 8 * i, y);
     }
@@ -677,7 +712,7 @@ static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
                                                : run_attend<D, FMT, 2>(p, st);
   if (rc || !p.c.weights) return rc;
   const bool few = (int64_t)p.c.n_rows * p.group <= (int64_t)p.c.batch * kRowChunk;
-  const int tokens = few ? 2 * kUnit : kUnit;
+  const int tokens = few ? 2 * kWUnit : kWUnit;
   const dim3 grid((unsigned)(((int64_t)p.c.width * p.c.block + tokens - 1) / tokens), p.c.heads, p.c.batch);
   if (few) kv_weights_kernel<D, FMT, 2><<<grid, kWarps * 32, 0, st>>>(p);
   else kv_weights_kernel<D, FMT, 1><<<grid, kWarps * 32, 0, st>>>(p);
