@@ -215,35 +215,6 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
     const int last_pos = s.n - s.rows + last_row / p.group;
     const Span sp = span_of<kUnit>(p, first_pos, last_pos, s.n);
 
-    // query rows: as the product's columns, lane (g, t) loads row g and accumulates rows 2t, 2t + 1
-    uint2 qf[NT][D / 16];
-    float csc[NT][2];
-    int pos[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int rr = row_base + nt * 8 + g;
-      const bool live = rr < row_all;
-      const float undo = load_q<D>(p, s.row0 + (live ? rr / p.group : 0), h * p.group + (live ? rr % p.group : 0), t, live, qf[nt]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        csc[nt][j] = __shfl_sync(~0u, undo, (2 * t + j) * 4) * p.scale_log2;
-        const int r2 = row_base + nt * 8 + 2 * t + j;
-        pos[nt][j] = r2 < row_all ? s.n - s.rows + r2 / p.group : -1;
-      }
-    }
-    float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126);
-    float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
-      ad[nt][0] = ad[nt][1] = kShift;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) O[nt][i][j] = 0.f;
-    }
-
     // this warp's 32 tokens of unit i, as two parts of 16 (a block holds whole parts): the blocks' ids, or
     // -1 where no row of the tile looks
     auto base_of = [&](int i) -> int {
@@ -280,6 +251,40 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       }
       cp_async_commit();
     };
+
+    // ST - 1 steps' copies in flight, the block ids one step further ahead
+#pragma unroll
+    for (int e = 0; e < ST - 1; ++e) issue(i0 + e, ids_of(i0 + e));
+    int2 id = ids_of(i0 + ST - 1);
+
+    // query rows: as the product's columns, lane (g, t) loads row g and accumulates rows 2t, 2t + 1
+    uint2 qf[NT][D / 16];
+    float csc[NT][2];
+    int pos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int rr = row_base + nt * 8 + g;
+      const bool live = rr < row_all;
+      const float undo = load_q<D>(p, s.row0 + (live ? rr / p.group : 0), h * p.group + (live ? rr % p.group : 0), t, live, qf[nt]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        csc[nt][j] = __shfl_sync(~0u, undo, (2 * t + j) * 4) * p.scale_log2;
+        const int r2 = row_base + nt * 8 + 2 * t + j;
+        pos[nt][j] = r2 < row_all ? s.n - s.rows + r2 / p.group : -1;
+      }
+    }
+    float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126);
+    float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+      ad[nt][0] = ad[nt][1] = kShift;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) O[nt][i][j] = 0.f;
+    }
 
     auto step = [&](const uint8_t* st, int tok) {
       const float4 sc = *reinterpret_cast<const float4*>(st + 64 * D);
@@ -413,10 +418,6 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       }
     };
 
-    // ST - 1 steps' copies in flight, the block ids one step further ahead
-#pragma unroll
-    for (int e = 0; e < ST - 1; ++e) issue(i0 + e, ids_of(i0 + e));
-    int2 id = ids_of(i0 + ST - 1);
 #pragma unroll 1
     for (int i = i0; i < i1; ++i) {
       cp_async_wait<ST - 2>();
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
 template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p, int ctas) {
   constexpr int ROWS = 8 * NT, RC = 512 / D;  // rows of a CTA
-  extern __shared__ __align__(16) uint8_t dyn[];
+  extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ float s_m[RC], s_l[RC];
   int64_t* off = reinterpret_cast<int64_t*>(dyn);
   const KvView& c = p.c;

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::bars);
   uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *s_full = bar + 8, *p_ready = bar + 10,
-           *o_full = bar + 12, *drain = bar + 13, *q_full = bar + 14;
+           *o_full = bar + 12, *drain = bar + 13, *q_full = bar + 14, *p_half = bar + 16;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + i, 8);
@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       mbar_init(v_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(p_ready + i, 4);
+      mbar_init(p_half + i, 4);
     }
     mbar_init(o_full, 1);
     mbar_init(drain, 1);
@@ -279,7 +280,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
   pdl_launch_dependents();
 
   auto wait = [&](uint64_t* b, uint32_t n) -> bool {  // the n-th completion (from 0) of a barrier, by a whole warp
-    const bool ok = mbar_wait_bounded(b, n & 1, &s_abort);
+    bool ok = mbar_try_wait(b, n & 1);
+    if (__all_sync(~0u, ok)) return true;
+    ok = mbar_wait_bounded(b, n & 1, &s_abort);
     if (!ok) set_error(p.err, DUPLEX_DEVERR_TIMEOUT);
     return __all_sync(~0u, ok) != 0;
   };
@@ -300,61 +303,71 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
     uint8_t* const q_tile = sm + L::q + mt * L::kTile;
     uint32_t n_s = 0, n_o = 0;  // completions of s_full[mt], o_full so far
     bool ok = true;
-    for (; ok && u < u_end; u += x.len) {
+    // query rows on their way: 8 rows at a time, 4 lanes a row; rows 16 i .. + 15 of the warp's 32
+    uint4 raw[2][D / 32];
+    auto load_rows = [&](int i) {
+      const int row_all = x.row_all(p.group);
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        const int r2 = x.row_base() + 32 * warp + 16 * i + 8 * e2 + (lane & 7), t2 = p.by_group(r2);
+        const uint8_t* src = static_cast<const uint8_t*>(p.q) + 16 * (lane >> 3);
+        const bool in = r2 < row_all;
+        if (in) src += 2 * ((int64_t)(x.it.s.row0 + t2) * p.q_row + (int64_t)(x.h * p.group + r2 - t2 * p.group) * p.q_head);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+          raw[e2][e] = in ? __ldg(reinterpret_cast<const uint4*>(src + 64 * e)) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    // ... and to shared memory, as fp16 scaled by a power of two (kv_attend.cu: load_q)
+    auto put_rows = [&](int i) {
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        const int row = (32 * warp + 16 * i + 8 * e2 + (lane & 7)) & 127;
+        float amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t y = (&raw[e2][e].x)[w];
+            const float2 f = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(y) : act2<DUPLEX_DTYPE_BF16>(y);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 8));
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 16));
+        const int ex = (int)(__float_as_uint(amax) >> 23) - 127;
+        const int up = (amax == 0.f || ex == 128) ? 0 : min(14 - ex, 126);
+        const float f = p.scale_log2 < 0.f ? -pow2f(up) : pow2f(up);  // its sign goes with the row
+        if (lane < 8) s_undo[32 * warp + 16 * i + 8 * e2 + lane] = pow2f(-up);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          uint4 y;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t z = (&raw[e2][e].x)[w];
+            const float2 a = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(z) : act2<DUPLEX_DTYPE_BF16>(z);
+            (&y.x)[w] = f2h(a.x * f, a.y * f);
+          }
+          const int ch = 4 * e + (lane >> 3);  // of the row's D / 8
+          *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * L::kHalf + sw128(row, ch & 7)) = y;
+        }
+      }
+    };
+    PromptRef ref{};
+    auto next = [&]() {
       find_piece(pp, u, u_end, pi, x);
+      ref = pp.ref[x.it.b * c.heads + x.h];
+      if (x.n > 0) load_rows(0);
+    };
+    if (u < u_end) next();
+    while (ok && u < u_end) {
       const int n = x.n, row_base = x.row_base(), row_all = x.row_all(p.group);
       const KvSeq s = x.it.s;
       const int rr = row_base + tid, t_row = p.by_group(rr);
       const bool live = rr < row_all;
-      const PromptRef ref = pp.ref[x.it.b * c.heads + x.h];
-      // ---- query rows to shared memory, as fp16 scaled by a power of two (kv_attend.cu: load_q): 8 rows
-      // at a time, 4 lanes a row
       if (n > 0) {
-#pragma unroll 1
-        for (int i = 0; i < 4; i += 2) {
-          uint4 raw[2][D / 32];
-#pragma unroll
-          for (int e2 = 0; e2 < 2; ++e2) {
-            const int r2 = row_base + 32 * warp + 8 * (i + e2) + (lane & 7), t2 = p.by_group(r2);
-            const uint8_t* src = static_cast<const uint8_t*>(p.q) + 16 * (lane >> 3);
-            const bool in = r2 < row_all;
-            if (in) src += 2 * ((int64_t)(s.row0 + t2) * p.q_row + (int64_t)(x.h * p.group + r2 - t2 * p.group) * p.q_head);
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e)
-              raw[e2][e] = in ? __ldg(reinterpret_cast<const uint4*>(src + 64 * e)) : make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int e2 = 0; e2 < 2; ++e2) {
-            const int row = (32 * warp + 8 * (i + e2) + (lane & 7)) & 127;
-            float amax = 0.f;
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e)
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint32_t y = (&raw[e2][e].x)[w];
-                const float2 f = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(y) : act2<DUPLEX_DTYPE_BF16>(y);
-                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-              }
-            amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 8));
-            amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 16));
-            const int ex = (int)(__float_as_uint(amax) >> 23) - 127;
-            const int up = (amax == 0.f || ex == 128) ? 0 : min(14 - ex, 126);
-            const float f = p.scale_log2 < 0.f ? -pow2f(up) : pow2f(up);  // its sign goes with the row
-            if (lane < 8) s_undo[32 * warp + 8 * (i + e2) + lane] = pow2f(-up);
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) {
-              uint4 y;
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint32_t z = (&raw[e2][e].x)[w];
-                const float2 a = p.act == DUPLEX_DTYPE_F16 ? act2<DUPLEX_DTYPE_F16>(z) : act2<DUPLEX_DTYPE_BF16>(z);
-                (&y.x)[w] = f2h(a.x * f, a.y * f);
-              }
-              const int ch = 4 * e + (lane >> 3);  // of the row's D / 8
-              *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * L::kHalf + sw128(row, ch & 7)) = y;
-            }
-          }
-        }
+        put_rows(0);
+        load_rows(1);
+        put_rows(1);
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
@@ -463,6 +476,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
             tc_wait_ld();
             if (q == 0) tmem_ld32(ts + 64, va);
             part(vb, q + 1);
+            if (q == 0) {  // the products of the first 64 tokens can start
+              tc_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_half + mt);
+            }
           }
         }
         l += ls.x + ls.y;
@@ -471,12 +490,19 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready + mt);
       }
-      // ---- the row's result.  Both tiles wait for all products: the query rows' place is free then.
+      // ---- the row's result, with the next piece's rows on their way.  Both tiles wait for all products:
+      // the query rows' place is free then.
+      if (!ok) break;
+      const bool mine_w = x.whole, first = u == u_begin;
+      const int h = x.h;
+      const float vref = ref.v;
+      u += x.len;
+      if (u < u_end) next();
       if (!ok || (n > 0 && !(ok = wait(o_full, n_o)))) break;
       tc_fence_after();
       if (mine) {
-        const float inv = x.whole ? (l == 0.f ? 0.f : ref.v / l) : ref.v;
-        float* part = p.part + (2 * (int64_t)blockIdx.x + (u == u_begin ? 0 : 1)) * prompt_part<D>();
+        const float inv = mine_w ? (l == 0.f ? 0.f : vref / l) : vref;
+        float* part = p.part + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * prompt_part<D>();
         // a whole item's rows go through the query rows' place, to be written 16 lanes a row; a piece's
         // [dim / 4][row] as they come
 #pragma unroll 1
@@ -495,7 +521,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
             float o[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[e + k]) * inv;
-            if (x.whole) {
+            if (mine_w) {
               const uint2 y = pack4(p.act, make_float4(o[0], o[1], o[2], o[3])), z = pack4(p.act, make_float4(o[4], o[5], o[6], o[7]));
               const int ch = 4 * q + e / 8;
               *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * L::kHalf + sw128(tid & 127, ch & 7)) = make_uint4(y.x, y.y, z.x, z.y);
@@ -507,18 +533,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
           }
         }
         __syncwarp();
-        if (x.whole) {
+        if (mine_w) {
           constexpr int LR = D / 8, RI = 32 / LR;  // lanes a row, rows a store
 #pragma unroll 4
           for (int i = 0; i < 32; i += RI) {
             const int row = 32 * warp + i + lane / LR, ch = lane % LR, r2 = row_base + row, t2 = p.by_group(r2);
             if (r2 < row_all) {
-              const int64_t o = (int64_t)(s.row0 + t2) * p.heads + x.h * p.group + r2 - t2 * p.group;
+              const int64_t o = (int64_t)(s.row0 + t2) * p.heads + h * p.group + r2 - t2 * p.group;
               *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + 2 * (o * D + 8 * ch)) =
                   *reinterpret_cast<const uint4*>(q_tile + (ch >> 3) * L::kHalf + sw128(row & 127, ch & 7));
             }
           }
-          if (live) p.lse[(int64_t)(s.row0 + t_row) * p.heads + x.h * p.group + rr - t_row * p.group] = lse_of(m, l);
+          if (live) p.lse[(int64_t)(s.row0 + t_row) * p.heads + h * p.group + rr - t_row * p.group] = lse_of(m, l);
           __syncwarp();
         } else if (live) {
           part[kPRows * D + tid] = m;
@@ -625,11 +651,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         }
         done(s_full + mt);
       };
-      auto pv = [&](int mt, uint32_t slot, bool more) {
+      auto pv = [&](int mt, uint32_t slot, bool more, int half) {
         const uint64_t dv = smem_desc_sw128(sv + slot * L::kTile, L::kHalf);
 #pragma unroll
-        for (int y = 0; y < kPTok / 16; ++y)
+        for (int e = 0; e < kPTok / 32; ++e) {
+          const int y = half * (kPTok / 32) + e;
           if (elect_one()) umma_ts(t_o(mt), t_s(mt) + 8 * y, dv + y * (2048 >> 4), id_pv, more || y != 0);
+        }
+      };
+      // tile mt's output of tile j, as its probabilities come
+      auto out = [&](int mt, uint32_t slot, bool more, uint32_t k) {
+        if (!wait(p_half + mt, k)) return false;
+        tc_fence_after();
+        pv(mt, slot, more, 0);
+        if (!wait(p_ready + mt, k)) return false;
+        tc_fence_after();
+        pv(mt, slot, more, 1);
+        return true;
       };
       uint32_t n_tile = 0, n1 = 0, n_q = 0;  // tiles so far (p_ready[0], the rings); completions of p_ready[1], q_full
       bool ok = true;
@@ -644,21 +682,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         done(k_empty + (n_tile & 1));
         for (int j = 0; j < n; ++j) {
           const uint32_t cnt = n_tile + j, slot = cnt & 1, nslot = slot ^ 1;
-          if (!(ok = wait(v_full + slot, cnt >> 1) && wait(p_ready, cnt))) break;
-          tc_fence_after();
-          pv(0, slot, j > 0);
-          if (j + 1 < n) {
-            if (!(ok = wait(k_full + nslot, (cnt + 1) >> 1))) break;
-            tc_fence_after();
-            qk(0, nslot);
-          }
-          if (x.two) {
-            if (!(ok = wait(p_ready + 1, n1 + j))) break;
-            tc_fence_after();
-            pv(1, slot, j > 0);
-          }
+          const bool more = j + 1 < n;
+          if (!(ok = wait(v_full + slot, cnt >> 1) && (!more || wait(k_full + nslot, (cnt + 1) >> 1)))) break;
+          if (!(ok = out(0, slot, j > 0, cnt))) break;
+          if (more) qk(0, nslot);
+          if (x.two && !(ok = out(1, slot, j > 0, n1 + j))) break;
           done(v_empty + slot);
-          if (j + 1 < n) {
+          if (more) {
             if (x.two) qk(1, nslot);
             done(k_empty + nslot);
           }
