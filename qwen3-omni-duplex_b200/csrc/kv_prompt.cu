@@ -20,6 +20,7 @@
 // joins the items that a cut went through.  The roles meet only at the barriers of the buffers they
 // share, so the next item's keys are under way while the last one's rows are written.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attend.cuh"
 #include "umma.cuh"
@@ -179,7 +180,8 @@ DEVI int pair_of(const PromptItem* list, int pairs, int64_t u) {
 // [dim / 64][row][64 dims] are K-major; V [dim / 64][token][64 dims], the same layout, is MN-major.
 template <int D> struct PromptSmem {
   static constexpr uint32_t kHalf = 128 * 128, kTile = D / 64 * kHalf;
-  static constexpr uint32_t q = 0, k = 2 * kTile, v = k + 2 * kTile, undo = v + 2 * kTile, bars = undo + kPRows * 4;
+  static constexpr uint32_t q = 0, k = 2 * kTile, v = k + 2 * kTile, stage = v + 2 * kTile, undo = stage + 8 * 32 * 64,
+                            bars = undo + kPRows * 4;
   static constexpr uint32_t bytes = bars + 256 + 1024;
 };
 
@@ -236,7 +238,7 @@ DEVI void find_piece(const PromptParams& pp, int64_t u, int64_t u_end, int& pi, 
 }
 
 // Registers: 640 threads start with 96 each, 61,440; the softmax warps take what the others leave.
-constexpr int kRegSoftmax = 144, kRegConvert = 64, kRegMma = 56;
+constexpr int kRegSoftmax = 144, kRegConvert = 64, kRegMma = 64;
 static_assert(256 * kRegSoftmax + 256 * kRegConvert + 128 * kRegMma <= kPThreads * 96, "register split");
 
 template <int D, int FMT>
@@ -247,6 +249,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
   float* const s_undo = reinterpret_cast<float*>(sm + L::undo);
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
+  __shared__ int2 s_piece;  // for the products: the piece's tiles and whether its second row tile has rows; -1: no more
   const AttendParams& p = pp.a;
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -358,20 +361,27 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       ref = pp.ref[x.it.b * c.heads + x.h];
       if (x.n > 0) load_rows(0);
     };
-    if (u < u_end) next();
+    auto give_rows = [&]() {
+      if (x.n <= 0) return;
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        if (i) load_rows(i);
+        put_rows(i);
+      }
+      if (tid == 0) s_piece = make_int2(x.n, x.two);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    if (u < u_end) {
+      next();
+      give_rows();
+    }
     while (ok && u < u_end) {
       const int n = x.n, row_base = x.row_base(), row_all = x.row_all(p.group);
       const KvSeq s = x.it.s;
       const int rr = row_base + tid, t_row = p.by_group(rr);
       const bool live = rr < row_all;
-      if (n > 0) {
-        put_rows(0);
-        load_rows(1);
-        put_rows(1);
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-      }
       const int pos = live ? s.n - s.rows + t_row : -1;
       const int wlo = p.window ? pos - p.window : -1;  // tokens k > wlo, or k < sinks
       const int row_lo = row_base + mt * 128, row_hi = min(row_lo + 128, row_all);
@@ -490,71 +500,88 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready + mt);
       }
-      // ---- the row's result, with the next piece's rows on their way.  Both tiles wait for all products:
-      // the query rows' place is free then.
+      // ---- the row's result.  Once all products are done (both tiles wait for them) the next piece's rows
+      // take the query rows' place, so its first scores are computed under the writing of this one's results.
       if (!ok) break;
-      const bool mine_w = x.whole, first = u == u_begin;
+      const bool whole = x.whole, first = u == u_begin;
       const int h = x.h;
-      const float vref = ref.v;
+      const float inv = whole ? (l == 0.f ? 0.f : ref.v / l) : ref.v;
       u += x.len;
       if (u < u_end) next();
-      if (!ok || (n > 0 && !(ok = wait(o_full, n_o)))) break;
+      if (n > 0 && !(ok = wait(o_full, n_o))) break;
       tc_fence_after();
+      if (u < u_end) give_rows();
       if (mine) {
-        const float inv = mine_w ? (l == 0.f ? 0.f : vref / l) : vref;
-        float* part = p.part + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * prompt_part<D>();
-        // a whole item's rows go through the query rows' place, to be written 16 lanes a row; a piece's
-        // [dim / 4][row] as they come
+        if (whole) {  // through 2 KB a warp, 32 dims at a time, to be written 4 lanes a row
+          uint8_t* const stage = sm + L::stage + warp * 2048;
+          auto at = [&](int row, int ch) { return stage + row * 64 + ((ch ^ ((row >> 1) & 3)) << 4); };
+          auto put_out = [&](auto act) {
+            constexpr int A = decltype(act)::value;
 #pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t v[32];
-          __syncwarp();
-          if (n > 0) {
-            tmem_ld32(to + 32 * q, v);
-            tc_wait_ld();
-          } else {
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t v[32];
+              __syncwarp();
+              if (n > 0) {
+                tmem_ld32(to + 32 * q, v);
+                tc_wait_ld();
+              } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0;
-          }
+                for (int e = 0; e < 32; ++e) v[e] = 0;
+              }
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float o[8];
+              for (int e = 0; e < 32; e += 8) {
+                float o[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[e + k]) * inv;
-            if (mine_w) {
-              const uint2 y = pack4(p.act, make_float4(o[0], o[1], o[2], o[3])), z = pack4(p.act, make_float4(o[4], o[5], o[6], o[7]));
-              const int ch = 4 * q + e / 8;
-              *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * L::kHalf + sw128(tid & 127, ch & 7)) = make_uint4(y.x, y.y, z.x, z.y);
-            } else {
-              float4* to4 = reinterpret_cast<float4*>(part) + (8 * q + e / 4) * kPRows + tid;
-              to4[0] = make_float4(o[0], o[1], o[2], o[3]);
-              to4[kPRows] = make_float4(o[4], o[5], o[6], o[7]);
+                for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[e + k]) * inv;
+                const uint2 y = pack4(A, make_float4(o[0], o[1], o[2], o[3])), z = pack4(A, make_float4(o[4], o[5], o[6], o[7]));
+                *reinterpret_cast<uint4*>(at(lane, e / 8)) = make_uint4(y.x, y.y, z.x, z.y);
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int row = 8 * i + (lane >> 2), r2 = row_base + 32 * warp + row, t2 = p.by_group(r2);
+                if (r2 < row_all) {
+                  const int64_t o = (int64_t)(s.row0 + t2) * p.heads + h * p.group + r2 - t2 * p.group;
+                  *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + 2 * (o * D + 32 * q + 8 * (lane & 3))) =
+                      *reinterpret_cast<const uint4*>(at(row, lane & 3));
+                }
+              }
             }
-          }
-        }
-        __syncwarp();
-        if (mine_w) {
-          constexpr int LR = D / 8, RI = 32 / LR;  // lanes a row, rows a store
-#pragma unroll 4
-          for (int i = 0; i < 32; i += RI) {
-            const int row = 32 * warp + i + lane / LR, ch = lane % LR, r2 = row_base + row, t2 = p.by_group(r2);
-            if (r2 < row_all) {
-              const int64_t o = (int64_t)(s.row0 + t2) * p.heads + h * p.group + r2 - t2 * p.group;
-              *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + 2 * (o * D + 8 * ch)) =
-                  *reinterpret_cast<const uint4*>(q_tile + (ch >> 3) * L::kHalf + sw128(row & 127, ch & 7));
-            }
-          }
+          };
+          if (p.act == DUPLEX_DTYPE_F16) put_out(std::integral_constant<int, DUPLEX_DTYPE_F16>{});
+          else put_out(std::integral_constant<int, DUPLEX_DTYPE_BF16>{});
           if (live) p.lse[(int64_t)(s.row0 + t_row) * p.heads + h * p.group + rr - t_row * p.group] = lse_of(m, l);
-          __syncwarp();
-        } else if (live) {
+        } else {  // a piece's as they come, [dim / 4][row]
+          float* part = p.part + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * prompt_part<D>();
+          float4* to4 = reinterpret_cast<float4*>(part) + tid;
+#pragma unroll 1
+          for (int q = 0; q < D / 16; ++q, to4 += 4 * kPRows) {
+            uint32_t v[16];
+            __syncwarp();
+            if (n > 0) {
+              tmem_ld16(to + 16 * q, v);
+              tc_wait_ld();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) v[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              to4[e * kPRows] = make_float4(__uint_as_float(v[4 * e]) * inv, __uint_as_float(v[4 * e + 1]) * inv,
+                                            __uint_as_float(v[4 * e + 2]) * inv, __uint_as_float(v[4 * e + 3]) * inv);
+          }
           part[kPRows * D + tid] = m;
           part[kPRows * D + kPRows + tid] = l;
         }
+        __syncwarp();
         tc_fence_before();
         n_s += n;
       }
       if (n > 0) ++n_o;
     }
+    if (tid == 0) s_piece = make_int2(-1, 0);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
   } else if (warp < 16) {
     // ---------------------------------------------------------------- keys and values
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegConvert));
@@ -671,32 +698,32 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       };
       uint32_t n_tile = 0, n1 = 0, n_q = 0;  // tiles so far (p_ready[0], the rings); completions of p_ready[1], q_full
       bool ok = true;
-      for (; ok && u < u_end; u += x.len) {
-        find_piece(pp, u, u_end, pi, x);
-        const int n = x.n;
-        if (n <= 0) continue;
-        if (!(ok = wait(k_full + (n_tile & 1), n_tile >> 1) && wait(q_full, n_q))) break;
+      for (; ok; ++n_q) {
+        if (!(ok = wait(q_full, n_q))) break;
+        const int n = s_piece.x;
+        const int two = s_piece.y;
+        if (n < 0) break;
+        if (!(ok = wait(k_full + (n_tile & 1), n_tile >> 1))) break;
         tc_fence_after();
-        qk(0, n_tile & 1);
-        if (x.two) qk(1, n_tile & 1);
+#pragma unroll 1
+        for (int mt = 0; mt <= two; ++mt) qk(mt, n_tile & 1);
         done(k_empty + (n_tile & 1));
         for (int j = 0; j < n; ++j) {
           const uint32_t cnt = n_tile + j, slot = cnt & 1, nslot = slot ^ 1;
           const bool more = j + 1 < n;
           if (!(ok = wait(v_full + slot, cnt >> 1) && (!more || wait(k_full + nslot, (cnt + 1) >> 1)))) break;
-          if (!(ok = out(0, slot, j > 0, cnt))) break;
-          if (more) qk(0, nslot);
-          if (x.two && !(ok = out(1, slot, j > 0, n1 + j))) break;
-          done(v_empty + slot);
-          if (more) {
-            if (x.two) qk(1, nslot);
-            done(k_empty + nslot);
+#pragma unroll 1
+          for (int mt = 0; ok && mt <= two; ++mt) {
+            if (!(ok = out(mt, slot, j > 0, (mt ? n1 : n_tile) + j))) break;
+            if (mt == two) done(v_empty + slot);
+            if (more) qk(mt, nslot);
           }
+          if (!ok) break;
+          if (more) done(k_empty + nslot);
         }
         if (ok) done(o_full);
         n_tile += n;
-        if (x.two) n1 += n;
-        ++n_q;
+        if (two) n1 += n;
       }
       // no product may still be running when tensor memory goes
       done(drain);
