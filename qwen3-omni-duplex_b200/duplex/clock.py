@@ -12,6 +12,14 @@ the hidden state stays finite through the stack:
        -> h1  = h + W_o . qkv[:, :4096]        (K 4096)
        -> h'  = h1 + MoE(rms(h1))              (router + 128-expert top-8 int4 MoE)
 
+`attach_cache()` puts the attention core back for the 5-kernel form: each of the T
+tokens is the next one of a stream of its own, its k and v rows go into an 8-bit paged
+cache per layer, and o reads the attention over that cache (whole context, or a sliding
+window with sinks; without rotary embedding, as the q and k rows come).  `evict()` keeps
+the tokens that were looked at most:
+
+       -> kv_append(k, v);  h1 = h + W_o . kv_attend(q)
+
 By default the whole stack is ONE launch of the persistent clock-path kernel
 (`duplex_stack_forward`: one CTA per SM, grid barriers between the phases of a
 layer, weights streamed ahead across phases).  `fused=False` runs the same math
@@ -29,6 +37,7 @@ import torch
 
 from duplex import _lib, synth
 from duplex.streaming.fused_packed_moe import FusedPackedMoE
+from duplex.streaming.kv_cache import PackedKVCache
 from duplex.streaming.triton_dequant_gemv import TritonPackedLinear
 
 RMS_EPS = 1e-6  # Thinker text config rms_norm_eps
@@ -153,6 +162,32 @@ class ClockLayer:
         self.qkv, self.o, self.moe = qkv, o, moe
 
 
+class StreamCaches:
+    """The KV caches of a stack's layers, one set of block tables and lengths: T streams of at
+    most `tokens` tokens each (a second set of blocks beside it if they can be evicted)."""
+
+    def __init__(self, n_layers, T, tokens, heads, kv_heads, head_dim, block, fmt, window, sinks,
+                 evictable, device):
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.window, self.sinks, self.evictable = window, sinks, evictable
+        W = -(-tokens // block)
+        sets = 2 if evictable else 1
+        self.layers = [PackedKVCache(sets * T * W, kv_heads, head_dim, block, fmt, evictable, device)
+                       for _ in range(n_layers)]
+        ids = torch.arange(sets * T * W, dtype=torch.int32, device=device).view(sets, T, W)
+        self.table, self.spare = ids[0].clone(), ids[-1].clone()
+        self.kv_len = torch.zeros(T, dtype=torch.int32, device=device)
+        self.capacity = W * block
+        self.tokens = 0                      # of each stream
+
+    def room(self):
+        """One more token; raises if the streams are at capacity."""
+        if self.tokens >= self.capacity:
+            raise _lib.DuplexError(f"KV cache full: {self.tokens} tokens of {self.capacity} a stream "
+                                   "(evict() or attach a larger cache)")
+        self.tokens += 1
+
+
 class ClockStack:
     """Thinker layers [0, n) of the clock path on the B200 kernels (batch T <= 8)."""
 
@@ -171,6 +206,7 @@ class ClockStack:
         for L in layers:
             L.moe.workspace(T, self.device)
         self.graph = None
+        self.caches = None
 
     # ------------------------------------------------------------------ construction
     @classmethod
@@ -226,7 +262,52 @@ class ClockStack:
         return n
 
     def kernels_per_step(self) -> int:
+        if self.caches is not None:          # append, attend and its combine; the weights' pass
+            return (8 + self.caches.evictable) * len(self.layers)
         return 1 if self.fused else 5 * len(self.layers)
+
+    def attach_cache(self, tokens, block=64, fmt="e4m3", window=0, sinks=0, evictable=False,
+                     head_dim=synth.HEAD_DIM) -> StreamCaches:
+        """Give the stack its attention core: empty 8-bit caches for T streams of at most `tokens`
+        tokens (rounded up to blocks).  window, sinks: kv_attend's.  evictable: accumulate the
+        attention weights and hold a second set of blocks, for evict().  fused=False only."""
+        if self.fused:
+            raise _lib.DuplexError("the one-launch stack has no attention core: build it with fused=False")
+        kv_dim = self.qkv_dim - self.q_dim       # k and v
+        if self.q_dim % head_dim or kv_dim % (2 * head_dim) or kv_dim <= 0 or (
+                self.q_dim // head_dim) % (kv_dim // (2 * head_dim)):
+            raise _lib.DuplexError(f"q|k|v of {self.qkv_dim} rows, q of {self.q_dim}, is not heads of {head_dim}")
+        if tokens < 1 or window < 0 or sinks < 0:
+            raise _lib.DuplexError(f"bad cache: {tokens} tokens, window {window}, sinks {sinks}")
+        self.caches = StreamCaches(len(self.layers), self.T, tokens, self.q_dim // head_dim,
+                                   kv_dim // (2 * head_dim), head_dim, block, fmt, window, sinks,
+                                   evictable, self.device)
+        self.attn_buf = torch.zeros(self.T, self.q_dim, device=self.device, dtype=self.dtype)
+        self.graph = None
+        return self.caches
+
+    def evict(self, keep, sinks=0, recent=0) -> None:
+        """Keep at most `keep` tokens of each stream, layer and KV head (kv_evict).  A captured step
+        goes on with the kept ones."""
+        c = self.caches
+        if c is None or not c.evictable:
+            raise _lib.DuplexError("evict() needs attach_cache(..., evictable=True)")
+        for cache in c.layers:
+            new = cache.evict(c.table, c.kv_len, c.spare, keep, sinks, recent)
+        c.kv_len.copy_(new)
+        old = c.table.clone()
+        c.table.copy_(c.spare)
+        c.spare.copy_(old)
+        c.tokens = min(c.tokens, keep)
+
+    def _attention(self, i, accumulate=True):
+        """Layer i's attention of the step's q|k|v rows, into attn_buf."""
+        c = self.caches
+        rows = self.qkv_buf.view(self.T, self.qkv_dim // c.head_dim, c.head_dim)
+        k, v = rows[:, c.heads: c.heads + c.kv_heads], rows[:, c.heads + c.kv_heads:]
+        c.layers[i].append(k, v, c.table, c.kv_len)
+        c.layers[i].attend(rows[:, : c.heads], c.table, c.kv_len, window=c.window, sinks=c.sinks,
+                           out=self.attn_buf.view(self.T, c.heads, c.head_dim), accumulate=accumulate)
 
     def persistent(self) -> Persistent:
         if self._persist is None:
@@ -239,23 +320,41 @@ class ClockStack:
         return self._persist
 
     def step_into(self, x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
-        """Enqueue one decode step for x [T, H] on the current stream; result in out."""
+        """Enqueue one decode step for x [T, H] on the current stream; result in out.  With caches,
+        the T streams grow by a token each."""
         if self.fused:
             return self.persistent().run(x, out)
+        if self.caches is not None and not torch.cuda.is_current_stream_capturing():
+            self.caches.room()
+        return self._chain(x, out)
+
+    def _chain(self, x, out, accumulate=True):
+        if self.caches is not None:
+            self.caches.kv_len.add_(1)
         h_in = x
         n = len(self.layers)
         for i, L in enumerate(self.layers):
             h_out = out if i == n - 1 else (self.hA if i % 2 == 0 else self.hB)
             L.qkv.forward(h_in, out=self.qkv_buf, rms_eps=self.rms_eps)
-            L.o.forward(self.qkv_buf[:, : self.q_dim], residual=h_in, out=self.h1,
-                        x_row_stride=self.qkv_dim)
+            if self.caches is not None:
+                self._attention(i, accumulate)
+                L.o.forward(self.attn_buf, residual=h_in, out=self.h1)
+            else:
+                L.o.forward(self.qkv_buf[:, : self.q_dim], residual=h_in, out=self.h1,
+                            x_row_stride=self.qkv_dim)
             L.moe.forward_into(self.h1, h_out, residual=self.h1, rms_eps=self.rms_eps)
             h_in = h_out
         return out
 
     def capture(self):
         """Record one step (x_in -> out) in a CUDA graph."""
-        self.step_into(self.x_in, self.out)          # warm: workspaces, attributes
+        if self.caches is None:
+            self.step_into(self.x_in, self.out)      # warm: workspaces, attributes
+        else:                                        # ... and the streams are as long as before
+            if self.caches.tokens >= self.caches.capacity:
+                raise _lib.DuplexError("KV cache full: nothing to capture a step on")
+            self._chain(self.x_in, self.out, accumulate=False)
+            self.caches.kv_len.sub_(1)
         torch.cuda.synchronize(self.device)
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
@@ -269,6 +368,8 @@ class ClockStack:
         return g
 
     def replay(self):
+        if self.caches is not None:
+            self.caches.room()
         self.graph.replay()
 
     def decode(self, x_host: torch.Tensor, out_host: torch.Tensor) -> torch.Tensor:
@@ -277,12 +378,14 @@ class ClockStack:
         if self.graph is None:
             self.capture()
         self.x_in.copy_(x_host, non_blocking=True)
-        self.graph.replay()
+        self.replay()
         out_host.copy_(self.out, non_blocking=True)
         return out_host
 
     def device_errors(self) -> int:
         n = sum(L.moe.device_errors() for L in self.layers)
+        if self.caches is not None:
+            n += sum(c.device_errors() for c in self.caches.layers)
         if self._persist is not None:
             n += self._persist.device_errors()
         return n
