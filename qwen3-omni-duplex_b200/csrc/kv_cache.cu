@@ -41,7 +41,7 @@ struct AppendParams {
 // Work item w of a sequence's touched blocks: sequence b owns items [cu[b]/P + 2b, cu[b+1]/P + 2(b+1)),
 // which is never fewer than the blocks that its rows touch.
 template <int FMT, int ACT, int kRounds>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams p) {
+__global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 : 2) kv_append_kernel(AppendParams p) {
   __shared__ float red[kThreads / 32];
   const KvView& c = p.c;
   const int P = c.block, D = c.dim, h = blockIdx.y, tid = threadIdx.x;
@@ -172,7 +172,7 @@ template <bool SM_KEYS>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
   constexpr int W = kSelThreads / 32;
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[W][256];
+  __shared__ int hist[W][257];  // weights share their upper digits: one digit's counts of all warps in as many banks
   __shared__ int total[256];
   __shared__ int s_held[W], s_equal[W];
   __shared__ int s_digit, s_above;
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
   const bool none = want == 0;
   uint32_t prefix = 0, mask = 0;
   for (int shift = 24; shift >= 0 && !none; shift -= 8) {
-    for (int i = tid; i < 256 * W; i += kSelThreads) (&hist[0][0])[i] = 0;
+    for (int i = tid; i < 257 * W; i += kSelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
     for (int j = lo + tid; j < hi; j += kSelThreads) {
       const uint32_t u = key_of(j);
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
 // One CTA per (destination block, sequence and head): its tokens' codes, keys and values, are read
 // where they are, and rounded at the new block's scale.
 template <int FMT, int R>
-__global__ void __launch_bounds__(kThreads) kv_gather_kernel(EvictParams p) {
+__global__ void __launch_bounds__(kThreads, R == 1 ? 5 : R == 2 ? 3 : 1) kv_gather_kernel(EvictParams p) {
   __shared__ float red[2][kThreads / 32];
   const KvView& c = p.c;
   const int P = c.block, D = c.dim, tid = threadIdx.x;

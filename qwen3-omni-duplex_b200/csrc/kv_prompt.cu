@@ -406,12 +406,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
             uint32_t w[32];
             tmem_ld32(ts + 32 * q, w);
             tc_wait_ld();
-            const int a = k_max - 32 * q, d = k_min - 32 * q, e1 = k_sink - 32 * q;
+            auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1; };  // bits of columns < k
+            const uint32_t see = below(k_max + 1 - 32 * q) & (~below(k_min + 1 - 32 * q) | below(k_sink - 32 * q));
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const bool see = e <= a && (e > d || e < e1);
-              w[e] = see ? w[e] : __float_as_uint(-INFINITY);
-            }
+            for (int e = 0; e < 32; ++e) w[e] = (see >> e) & 1u ? w[e] : __float_as_uint(-INFINITY);
             if (ref.bad) {
 #pragma unroll 1
               for (int o = 0; o < 32; o += 16) {  // 16 tokens are in one block
