@@ -708,7 +708,7 @@ static int run_attend(const AttendParams& p, cudaStream_t st) {
 
 template <int D, int FMT>
 static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
-  const int rc = kv_prompt_takes(p.c, p.group) ? kv_prompt_run(p, workspace, st)
+  const int rc = kv_prompt_takes(p) ? kv_prompt_run(p, workspace, st)
                  : nt_of(p.c, p.group) == 1    ? run_attend<D, FMT, 1>(p, st)
                                                : run_attend<D, FMT, 2>(p, st);
   if (rc || !p.c.weights) return rc;
@@ -720,9 +720,10 @@ static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
   return record_cuda(cudaGetLastError());
 }
 
-// the rows' sums of exponentials lie behind the rest of the workspace
+// either kernel's (the choice depends on the window too); the rows' sums of exponentials lie behind it
 static size_t front_bytes(const KvView& c, int group) {
-  return kv_prompt_takes(c, group) ? kv_prompt_workspace(c, group) : part_bytes(c, nt_of(c, group));
+  const size_t few = part_bytes(c, nt_of(c, group));
+  return nt_of(c, group) == 1 ? few : std::max(few, kv_prompt_workspace(c, group));
 }
 
 int device_sms(int* sms) {

@@ -75,7 +75,7 @@ int kv_check(const duplex_kv_cache* c, const duplex_kv_batch* b, KvView* out);
 int device_sms(int* sms);
 
 // kv_prompt.cu
-bool kv_prompt_takes(const KvView& c, int group);
+bool kv_prompt_takes(const AttendParams& p);
 size_t kv_prompt_workspace(const KvView& c, int group);
 int kv_prompt_run(const AttendParams& p, void* workspace, cudaStream_t st);
 

@@ -20,6 +20,7 @@
 // joins the items that a cut went through.  The roles meet only at the barriers of the buffers they
 // share, so the next item's keys are under way while the last one's rows are written.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "kv_attend.cuh"
@@ -54,6 +55,9 @@ struct PromptParams {
   int* n_pairs;
   int64_t* total;
 };
+
+// A piece's units: an equal share, but no fewer than make the pieces worth joining.
+DEVI int64_t share_of(int64_t total, int ctas) { return max((total + ctas - 1) / ctas, (int64_t)(2 * kPOver)); }
 
 DEVI int units_in(const Span& sp) {
   return sp.sink_units + (sp.end > sp.lo ? (sp.end - sp.lo + kPTok - 1) / kPTok : 0);
@@ -238,7 +242,7 @@ DEVI void find_piece(const PromptParams& pp, int64_t u, int64_t u_end, int& pi, 
 }
 
 // Registers: 640 threads start with 96 each, 61,440; the softmax warps take what the others leave.
-constexpr int kRegSoftmax = 144, kRegConvert = 64, kRegMma = 64;
+constexpr int kRegSoftmax = 152, kRegConvert = 56, kRegMma = 64;
 static_assert(256 * kRegSoftmax + 256 * kRegConvert + 128 * kRegMma <= kPThreads * 96, "register split");
 
 template <int D, int FMT>
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
   };
 
   const int pairs = *pp.n_pairs;
-  const int64_t total = *pp.total, share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1);
+  const int64_t total = *pp.total, share = share_of(total, gridDim.x);
   const int64_t u_begin = (int64_t)blockIdx.x * share, u_end = min(u_begin + share, total);
   int64_t u = u_begin;
   int pi = u < u_end ? pair_of(pp.list, pairs, u) : 0;
@@ -747,7 +751,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
   static_assert(kJoinThreads == kPRows, "a thread is a row");
   const AttendParams& p = pp.a;
   pdl_wait();
-  const int64_t total = *pp.total, share = max((total + ctas - 1) / ctas, (int64_t)1);
+  const int64_t total = *pp.total, share = share_of(total, ctas);
   const int64_t u = (int64_t)(blockIdx.x + 1) * share;
   if (u >= total) return;
   const int pi = pair_of(pp.list, *pp.n_pairs, u);
@@ -796,7 +800,23 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
   if (blockIdx.y == 0) p.lse[at] = lse_of(M, l);
 }
 
-bool kv_prompt_takes(const KvView& c, int group) { return (int64_t)c.n_rows * group >= 128ll * c.batch; }
+// Which kernel is faster, by the time each takes as measured on one B200 (128 dims, 32 query heads on 4;
+// its own / kv_attend_kernel's us):
+//   7 sequences of 3000 tokens, 4 rows each 42 / 31, 8 rows 43 / 40, 16 rows 39 / 58, 32 rows 47 / 97
+//   64 of 4096: 4 rows 187 / 139, 8 rows 188 / 254      1 of 8192: 4 rows 46 / 23, 32 rows 50 / 48
+// A 128-token step of 16 rows, two CTAs an SM, takes there as long as one of 256 rows takes here, 2.3 us;
+// the rest is what a call costs before and after.  Lengths are the block table's, which the host knows.
+bool kv_prompt_takes(const AttendParams& p) {
+  const KvView& c = p.c;
+  const double rows = (double)c.n_rows * p.group / c.batch;
+  if (rows <= 16) return false;
+  double tokens = (double)c.width * c.block;
+  if (p.window) tokens = std::min(tokens, (double)p.sinks + p.window + rows / p.group);
+  const double steps = tokens / kPTok + 1, lists = (double)c.batch * c.heads;
+  const double few = 18 + 2.3 * lists * std::ceil(rows / 16) * steps / 296;
+  const double many = 28 + 2.3 * std::max(2.0 * kPOver, lists * std::ceil(rows / kPRows) * (steps + kPOver) / 148);
+  return many < few;
+}
 
 static int64_t max_pairs(const KvView& c, int group) { return (int64_t)c.n_rows * group / kPRows + c.batch; }
 
