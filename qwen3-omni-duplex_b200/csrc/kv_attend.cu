@@ -106,15 +106,22 @@ DEVI uint32_t movmatrix_trans(uint32_t a) {
 // brings the row's largest into [2^14, 2^15): bf16's 8 bits fit fp16's 11, and only values below
 // 2^-28 of the row's largest lose bits.  Returns the factor that undoes it.
 template <int D>
-DEVI float load_q(const AttendParams& p, int64_t row, int head, int t, bool live, uint2 (&qf)[D / 16]) {
-  uint4 raw[D / 64][2];
+DEVI void load_raw(const AttendParams& p, int64_t row, int head, int t, bool live, uint4 (&raw)[D / 64][2]) {
   const uint8_t* src = static_cast<const uint8_t*>(p.q) + 2 * (row * p.q_row + head * p.q_head);
+#pragma unroll
+  for (int cc = 0; cc < D / 64; ++cc)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      raw[cc][j] = live ? __ldg(reinterpret_cast<const uint4*>(src + 2 * (64 * cc + 16 * t + 8 * j))) : make_uint4(0, 0, 0, 0);
+}
+
+template <int D>
+DEVI float make_q(const AttendParams& p, const uint4 (&raw)[D / 64][2], uint2 (&qf)[D / 16]) {
   float amax = 0.f;
 #pragma unroll
   for (int cc = 0; cc < D / 64; ++cc)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      raw[cc][j] = live ? __ldg(reinterpret_cast<const uint4*>(src + 2 * (64 * cc + 16 * t + 8 * j))) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t w = (&raw[cc][j].x)[i];
@@ -137,6 +144,13 @@ DEVI float load_q(const AttendParams& p, int64_t row, int head, int t, bool live
       qf[cc * 4 + s] = make_uint2(f2h(a.x * f, a.y * f), f2h(b.x * f, b.y * f));
     }
   return pow2f(-up);
+}
+
+template <int D>
+DEVI float load_q(const AttendParams& p, int64_t row, int head, int t, bool live, uint2 (&qf)[D / 16]) {
+  uint4 raw[D / 64][2];
+  load_raw<D>(p, row, head, t, live, raw);
+  return make_q<D>(p, raw, qf);
 }
 
 // S[nt] += K (16 tokens) . Q (8 rows), both as fragments
@@ -571,32 +585,31 @@ __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p,
 }
 
 // Accumulated attention weights: weights[token] += sum over the sequence's rows and the group's
-// heads of exp(s - lse), after the attention itself.  A warp owns 16 tokens: their keys stay in its
+// heads of exp(s - lse), after the attention itself.  A warp owns 2 x 16 tokens: their keys stay in its
 // registers as fp16, the query rows come by, 32 at a time, through shared memory.
-constexpr int kRowChunk = 32;
+constexpr int kRowChunk = 32, kWU = 2;  // rows in shared memory at a time, twice; 64-token units a CTA
 
-// U units a CTA: where all rows are one chunk (decode) the chunk is staged once for several; otherwise
-// one unit, whose keys stay in registers while the chunks go by.
-template <int D, int FMT, int U>
+template <int D, int FMT>
 __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p) {
-  __shared__ uint2 sq[kRowChunk / 8][D / 16][32];
-  __shared__ float s_sc[kRowChunk], s_lse[kRowChunk];
-  __shared__ int s_pos[kRowChunk];
+  __shared__ uint2 sq[2][kRowChunk / 8][D / 16][32];
+  __shared__ float s_sc[2][kRowChunk], s_lse[2][kRowChunk];
+  __shared__ int s_pos[2][kRowChunk];
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
   const KvSeq s = kv_seq(c, b);
-  const int tile = blockIdx.x * (U * kWUnit), start = s.n - s.rows;
+  const int tile = blockIdx.x * (kWU * kWUnit), tile_end = tile + kWU * kWUnit, start = s.n - s.rows;
   if (tile >= s.n) return;
   // the sequence's rows that see a token of the tile
-  int t0 = max(tile - start, 0), t1 = s.rows;
-  if (p.window && tile >= p.sinks) t1 = (int)min((int64_t)t1, (int64_t)tile + U * kWUnit - 1 + p.window - start);
+  const int t0 = max(tile - start, 0);
+  int t1 = s.rows;
+  if (p.window && tile >= p.sinks) t1 = (int)min((int64_t)t1, (int64_t)tile_end - 1 + p.window - start);
   if (t0 >= t1) return;
-  uint4 kr[U][2][D / 64];
-  float ks[U], sum[U][2];
-  int64_t at[U];  // the warp's 16 tokens' slot, or -1
+  uint32_t kf[kWU][D / 16][4];  // the keys as fragments, fp16
+  float ks[kWU], sum[kWU][2];
+  int64_t at[kWU];  // the warp's 16 tokens' slot, or -1
 #pragma unroll
-  for (int x = 0; x < U; ++x) {
+  for (int x = 0; x < kWU; ++x) {
     const int tok = tile + x * kWUnit + 16 * warp;
     const bool hidden = tok >= s.n || (p.window && tok + 15 <= start - p.window && tok >= p.sinks);
     const int id = hidden ? -1 : kv_block_at(c, b, tok / c.block, p.err);
@@ -606,54 +619,91 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
     if (id >= 0) {
       const uint8_t* kp = c.k + at[x] * D + 16 * t;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int cc = 0; cc < D / 64; ++cc) {
+        const uint4 lo = __ldg(reinterpret_cast<const uint4*>(kp + g * D + 64 * cc));
+        const uint4 hi = __ldg(reinterpret_cast<const uint4*>(kp + (g + 8) * D + 64 * cc));
 #pragma unroll
-        for (int cc = 0; cc < D / 64; ++cc) kr[x][i][cc] = __ldg(reinterpret_cast<const uint4*>(kp + (g + 8 * i) * D + 64 * cc));
+        for (int e = 0; e < 4; ++e) {
+          kf[x][cc * 4 + e][0] = KvFmt<FMT>::lo((&lo.x)[e]);
+          kf[x][cc * 4 + e][1] = KvFmt<FMT>::lo((&hi.x)[e]);
+          kf[x][cc * 4 + e][2] = KvFmt<FMT>::hi((&lo.x)[e]);
+          kf[x][cc * 4 + e][3] = KvFmt<FMT>::hi((&hi.x)[e]);
+        }
+      }
       ks[x] = __ldg(c.k_scale + bh);
+    } else {
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) kf[x][e][0] = kf[x][e][1] = kf[x][e][2] = kf[x][e][3] = 0;
     }
   }
-  const int r1 = t1 * p.group;
-  for (int r0 = t0 * p.group; r0 < r1; r0 += kRowChunk) {
-    __syncthreads();
-    {  // thread 4 r + t stages row r's dims 64 cc + 16 t .. + 16
-      const int r = tid >> 2, rr = r0 + r;
-      const bool live = rr < r1;
-      uint2 qf[D / 16];
-      const int row = s.row0 + (live ? rr / p.group : 0), head = h * p.group + (live ? rr % p.group : 0);
-      const float undo = load_q<D>(p, row, head, t, live, qf);
+  // thread 4 r + t stages row r's dims 64 cc + 16 t .. + 16 of a chunk, loaded under the chunk before it
+  const int r1 = t1 * p.group, r = tid >> 2;
+  uint4 raw[D / 64][2];
+  float lse2;
+  int pos_r;
+  auto load = [&](int r0) {
+    const int rr = r0 + r, tr = p.by_group(rr);
+    const bool live = rr < r1;
+    const int64_t row = s.row0 + (live ? tr : 0);
+    const int head = h * p.group + (live ? rr - tr * p.group : 0);
+    load_raw<D>(p, row, head, t, live, raw);
+    lse2 = live ? p.lse[row * p.heads + head] * kLog2e : INFINITY;  // exp2 of it: 0
+    pos_r = live ? start + tr : -1;
+  };
+  auto stage = [&](int buf) {
+    uint2 qf[D / 16];
+    const float undo = make_q<D>(p, raw, qf);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) sq[r >> 3][i][(r & 7) * 4 + t] = qf[i];
-      if (t == 0) {
-        s_sc[r] = undo * p.scale_log2;
-        s_lse[r] = live ? p.lse[(int64_t)row * p.heads + head] * kLog2e : 0.f;
-        s_pos[r] = live ? start + rr / p.group : -1;
-      }
+    for (int e = 0; e < D / 16; ++e) sq[buf][r >> 3][e][(r & 7) * 4 + t] = qf[e];
+    if (t == 0) {
+      s_sc[buf][r] = undo * p.scale_log2;
+      s_lse[buf][r] = lse2;
+      s_pos[buf][r] = pos_r;
     }
     __syncthreads();
-#pragma unroll
+  };
+  int buf = 0;
+  load(t0 * p.group);
+  stage(0);
+  for (int r0 = t0 * p.group; r0 < r1; r0 += kRowChunk, buf ^= 1) {
+    const bool more = r0 + kRowChunk < r1;
+    if (more) load(r0 + kRowChunk);
+    // all rows of the chunk see all tokens of the tile
+    const int first = start + p.by_group(r0), last = start + p.by_group(min(r0 + kRowChunk, r1) - 1);
+    const bool plain = tile_end - 1 <= first && (!p.window || tile > last - p.window || tile_end <= p.sinks);
+#pragma unroll 2
     for (int nt = 0; nt < kRowChunk / 8; ++nt) {
       if (r0 + nt * 8 >= r1) break;
-      uint2 qf[1][D / 16];
+      const float sc[2] = {s_sc[buf][nt * 8 + 2 * t], s_sc[buf][nt * 8 + 2 * t + 1]}, ls[2] = {s_lse[buf][nt * 8 + 2 * t], s_lse[buf][nt * 8 + 2 * t + 1]};
+      float S[kWU][4];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) qf[0][i] = sq[nt][i][lane];
-      const float sc[2] = {s_sc[nt * 8 + 2 * t], s_sc[nt * 8 + 2 * t + 1]}, ls[2] = {s_lse[nt * 8 + 2 * t], s_lse[nt * 8 + 2 * t + 1]};
-      const int pos[2] = {s_pos[nt * 8 + 2 * t], s_pos[nt * 8 + 2 * t + 1]};
+      for (int x = 0; x < kWU; ++x) S[x][0] = S[x][1] = S[x][2] = S[x][3] = 0.f;
 #pragma unroll
-      for (int x = 0; x < U; ++x) {
-        if (at[x] < 0) continue;
-        float S[1][4] = {{0.f, 0.f, 0.f, 0.f}};
-        qk<D, FMT, 1>(kr[x], qf, S);
+      for (int e = 0; e < D / 16; ++e) {
+        const uint2 q = sq[buf][nt][e][lane];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int k = tile + x * kWUnit + 16 * warp + g + 8 * (j >> 1), q = pos[j & 1];
-          if (k <= q && (!p.window || k > q - p.window || k < p.sinks))
-            sum[x][j >> 1] += ex2(S[0][j] * (sc[j & 1] * ks[x]) - ls[j & 1]);
+        for (int x = 0; x < kWU; ++x) MmaOp<__half>::run(S[x], kf[x][e][0], kf[x][e][1], kf[x][e][2], kf[x][e][3], q.x, q.y);
+      }
+#pragma unroll
+      for (int x = 0; x < kWU; ++x) {
+        const float f[2] = {sc[0] * ks[x], sc[1] * ks[x]};
+        if (plain) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[x][j >> 1] += ex2(fmaf(S[x][j], f[j & 1], -ls[j & 1]));
+        } else {
+          const int pos[2] = {s_pos[buf][nt * 8 + 2 * t], s_pos[buf][nt * 8 + 2 * t + 1]};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = tile + x * kWUnit + 16 * warp + g + 8 * (j >> 1), q = pos[j & 1];
+            if (k <= q && (!p.window || k > q - p.window || k < p.sinks)) sum[x][j >> 1] += ex2(fmaf(S[x][j], f[j & 1], -ls[j & 1]));
+          }
         }
       }
     }
+    if (more) stage(buf ^ 1);  // (the chunk before last was read by all before the last barrier)
   }
 #pragma unroll
-  for (int x = 0; x < U; ++x)
+  for (int x = 0; x < kWU; ++x)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float y = sum[x][i];
@@ -712,11 +762,9 @@ static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
                  : nt_of(p.c, p.group) == 1    ? run_attend<D, FMT, 1>(p, st)
                                                : run_attend<D, FMT, 2>(p, st);
   if (rc || !p.c.weights) return rc;
-  const bool few = (int64_t)p.c.n_rows * p.group <= (int64_t)p.c.batch * kRowChunk;
-  const int tokens = few ? 2 * kWUnit : kWUnit;
+  const int tokens = kWU * kWUnit;
   const dim3 grid((unsigned)(((int64_t)p.c.width * p.c.block + tokens - 1) / tokens), p.c.heads, p.c.batch);
-  if (few) kv_weights_kernel<D, FMT, 2><<<grid, kWarps * 32, 0, st>>>(p);
-  else kv_weights_kernel<D, FMT, 1><<<grid, kWarps * 32, 0, st>>>(p);
+  kv_weights_kernel<D, FMT><<<grid, kWarps * 32, 0, st>>>(p);
   return record_cuda(cudaGetLastError());
 }
 

@@ -166,7 +166,7 @@ constexpr int kSelThreads = 1024;
 // warp counts and writes its own stretch of the tokens in order: all above that key, and the first of
 // those equal.  Keys stay in shared memory (SM_KEYS: up to kMaxKeys tokens), so weights and block ids
 // are read once; longer sequences read them anew in each pass.
-constexpr int kMaxKeys = 40 * 1024;
+constexpr int kMaxKeys = 40 * 1024;  // and their block ids: 170 KB beside 34 KB
 
 template <bool SM_KEYS>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
@@ -181,9 +181,15 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
   const int n = kv_seq(c, b).n;
   if (h == 0 && tid == 0) p.new_len[b] = min(n, p.keep);
   int32_t* out = p.index + ((int64_t)b * c.heads + h) * p.keep;
+  int32_t* ids = reinterpret_cast<int32_t*>(keys + (int64_t)c.width * c.block);  // the sequence's block ids (SM_KEYS)
+  const int shift_p = __ffs(c.block) - 1;
+  if (SM_KEYS) {
+    for (int i = tid; i < (n + c.block - 1) / c.block; i += kSelThreads) ids[i] = kv_block_at(c, b, i, p.err);
+    __syncthreads();
+  }
   auto slot_of = [&](int j) -> int {  // a token's place among all blocks' tokens, or -1
-    const int id = kv_block_at(c, b, j / c.block, p.err);
-    return id < 0 ? -1 : id * c.block + (j & (c.block - 1));
+    const int id = SM_KEYS ? ids[j >> shift_p] : kv_block_at(c, b, j >> shift_p, p.err);
+    return id < 0 ? -1 : (id << shift_p) + (j & (c.block - 1));
   };
   if (n <= p.keep) {
     for (int j = tid; j < n; j += kSelThreads) out[j] = slot_of(j);
@@ -191,11 +197,11 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
   }
   auto read_key = [&](int j) -> uint32_t {
     const int s = slot_of(j);
-    return s < 0 ? 0u : order_key(c.weights[((int64_t)(s / c.block) * c.heads + h) * c.block + (s & (c.block - 1))]);
+    return s < 0 ? 0u : order_key(c.weights[(((int64_t)(s >> shift_p) * c.heads + h) << shift_p) + (s & (c.block - 1))]);
   };
   const int lo = p.sinks, hi = n - p.recent;  // keep >= sinks + recent and n > keep, so lo < hi
   if (SM_KEYS) {
-#pragma unroll 4
+#pragma unroll 8
     for (int j = lo + tid; j < hi; j += kSelThreads) keys[j] = read_key(j);
   }
   auto key_of = [&](int j) -> uint32_t { return SM_KEYS ? keys[j] : read_key(j); };
@@ -462,8 +468,9 @@ extern "C" int duplex_kv_evict(const duplex_kv_cache* cache, const duplex_kv_bat
   const dim3 heads(cache->kv_heads, batch->batch);
   const int64_t cap = (int64_t)batch->width * cache->block;
   if (cap <= kMaxKeys) {
-    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_select_kernel<true>), kMaxKeys * 4)) return rc;
-    kv_select_kernel<true><<<heads, kSelThreads, (size_t)cap * 4, st>>>(p);
+    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_select_kernel<true>), kMaxKeys * 4 + kMaxKeys / 16 * 4))
+      return rc;
+    kv_select_kernel<true><<<heads, kSelThreads, (size_t)(cap + batch->width) * 4, st>>>(p);
   } else {
     kv_select_kernel<false><<<heads, kSelThreads, 0, st>>>(p);
   }

@@ -391,12 +391,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       const int row_lo = row_base + mt * 128, row_hi = min(row_lo + 128, row_all);
       const int t_first = s.n - s.rows + p.by_group(min(row_lo, row_all - 1));  // positions of the tile's rows
       const int t_last = s.n - s.rows + p.by_group(row_hi - 1);
-      const bool ragged = row_lo + 128 > row_all, mine = mt == 0 || x.two;
+      const bool mine = mt == 0 || x.two;
       const float cs = fmaxf(s_undo[tid] * fabsf(p.scale_log2) * ref.k, 1.2e-38f);  // not 0: hidden scores are -inf
       float m = -INFINITY, l = 0.f;
       for (int j = 0; mine && j < n; ++j) {
         const int base = x.base_of(x.i0 + j);
-        const bool masked = ref.bad || ragged || base + kPTok - 1 > t_first ||
+        // (rows past the last have zeros for a query and are not written: they need no mask)
+        const bool masked = ref.bad || base + kPTok - 1 > t_first ||
                             (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
         if (!(ok = wait(s_full + mt, n_s + j))) break;
         tc_fence_after();
