@@ -732,7 +732,8 @@ static int run_attend(const AttendParams& p, cudaStream_t st) {
   const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = front_smem<D, NT>() + plan;
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attend_kernel<D, FMT, NT>), 100 * 1024)) return rc;
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attend_kernel<D, FMT, NT>),
+                                front_smem<D, NT>() + 8 * (DUPLEX_KV_MAX_BATCH + 1))) return rc;
   // no more CTAs than units there can be
   const int64_t tiles = ((int64_t)p.c.n_rows * p.group) / ROWS + p.c.batch;
   const int64_t units = tiles * p.c.heads * (((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit);
@@ -740,7 +741,8 @@ static int run_attend(const AttendParams& p, cudaStream_t st) {
   kv_attend_kernel<D, FMT, NT><<<ctas, kWarps * 32, smem, st>>>(p);
   if (int rc = record_cuda(cudaGetLastError())) return rc;
   if (ctas > 1) {
-    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_combine_kernel<D, NT>), 100 * 1024)) return rc;
+    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_combine_kernel<D, NT>),
+                                  8 * (DUPLEX_KV_MAX_BATCH + 1) + 4 * kMaxCtas * (512 / D))) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas - 1, ROWS * D / 512);
     cfg.blockDim = dim3(kWarps * 32);

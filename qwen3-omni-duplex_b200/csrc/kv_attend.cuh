@@ -48,7 +48,7 @@ struct Span {
 template <int U>
 DEVI Span span_of(const AttendParams& p, int first_pos, int last_pos, int n) {
   Span s;
-  s.end = min(last_pos + 1, n);
+  s.end = max(min(last_pos + 1, n), 0);  // rows before token 0 see nothing
   s.lo = 0;
   s.sink_units = 0;
   s.sink_end = 0;

@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
   if (s.rows == 0) return;
   const int first = s.n - s.rows;  // slot of the sequence's first new token (< 0: no room for it)
   const int64_t item = w - (s.row0 / P + 2ll * b);
+  if (item < 0) return;  // rows before the first sequence's
   const int64_t col = max(first, 0) / P + item;
   if (col * P >= s.n) return;
   const int id = kv_block_at(c, b, (int)col, tid == 0 ? p.err : nullptr);

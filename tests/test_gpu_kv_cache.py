@@ -109,6 +109,15 @@ CASES = [
     (3, [700, 129, 300], [700, 1500, 333], 16, 2, 128, 64, "e4m3", "bf16", 0, 0),     # prompts
     (2, [260, 515], [1300, 515], 12, 4, 64, 32, "int8", "fp16", 200, 20),
     (1, [1030], [2100], 4, 4, 128, 128, "int8", "bf16", 0, 0),
+    (2, [500, 3], [20, 3], 8, 1, 64, 16, "e4m3", "bf16", 30, 5),          # ... and a window
+    # prompts long enough for the tensor-core kernel whatever the window
+    (2, [1500, 900], [3000, 900], 12, 4, 64, 32, "int8", "fp16", 200, 20),
+    (1, [3000], [3100], 8, 1, 128, 16, "e4m3", "bf16", 1, 0),             # each row sees itself alone
+    (2, [1300, 1], [5000, 700], 8, 1, 128, 128, "e4m3", "bf16", 300, 150),
+    (2, [2000, 1700], [1500, 1700], 4, 1, 64, 64, "e4m3", "fp16", 0, 0),  # more rows than tokens
+    (4, [2500, 0, 5, 1], [2600, 700, 0, 1], 16, 2, 128, 16, "int8", "bf16", 0, 0),
+    (1, [1537], [1537], 6, 2, 128, 32, "e4m3", "fp16", 1000, 4),
+    (2, [2500, 1700], [700, 1700], 8, 1, 128, 64, "e4m3", "bf16", 900, 20),   # rows before token 0, a window, sinks
 ]
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
@@ -180,6 +189,42 @@ def test_attend_uniform_rows_and_strides(cuda):
     assert torch.equal(kv_cache.kv_attend(turned, *cache_args(s), softmax_scale=0.05), ref)
 
 
+@pytest.mark.parametrize("T", [1, 2])
+def test_largest_batch(cuda, T):
+    """4096 sequences in a call against the same in calls of 128; one more is refused."""
+    from duplex.streaming import kv_cache
+    B = 4096
+    lens = [T + (7 * i) % 40 for i in range(B)]
+    s = make(cuda, B, [T] * B, lens, 8, 1, 128, 16, "e4m3", torch.float16, seed=9, width=3)
+    out = kv_cache.kv_attend(s["q"], *cache_args(s))
+    for b in range(0, B, 128):
+        part = kv_cache.kv_attend(s["q"][b * T: (b + 128) * T], *cache_args(s)[:4], s["table"][b: b + 128],
+                                  s["kv_len"][b: b + 128])
+        assert torch.equal(part, out[b * T: (b + 128) * T])
+    kv_cache.kv_append(s["q"][:, :1], s["q"][:, 1:2], *cache_args(s))
+    with pytest.raises(RuntimeError):
+        kv_cache.kv_attend(s["q"], *cache_args(s)[:4], torch.cat([s["table"], s["table"][:1]]),
+                           torch.cat([s["kv_len"], s["kv_len"][:1]]), cu_q=torch.zeros(B + 2, dtype=torch.int32, device=cuda))
+
+
+def test_rows_before_and_between(cuda):
+    """Row offsets that do not begin at 0: the rows before belong to nobody."""
+    from duplex.streaming import kv_cache
+    s = make(cuda, 2, [40, 3], [60, 33], 4, 1, 64, 16, "int8", torch.float16, extra_rows=70)
+    cu = s["cu"] + 65
+    q, k = s["q"], s["q"][:, :1]
+    ref = [t.clone() for t in (s["k"], s["k_scale"])]
+    kv_cache.kv_append(k, k, *cache_args(s), cu_q=cu)
+    got = [t.clone() for t in (s["k"], s["k_scale"])]
+    s["k"].copy_(ref[0]), s["k_scale"].copy_(ref[1])
+    kv_cache.kv_append(k[65:], k[65:], *cache_args(s), cu_q=s["cu"])
+    assert torch.equal(got[0], s["k"]) and torch.equal(got[1], s["k_scale"])
+    out = torch.full_like(q, 7.0, memory_format=torch.contiguous_format)
+    kv_cache.kv_attend(q, *cache_args(s), cu_q=cu, out=out)
+    assert bool((out[:65] == 7).all()) and bool((out[108:] == 7).all())
+    assert torch.equal(out[65:108], kv_cache.kv_attend(q[65:], *cache_args(s), cu_q=s["cu"])[:43])
+
+
 def test_attend_nan_and_inf_rows_stay_alone(cuda):
     from duplex.streaming import kv_cache
     rows, lens = [1, 3], [200, 90]
@@ -226,6 +271,56 @@ def test_append(cuda, fmt, dt, P, D):
     assert torch.equal(weights.cpu(), want)
 
 
+def test_prompt_matches_single_rows(cuda):
+    """The tensor-core kernel and the few-rows kernel agree where the first meets what the second is
+    tested for: a NaN row, a block id out of range, garbage behind the sequence; rows taken one by one."""
+    from duplex import _lib
+    from duplex.streaming import kv_cache
+    T, n, Hq, H, D, P = 2048, 2300, 8, 2, 128, 64
+    s = make(cuda, 1, [T], [n], Hq, H, D, P, "e4m3", torch.bfloat16, seed=11)
+    s["q"][700, 3, 9] = float("nan")
+    s["table"][0, 20] = -7
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), return_lse=True, err=err)
+    assert int(err) == _lib.DEVERR_BLOCK
+    assert bool(torch.isnan(out[700, 3]).all()) and int(torch.isnan(out).any(-1).sum()) == 1
+    for t in (0, 1, 255, 699, 700, 701, 1027, 1028, 1100, T - 1):
+        one, l = kv_cache.kv_attend(s["q"][t: t + 1], *cache_args(s)[:5], s["kv_len"] - T + t + 1, return_lse=True)
+        ok = ~torch.isnan(one)
+        # both are within the bars of the float64 result: fp16 probabilities, and a rounding to bf16 each
+        bar = 2 * (2.0 ** -11 + 2.0 ** -12) * 448 * float(s["v_scale"].max()) + 2.0 ** -8 * one.float().abs()
+        assert bool(((out[t] - one[0]).float().abs() <= bar[0])[ok[0]].all())
+        assert torch.allclose(lse[t], l[0], rtol=2.0 ** -17, atol=2.0 ** -15, equal_nan=True)
+
+
+def test_prompt_captured(cuda):
+    """A captured prompt call follows lengths, rows and values; two replays side by side."""
+    from duplex.streaming import kv_cache
+    rows, lens = [1200, 900], [2000, 900]
+    s = make(cuda, 2, rows, lens, 8, 1, 128, 32, "int8", torch.float16, seed=12)
+    kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"])
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream() for _ in range(2)], []
+    for st in streams:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            o = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], return_lse=True)
+        graphs.append((g, o))
+    for r, n in (([1200, 900], [2000, 900]), ([2100, 0], [2000, 900]), ([300, 1800], [301, 896])):
+        s["kv_len"].copy_(torch.tensor(n, dtype=torch.int32))
+        s["cu"].copy_(torch.tensor([0, r[0], r[0] + r[1]], dtype=torch.int32))
+        s["q"].copy_(torch.randn_like(s["q"]))
+        torch.cuda.synchronize()
+        for st, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        ref = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], return_lse=True)
+        k = r[0] + r[1]
+        for _, o in graphs:
+            assert torch.equal(o[0][:k], ref[0][:k]) and torch.equal(o[1][:k], ref[1][:k])
+
+
 def test_append_not_finite(cuda):
     from duplex import _lib
     from duplex.streaming import kv_cache
@@ -264,6 +359,8 @@ EVICT = [
     ([257, 300], 256, 256, 0, 2, 64, 32, "int8"),        # nothing to choose
     ([130, 0, 1], 100, 30, 70, 1, 128, 32, "e4m3"),
     ([50], 1, 0, 0, 2, 64, 16, "e4m3"),
+    ([40_700, 39_000], 5000, 7, 900, 1, 64, 16, "int8"),    # as many keys as shared memory holds
+    ([70_000, 3], 9000, 0, 1, 1, 64, 128, "e4m3"),          # and more
 ]
 
 
@@ -294,8 +391,7 @@ def test_evict(cuda, case, kind):
     table, target = s["table"].cpu(), dst.cpu()
     for b, n in enumerate(lens):
         for h in range(H):
-            mine = [float(w0.cpu()[int(table[b, j // P]), h, j % P]) for j in range(n)] if n < 4000 else \
-                w0[s["table"][b].long(), h].reshape(-1)[:n].tolist()
+            mine = w0[s["table"][b, : -(-n // P)].long(), h].reshape(-1)[:n].tolist()
             at = kv_ref.kept_tokens(mine, n, keep, sinks, recent)
             for i, j in enumerate(at):
                 ww[int(target[b, i // P]), h, i % P] = mine[j]
