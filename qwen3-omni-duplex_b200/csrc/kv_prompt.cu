@@ -170,12 +170,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
   }
 }
 
-// the last pair whose first unit is <= u
+// the last pair whose first unit is <= u, 32 of them a look (by whole warps)
 DEVI int pair_of(const PromptItem* list, int pairs, int64_t u) {
-  int lo = 0, hi = pairs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (list[mid].off <= u) lo = mid; else hi = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, left = pairs;
+  while (left > 1) {
+    const int step = (left + 31) / 32, at = lo + lane * step;
+    const bool before = at < lo + left && list[at].off <= u;
+    const int i = 31 - __clz(__ballot_sync(~0u, before) | 1u);
+    left = min(step, left - i * step);
+    lo += i * step;
   }
   return lo;
 }
