@@ -13,7 +13,14 @@
 //                    buffers each
 //   warp 16          issues the products: S = Q K^T (both shared memory), O += P V
 //
-// The running maximum is a reference that may lag by 2^kSlack, so O is rescaled rarely.
+// The running maximum is a reference that may lag by 2^kSlack, so O is rescaled rarely.  The products of a
+// tile's first 64 tokens start while the softmax is at the second 64.
+//
+// One B200, 32 query heads on 4, dim 128: a prompt of 8192 tokens takes 617 us, 890 TFLOP/s, 53 % of a
+// plain bf16 product's rate; 4200 cycles a step of 256 rows and 128 tokens, of which products are 2048.  A
+// step is a chain: softmax of a tile (2500), its products (1500); the other tile's chain fills in, but two
+// tiles are what 512 columns hold.  Skipping the exponentials, or the search for the maximum, or the
+// conversion each gains 3 to 8 %.  An item costs 4 steps more: query rows in, results out, masks.
 //
 // Work is one list of (row tile, head) items, 128 tokens a unit, cut into equal contiguous pieces, one
 // per SM; kv_prompt_plan_kernel writes it (causal row tiles differ in length), kv_prompt_join_kernel
