@@ -300,14 +300,14 @@ class ClockStack:
         c.spare.copy_(old)
         c.tokens = min(c.tokens, keep)
 
-    def _attention(self, i, accumulate=True):
+    def _attention(self, i):
         """Layer i's attention of the step's q|k|v rows, into attn_buf."""
         c = self.caches
         rows = self.qkv_buf.view(self.T, self.qkv_dim // c.head_dim, c.head_dim)
         k, v = rows[:, c.heads: c.heads + c.kv_heads], rows[:, c.heads + c.kv_heads:]
         c.layers[i].append(k, v, c.table, c.kv_len)
         c.layers[i].attend(rows[:, : c.heads], c.table, c.kv_len, window=c.window, sinks=c.sinks,
-                           out=self.attn_buf.view(self.T, c.heads, c.head_dim), accumulate=accumulate)
+                           out=self.attn_buf.view(self.T, c.heads, c.head_dim))
 
     def persistent(self) -> Persistent:
         if self._persist is None:
@@ -328,7 +328,7 @@ class ClockStack:
             self.caches.room()
         return self._chain(x, out)
 
-    def _chain(self, x, out, accumulate=True):
+    def _chain(self, x, out):
         if self.caches is not None:
             self.caches.kv_len.add_(1)
         h_in = x
@@ -337,7 +337,7 @@ class ClockStack:
             h_out = out if i == n - 1 else (self.hA if i % 2 == 0 else self.hB)
             L.qkv.forward(h_in, out=self.qkv_buf, rms_eps=self.rms_eps)
             if self.caches is not None:
-                self._attention(i, accumulate)
+                self._attention(i)
                 L.o.forward(self.attn_buf, residual=h_in, out=self.h1)
             else:
                 L.o.forward(self.qkv_buf[:, : self.q_dim], residual=h_in, out=self.h1,
@@ -350,11 +350,13 @@ class ClockStack:
         """Record one step (x_in -> out) in a CUDA graph."""
         if self.caches is None:
             self.step_into(self.x_in, self.out)      # warm: workspaces, attributes
-        else:                                        # ... and the streams are as long as before
-            if self.caches.tokens >= self.caches.capacity:
-                raise _lib.DuplexError("KV cache full: nothing to capture a step on")
-            self._chain(self.x_in, self.out, accumulate=False)
-            self.caches.kv_len.sub_(1)
+        else:                                        # ... on caches of its own: a token that is taken
+            c = self.caches                          # back could have raised a block's scale
+            self.caches = StreamCaches(len(self.layers), self.T, 1, c.heads, c.kv_heads, c.head_dim,
+                                       c.layers[0].block, c.layers[0].fmt, c.window, c.sinks,
+                                       c.evictable, self.device)
+            self._chain(self.x_in, self.out)
+            self.caches = c
         torch.cuda.synchronize(self.device)
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))

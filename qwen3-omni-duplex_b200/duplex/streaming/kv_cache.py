@@ -72,9 +72,10 @@ def kv_attend(q, k, v, k_scale, v_scale, block_table, kv_len, *, cu_q=None, wind
 
     window = 0: a row sees its own token and all before.  window > 0: the last `window` of those, and
     the sequence's first `sinks` tokens.  Windows count cached tokens, so after `kv_evict` they count
-    kept ones.  Blocks that no row sees are not read, and their table entries may be anything.  A row
-    that sees nothing (kv_len smaller than its sequence's rows) gets 0 and -inf.  Rows behind the last
-    sequence's are left as they were.
+    kept ones.  Blocks that no row sees are not read, and their table entries may be anything; slots
+    that no row sees may hold any code.  (An e4m3 NaN in a token that one row of a call sees may reach
+    rows that do not: 0 * NaN.  kv_append stores none.)  A row that sees nothing (kv_len smaller than
+    its sequence's rows) gets 0 and -inf.  Rows behind the last sequence's are left as they were.
 
     weights [n_blocks, kv_heads, block] fp32: each seen token's entry grows by its attention weights,
     summed over the call's rows and the query heads of its KV head.  `out` must not overlap q."""

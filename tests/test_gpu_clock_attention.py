@@ -46,8 +46,8 @@ def test_steps_vs_oracle(cuda, T, fmt, window):
     log = []
     real = st._attention
 
-    def attention(i, accumulate):
-        real(i, accumulate)
+    def attention(i):
+        real(i)
         log.append([st.qkv_buf.clone(), st.attn_buf.clone()])
 
     st._attention = attention
@@ -115,13 +115,33 @@ def test_captured_session_equals_eager(cuda):
     assert a.device_errors() == 0 and b.device_errors() == 0
 
 
+def test_capture_leaves_the_session_alone(cuda):
+    """Capturing in the middle of a block changes nothing of what is cached, whatever x_in holds."""
+    _, st = build(cuda, 2, fmt="int8", evictable=True)
+    x = torch.randn(2, 256, device=cuda).half()
+    out = torch.zeros_like(x)
+    for _ in range(5):
+        st.step_into(0.01 * x, out)
+    state = lambda: [t.clone() for c in st.caches.layers for t in (c.k, c.v, c.k_scale, c.v_scale, c.weights)] + [  # noqa: E731
+        st.caches.kv_len.clone()]
+    before = state()
+    st.x_in.copy_(1000 * x)
+    st.capture()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, state())) and st.caches.tokens == 5
+    st.replay()
+    torch.cuda.synchronize()
+    assert st.caches.kv_len.tolist() == [6, 6]
+
+
 def test_refusals(cuda):
     from duplex.clock import ClockStack
     arrays, st = build(cuda, 1, tokens=16)
     x, out = torch.zeros(1, 256, device=cuda).half(), torch.zeros(1, 256, device=cuda).half()
     for _ in range(16):
         st.step_into(x, out)
-    for call in (lambda: st.step_into(x, out), st.capture, lambda: st.evict(keep=4)):
+    st.capture()
+    for call in (lambda: st.step_into(x, out), st.replay, lambda: st.evict(keep=4)):
         with pytest.raises(RuntimeError):
             call()
     with pytest.raises(RuntimeError, match="heads"):
