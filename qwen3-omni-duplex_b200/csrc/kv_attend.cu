@@ -15,12 +15,13 @@
 // hence 32 tokens for one set of addresses, one vote and one rescale.
 // One B200, 32 query heads on 4, dim 128, 64 sequences of 12,288 tokens (805 MB): 143 us, 5.6 TB/s, 86 %
 // of a plain copy's rate.  With 16 tokens a step 165 us; with the next 16 tokens in registers instead of
-// a ring 182 us.  One sequence of 2000: 13 us, all of it latency (list, copies, one step, join).
+// a ring 182 us.  One sequence of 2000: 10.5 us, all of it latency (list, copies, two steps, join).
 //
 // The work of a launch is one list of 128-token units over (sequence, KV head, row tile); every CTA
 // takes an equal, contiguous piece of it, whatever the lengths, and reads the lengths itself (a
 // captured launch follows them).  Pieces that share a row tile leave partial results, which
-// kv_combine_kernel joins in order: no atomics, the same bits on each run.
+// kv_combine_kernel joins in order: no atomics, the same bits on each run.  Few row tiles are given a
+// cluster of 8 CTAs each instead, joined in the same launch.
 #include <algorithm>
 
 #include "kv_attend.cuh"
@@ -50,7 +51,7 @@ DEVI int units_of(const KvSeq& s, const AttendParams& p, int rows) {
   return (int)min(u, (int64_t)all);
 }
 
-template <int ROWS>
+template <int ROWS, bool ITEMS = false>
 DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
   __shared__ int64_t warp_sum[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = p.c.batch;
@@ -60,7 +61,7 @@ DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
     int64_t u = 0;
     if (b < B) {
       const KvSeq s = kv_seq(p.c, b);
-      u = (int64_t)p.c.heads * tiles_of(s, p.group, ROWS) * units_of(s, p, ROWS);
+      u = (int64_t)p.c.heads * tiles_of(s, p.group, ROWS) * (ITEMS ? 1 : units_of(s, p, ROWS));
     }
     int64_t incl = u;
 #pragma unroll
@@ -199,7 +200,30 @@ template <int N> DEVI void cp_async_wait() { asm volatile("cp.async.wait_group %
 
 template <int D, int NT> constexpr int attend_ctas() { return NT == 1 ? 3 : 2; }  // an SM
 
-template <int D, int FMT, int NT>
+// Clusters: where there are few row tiles, kCluster CTAs take one each and join it through their shared
+// memories, which saves the second launch.
+constexpr int kCluster = 8;
+
+DEVI void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+DEVI uint32_t cluster_addr(const void* p, int rank) {  // p of the cluster's CTA `rank`
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(p)), "r"(rank));
+  return d;
+}
+DEVI float cluster_ld(uint32_t a) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(a) : "memory");
+  return x;
+}
+DEVI float4 cluster_ld4(uint32_t a) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(a) : "memory");
+  return x;
+}
+
+template <int D, int FMT, int NT, bool CL>
 __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_kernel(AttendParams p) {
   constexpr int ROWS = 8 * NT, VW = D / 32, LD = D + 4, ST = ring_slots<D, NT>(), kStage = stage_bytes<D>();
   extern __shared__ __align__(128) uint8_t dyn[];
@@ -211,26 +235,36 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
   uint8_t* const ring = dyn + warp * (ST * kStage);
   const int psh = __ffs(c.block) - 1;
   pdl_launch_dependents();
-  const Plan plan = make_plan<ROWS>(p, off, gridDim.x);
-  int64_t u = (int64_t)blockIdx.x * plan.share;
-  const int64_t u_end = min(u + plan.share, plan.total);
-  if (u >= u_end) return;
+  __shared__ float c_m[CL ? ROWS : 1], c_l[CL ? ROWS : 1];
+  const Plan plan = make_plan<ROWS, CL>(p, off, gridDim.x);
+  // the CTA's piece of the units; with clusters, the cluster's row tile and the CTA's place in it
+  const int rank = blockIdx.x % kCluster;
+  int64_t u = CL ? blockIdx.x / kCluster : (int64_t)blockIdx.x * plan.share;
+  const int64_t u_end = CL ? min(u + 1, plan.total) : min(u + plan.share, plan.total);
+  if (u >= u_end) return;  // a cluster's CTAs all alike
   int b = seq_of(off, c.batch, u);
   const int64_t u_begin = u;
 
   while (u < u_end) {
     while (off[b + 1] <= u) ++b;
     const KvSeq s = kv_seq(c, b);
-    const int rt_all = tiles_of(s, p.group, ROWS), per = units_of(s, p, ROWS);
+    const int rt_all = tiles_of(s, p.group, ROWS), per = CL ? 1 : units_of(s, p, ROWS);
     const int64_t r = u - off[b];
-    const int it = (int)(r / per), i0 = (int)(r - (int64_t)it * per);
-    const int i1 = (int)min((int64_t)per, i0 + (u_end - u));
+    const int it = (int)(r / per);
+    int i0 = (int)(r - (int64_t)it * per), i1 = (int)min((int64_t)per, i0 + (u_end - u));
+    const bool whole = !CL && i0 == 0 && i1 == per;
+    const int len = i1 - i0;
     const int h = it / rt_all, rt = it - h * rt_all;
     const int row_base = rt * ROWS, row_all = s.rows * p.group;
     const int first_pos = s.n - s.rows + row_base / p.group;
     const int last_row = min(row_base + ROWS, row_all) - 1;
     const int last_pos = s.n - s.rows + last_row / p.group;
     const Span sp = span_of<kUnit>(p, first_pos, last_pos, s.n);
+    if (CL) {
+      const int n = sp.sink_units + (sp.end > sp.lo ? (sp.end - sp.lo + kUnit - 1) / kUnit : 0);
+      i0 = n * rank / kCluster;
+      i1 = n * (rank + 1) / kCluster;
+    }
 
     // this warp's 32 tokens of unit i, as two parts of 16 (a block holds whole parts): the blocks' ids, or
     // -1 where no row of the tile looks
@@ -476,7 +510,6 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(O[nt][i][j] * f, O[nt][i][j + 2] * f);
       }
     __syncthreads();
-    const bool whole = i0 == 0 && i1 == per;
     float* part = p.part + (2 * (int64_t)blockIdx.x + (u == u_begin ? 0 : 1)) * part_floats<D, NT>();
     for (int e = tid; e < ROWS * D / 4; e += kWarps * 32) {
       const int rr = e / (D / 4), d = (e - rr * (D / 4)) * 4;
@@ -494,6 +527,14 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         o.w += x.w;
         L += sl[w][rr] * (sm[w][rr] == M ? 1.f : ex2(sm[w][rr] - M));
       }
+      if (CL) {  // over the first warp's sums, which this thread alone has read
+        *reinterpret_cast<float4*>(&sO[rr][d]) = o;
+        if (d == 0) {
+          c_m[rr] = M;
+          c_l[rr] = L;
+        }
+        continue;
+      }
       if (!whole) {
         *reinterpret_cast<float4*>(part + rr * D + d) = o;
         if (d == 0) {
@@ -510,8 +551,38 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
       if (d == 0) p.lse[at] = lse_of(M, L);
     }
+    if (CL) {
+      cluster_sync();
+      const int rr = rank + kCluster * (tid / (D / 4)), d = tid % (D / 4) * 4, r2 = row_base + rr;  // NT rows a CTA
+      if (rr < ROWS && r2 < row_all) {
+        float M = -INFINITY, L = 0.f, mj[kCluster];
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f), x[kCluster];
+#pragma unroll
+        for (int j = 0; j < kCluster; ++j) {
+          mj[j] = cluster_ld(cluster_addr(&c_m[rr], j));
+          x[j] = cluster_ld4(cluster_addr(&sO[rr][d], j));
+          M = fmaxf(M, mj[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kCluster; ++j) {
+          const float f = mj[j] == M ? 1.f : ex2(mj[j] - M);
+          L += f * cluster_ld(cluster_addr(&c_l[rr], j));
+          o.x += x[j].x * f;
+          o.y += x[j].y * f;
+          o.z += x[j].z * f;
+          o.w += x[j].w * f;
+        }
+        const int64_t at = (int64_t)(s.row0 + r2 / p.group) * p.heads + h * p.group + r2 % p.group;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
+            pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        if (d == 0) p.lse[at] = lse_of(M, L);
+      }
+      cluster_sync();  // no CTA leaves while its sums are read
+      return;
+    }
     __syncthreads();
-    u += i1 - i0;
+    u += len;
   }
 }
 
@@ -731,19 +802,47 @@ static size_t part_bytes(const KvView& c, int nt) {
                                               : (nt == 1 ? part_floats<64, 1>() : part_floats<64, 2>())) * 4;
 }
 
+// Clusters up to two thirds of what is resident at once (beyond, clusters of 8 wait for one another's
+// places) and up to here in tokens (8 CTAs a row tile are too few then).  With / without, 32 query heads on
+// 4, dim 128, us: 1 sequence of 2000 tokens 10.5 / 14.9, of 8192 16.8 / 22.9, of 16,384 26.9 / 25.0;
+// 8 sequences of 4096 14.5 / 22.8; 13 (416 CTAs) of 4096 24.8 / 22.2.
+constexpr double kClusterTokens = 12288;
+
 template <int D, int FMT, int NT>
 static int run_attend(const AttendParams& p, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
   const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = front_smem<D, NT>() + plan;
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attend_kernel<D, FMT, NT>),
-                                front_smem<D, NT>() + 8 * (DUPLEX_KV_MAX_BATCH + 1))) return rc;
   // no more CTAs than units there can be
-  const int64_t tiles = ((int64_t)p.c.n_rows * p.group) / ROWS + p.c.batch;
+  const int64_t rows = (int64_t)p.c.n_rows * p.group;
+  const int64_t tiles = p.group % ROWS == 0 ? rows / ROWS
+                        : p.c.cu            ? rows / ROWS + p.c.batch
+                                            : (rows / p.c.batch + ROWS - 1) / ROWS * p.c.batch;
   const int64_t units = tiles * p.c.heads * (((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit);
   const int ctas = (int)std::min(std::min((int64_t)sms * attend_ctas<D, NT>(), (int64_t)kMaxCtas), units);
-  kv_attend_kernel<D, FMT, NT><<<ctas, kWarps * 32, smem, st>>>(p);
+  constexpr int most = front_smem<D, NT>() + 8 * (DUPLEX_KV_MAX_BATCH + 1);
+  double seen = (double)p.c.width * p.c.block;
+  if (p.window) seen = std::min(seen, (double)p.sinks + p.window + ROWS);
+  if (tiles * p.c.heads * kCluster <= (int64_t)sms * attend_ctas<D, NT>() * 2 / 3 && seen <= kClusterTokens) {
+    const auto kern = kv_attend_kernel<D, FMT, NT, true>;
+    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), most)) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles * p.c.heads * kCluster));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return record_cuda(cudaLaunchKernelEx(&cfg, kern, p));
+  }
+  const auto kern = kv_attend_kernel<D, FMT, NT, false>;
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), most)) return rc;
+  kern<<<ctas, kWarps * 32, smem, st>>>(p);
   if (int rc = record_cuda(cudaGetLastError())) return rc;
   if (ctas > 1) {
     if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_combine_kernel<D, NT>),
