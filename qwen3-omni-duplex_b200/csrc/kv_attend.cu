@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       const float inv = L == 0.f ? 0.f : 1.f / L;
       *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
           pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-      if (d == 0) p.lse[at] = lse_of(M, L);
+      if (d == 0) put_stats(p, at, M, L);
     }
     if (CL) {
       cluster_sync();
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         const float inv = L == 0.f ? 0.f : 1.f / L;
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
             pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-        if (d == 0) p.lse[at] = lse_of(M, L);
+        if (d == 0) put_stats(p, at, M, L);
       }
       cluster_sync();  // no CTA leaves while its sums are read
       return;
@@ -655,20 +655,21 @@ __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p,
   const float inv = L == 0.f ? 0.f : 1.f / L;
   *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + 2 * (at * D + d)) =
       pack4(p.act, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-  if (d == 0) p.lse[at] = lse_of(M, L);
+  if (d == 0) put_stats(p, at, M, L);
 }
 
 // Accumulated attention weights: weights[token] += sum over the sequence's rows and the group's
-// heads of exp(s - lse), after the attention itself.  A warp owns 2 x 16 tokens: their keys stay in its
+// heads of exp(s - lse), after the attention itself, by the rows' maxima and sums.  A warp owns 2 x 16 tokens: their keys stay in its
 // registers as fp16, the query rows come by, 32 at a time, through shared memory.  Reading the keys again
 // (mostly from L2) costs less than the scores' way through memory for long prompts, and is as fast for
 // decode: 21 us for 16 sequences of 6000 tokens, latency of short CTAs; four tiles a CTA took 24 us.
 constexpr int kRowChunk = 32, kWU = 2;  // rows in shared memory at a time, twice; 64-token units a CTA
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p) {
+__global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams p) {
   __shared__ uint2 sq[2][kRowChunk / 8][D / 16][32];
-  __shared__ float s_sc[2][kRowChunk], s_lse[2][kRowChunk];
+  __shared__ float s_sc[2][kRowChunk];
+  __shared__ float2 s_st[2][kRowChunk];
   __shared__ int s_pos[2][kRowChunk];
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
   // thread 4 r + t stages row r's dims 64 cc + 16 t .. + 16 of a chunk, loaded under the chunk before it
   const int r1 = t1 * p.group, r = tid >> 2;
   uint4 raw[D / 64][2];
-  float lse2;
+  float2 st;
   int pos_r;
   auto load = [&](int r0) {
     const int rr = r0 + r, tr = p.by_group(rr);
@@ -723,7 +724,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
     const int64_t row = s.row0 + (live ? tr : 0);
     const int head = h * p.group + (live ? rr - tr * p.group : 0);
     load_raw<D>(p, row, head, t, live, raw);
-    lse2 = live ? p.lse[row * p.heads + head] * kLog2e : INFINITY;  // exp2 of it: 0
+    st = live ? p.stats[row * p.heads + head] : make_float2(0.f, 0.f);
+    st.x = kShift - st.x;
     pos_r = live ? start + tr : -1;
   };
   auto stage = [&](int buf) {
@@ -733,7 +735,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
     for (int e = 0; e < D / 16; ++e) sq[buf][r >> 3][e][(r & 7) * 4 + t] = qf[e];
     if (t == 0) {
       s_sc[buf][r] = undo * p.scale_log2;
-      s_lse[buf][r] = lse2;
+      s_st[buf][r] = st;
       s_pos[buf][r] = pos_r;
     }
     __syncthreads();
@@ -747,10 +749,14 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
     // all rows of the chunk see all tokens of the tile
     const int first = start + p.by_group(r0), last = start + p.by_group(min(r0 + kRowChunk, r1) - 1);
     const bool plain = tile_end - 1 <= first && (!p.window || tile > last - p.window || tile_end <= p.sinks);
+    float part[kWU][2];  // a chunk's sum by itself: thousands of rows added one by one would lose bits
+#pragma unroll
+    for (int x = 0; x < kWU; ++x) part[x][0] = part[x][1] = 0.f;
 #pragma unroll 2
     for (int nt = 0; nt < kRowChunk / 8; ++nt) {
       if (r0 + nt * 8 >= r1) break;
-      const float sc[2] = {s_sc[buf][nt * 8 + 2 * t], s_sc[buf][nt * 8 + 2 * t + 1]}, ls[2] = {s_lse[buf][nt * 8 + 2 * t], s_lse[buf][nt * 8 + 2 * t + 1]};
+      const float sc[2] = {s_sc[buf][nt * 8 + 2 * t], s_sc[buf][nt * 8 + 2 * t + 1]};
+      const float2 st2[2] = {s_st[buf][nt * 8 + 2 * t], s_st[buf][nt * 8 + 2 * t + 1]};
       float S[kWU][4];
 #pragma unroll
       for (int x = 0; x < kWU; ++x) S[x][0] = S[x][1] = S[x][2] = S[x][3] = 0.f;
@@ -765,16 +771,22 @@ __global__ void __launch_bounds__(kWarps * 32) kv_weights_kernel(AttendParams p)
         const float f[2] = {sc[0] * ks[x], sc[1] * ks[x]};
         if (plain) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sum[x][j >> 1] += ex2(fmaf(S[x][j], f[j & 1], -ls[j & 1]));
+          for (int j = 0; j < 4; ++j) part[x][j >> 1] = fmaf(ex2(fmaf(S[x][j], f[j & 1], st2[j & 1].x)), st2[j & 1].y, part[x][j >> 1]);
         } else {
           const int pos[2] = {s_pos[buf][nt * 8 + 2 * t], s_pos[buf][nt * 8 + 2 * t + 1]};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int k = tile + x * kWUnit + 16 * warp + g + 8 * (j >> 1), q = pos[j & 1];
-            if (k <= q && (!p.window || k > q - p.window || k < p.sinks)) sum[x][j >> 1] += ex2(fmaf(S[x][j], f[j & 1], -ls[j & 1]));
+            if (k <= q && (!p.window || k > q - p.window || k < p.sinks)) 
+              part[x][j >> 1] = fmaf(ex2(fmaf(S[x][j], f[j & 1], st2[j & 1].x)), st2[j & 1].y, part[x][j >> 1]);
           }
         }
       }
+    }
+#pragma unroll
+    for (int x = 0; x < kWU; ++x) {
+      sum[x][0] += part[x][0];
+      sum[x][1] += part[x][1];
     }
     if (more) stage(buf ^ 1);  // (the chunk before last was read by all before the last barrier)
   }
@@ -874,7 +886,7 @@ static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
   return record_cuda(cudaGetLastError());
 }
 
-// either kernel's (the choice depends on the window too); the rows' sums of exponentials lie behind it
+// either kernel's (the choice depends on the window too); the rows' statistics lie behind it
 static size_t front_bytes(const KvView& c, int group) {
   const size_t few = part_bytes(c, nt_of(c, group));
   return nt_of(c, group) == 1 ? few : std::max(few, kv_prompt_workspace(c, group));
@@ -895,7 +907,7 @@ extern "C" int duplex_kv_attend_workspace_bytes(const duplex_kv_cache* cache, co
   KvView v;
   if (int rc = kv_check(cache, batch, &v)) return rc;
   if (!bytes || heads < 1 || heads % cache->kv_heads) return DUPLEX_ERR_ARG;
-  *bytes = front_bytes(v, heads / cache->kv_heads) + (size_t)batch->n_rows * heads * 4;
+  *bytes = front_bytes(v, heads / cache->kv_heads) + (size_t)batch->n_rows * heads * (cache->weights ? 12 : 4);
   return DUPLEX_OK;
 }
 
@@ -929,7 +941,12 @@ extern "C" int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_ba
   p.scale_log2 = softmax_scale * kLog2e;
   p.out = out;
   p.part = static_cast<float*>(workspace);
-  p.lse = lse ? lse : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + front_bytes(p.c, p.group));
+  uint8_t* rows = static_cast<uint8_t*>(workspace) + front_bytes(p.c, p.group);
+  if (cache->weights) {
+    p.stats = reinterpret_cast<float2*>(rows);
+    rows += (size_t)batch->n_rows * heads * 8;
+  }
+  p.lse = lse ? lse : reinterpret_cast<float*>(rows);
   p.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cache->dim == 128)

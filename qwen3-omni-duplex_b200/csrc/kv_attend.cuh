@@ -20,7 +20,8 @@ struct AttendParams {
   int window, sinks;
   float scale_log2;       // softmax_scale * log2(e)
   void* out;              // [n_rows][heads][dim]
-  float* lse;             // [n_rows][heads] or null
+  float* lse;             // [n_rows][heads]
+  float2* stats;          // [n_rows][heads] for the weights, or null: see put_stats
   float* part;            // partial results, 2 slots per CTA
   int32_t* err;
   uint32_t group_mul, group_shift;  // r / group = (mulhi(r, mul) + r) >> shift for 0 <= r < 2^31
@@ -62,14 +63,19 @@ DEVI Span span_of(const AttendParams& p, int first_pos, int last_pos, int n) {
   return s;
 }
 
-// one row's result: o / l in q's type, and the natural logarithm of the sum
+// four values of one row's result, in q's type
 DEVI uint2 pack4(int act, float4 o) {
   if (act == DUPLEX_DTYPE_F16) return make_uint2(f2h(o.x, o.y), f2h(o.z, o.w));
   const __nv_bfloat162 x = __floats2bfloat162_rn(o.x, o.y), y = __floats2bfloat162_rn(o.z, o.w);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
-DEVI float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * kLn2; }
+// A row's sum l of exp2(s - m + kShift).  The weights take (m, 1 / l) rather than the logarithm, whose
+// rounding would be as large as the rest of a weight's error (1e-6 of it instead of 3e-7).
+DEVI void put_stats(const AttendParams& p, int64_t at, float m, float l) {
+  p.lse[at] = l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * kLn2;
+  if (p.stats) p.stats[at] = l == 0.f ? make_float2(0.f, 0.f) : make_float2(m, 1.f / l);
+}
 
 int kv_check(const duplex_kv_cache* c, const duplex_kv_batch* b, KvView* out);
 int device_sms(int* sms);

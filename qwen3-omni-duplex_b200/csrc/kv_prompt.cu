@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
           };
           if (p.act == DUPLEX_DTYPE_F16) put_out(std::integral_constant<int, DUPLEX_DTYPE_F16>{});
           else put_out(std::integral_constant<int, DUPLEX_DTYPE_BF16>{});
-          if (live) p.lse[(int64_t)(s.row0 + t_row) * p.heads + h * p.group + rr - t_row * p.group] = lse_of(m, l);
+          if (live) put_stats(p, (int64_t)(s.row0 + t_row) * p.heads + h * p.group + rr - t_row * p.group, m, l);
         } else {  // a piece's as they come, [dim / 4][row]
           float* part = p.part + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * prompt_part<D>();
           float4* to4 = reinterpret_cast<float4*>(part) + tid;
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
     const uint2 z = pack4(p.act, make_float4(o[e + 1].x * inv, o[e + 1].y * inv, o[e + 1].z * inv, o[e + 1].w * inv));
     dst[e / 2] = make_uint4(y.x, y.y, z.x, z.y);
   }
-  if (blockIdx.y == 0) p.lse[at] = lse_of(M, l);
+  if (blockIdx.y == 0) put_stats(p, at, M, l);
 }
 
 // Which kernel is faster, by the time each takes as measured on one B200 (128 dims, 32 query heads on 4;
