@@ -659,11 +659,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv_combine_kernel(AttendParams p,
 }
 
 // Accumulated attention weights: weights[token] += sum over the sequence's rows and the group's
-// heads of exp(s - lse), after the attention itself, by the rows' maxima and sums.  A warp owns 2 x 16 tokens: their keys stay in its
-// registers as fp16, the query rows come by, 32 at a time, through shared memory.  Reading the keys again
-// (mostly from L2) costs less than the scores' way through memory for long prompts, and is as fast for
-// decode: 18 us for 16 sequences of 6000 tokens, latency of short CTAs (at 3 of them an SM 21 us; with four
-// tiles a CTA 24 us).
+// heads of exp(s - lse), after the attention itself, by the rows' maxima and sums.  A warp owns 2 x 16
+// tokens: their keys stay in its registers as fp16, the query rows come by, 32 at a time, through shared
+// memory.  It reads the keys again (mostly from L2), dim bytes a token; keeping the scores would be 4 bytes
+// written and read for each row.  Latency of short CTAs bounds it for decode: 16 sequences of 6000 tokens
+// take 18 us with 4 CTAs an SM, 21 us with 3, 24 us with four tiles a CTA.
 constexpr int kRowChunk = 32, kWU = 2;  // rows in shared memory at a time, twice; 64-token units a CTA
 
 template <int D, int FMT>
