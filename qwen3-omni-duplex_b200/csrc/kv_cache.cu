@@ -303,23 +303,25 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 5 : R == 2 ? 3 : 1) kv_gath
   const KvView& c = p.c;
   const int P = c.block, D = c.dim, tid = threadIdx.x;
   const int b = blockIdx.y / c.heads, h = blockIdx.y - b * c.heads;
-  const int kept = min(kv_seq(c, b).n, p.keep);
-  const int base = blockIdx.x * P;
-  if (base >= kept) return;
-  const int id = p.dst[(int64_t)b * p.dst_width + blockIdx.x];
-  if ((unsigned)id >= (unsigned)c.n_blocks) {
-    if (tid == 0) set_error(p.err, DUPLEX_DEVERR_BLOCK);
-    return;
-  }
-  const int count = min(kept - base, P);
+  const int base = blockIdx.x * P, per = D / 16;
+  // the length, the block and the tokens' places are loaded together
   const int32_t* index = p.index + ((int64_t)b * c.heads + h) * p.keep + base;
-  const int per = D / 16;
   int src[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int tok = (tid + i * kThreads) / per;
-    src[i] = tok < count ? __ldg(index + tok) : -1;
+    src[i] = tok < min(P, p.keep - base) ? __ldg(index + tok) : -1;
   }
+  const int id = p.dst[(int64_t)b * p.dst_width + blockIdx.x];
+  const int count = min(min(kv_seq(c, b).n, p.keep) - base, P);
+  if (count <= 0) return;
+  if ((unsigned)id >= (unsigned)c.n_blocks) {
+    if (tid == 0) set_error(p.err, DUPLEX_DEVERR_BLOCK);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)  // places past the last token are not written
+    if ((tid + i * kThreads) / per >= count) src[i] = -1;
   uint4 x[2][R];
   float sc[2][R], amax[2] = {0.f, 0.f};
 #pragma unroll
