@@ -195,7 +195,7 @@ DEVI int pair_of(const PromptItem* list, int pairs, int64_t u) {
 // [dim / 64][row][64 dims] are K-major; V [dim / 64][token][64 dims], the same layout, is MN-major.
 template <int D> struct PromptSmem {
   static constexpr uint32_t kHalf = 128 * 128, kTile = D / 64 * kHalf;
-  static constexpr uint32_t q = 0, k = 2 * kTile, v = k + 2 * kTile, stage = v + 2 * kTile, undo = stage + 8 * 32 * 64,
+  static constexpr uint32_t q = 0, k = 2 * kTile, v = k + 2 * kTile, undo = v + 2 * kTile,
                             bars = undo + kPRows * 4;
   static constexpr uint32_t bytes = bars + 256 + 1024;
 };
@@ -526,9 +526,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       tc_fence_after();
       if (u < u_end) give_rows();
       if (mine) {
-        if (whole) {  // through 2 KB a warp, 32 dims at a time, to be written 4 lanes a row
-          uint8_t* const stage = sm + L::stage + warp * 2048;
-          auto at = [&](int row, int ch) { return stage + row * 64 + ((ch ^ ((row >> 1) & 3)) << 4); };
+        if (whole) {  // a thread's row, 16 bytes a store
+          const int64_t at = live ? (int64_t)(s.row0 + t_row) * p.heads + h * p.group + rr - t_row * p.group : 0;
+          uint4* const row_out = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + 2 * at * D);
           auto put_out = [&](auto act) {
             constexpr int A = decltype(act)::value;
 #pragma unroll 1
@@ -542,29 +542,21 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
 #pragma unroll
                 for (int e = 0; e < 32; ++e) v[e] = 0;
               }
+              if (live) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                float o[8];
+                for (int e = 0; e < 32; e += 8) {
+                  float o[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[e + k]) * inv;
-                const uint2 y = pack4(A, make_float4(o[0], o[1], o[2], o[3])), z = pack4(A, make_float4(o[4], o[5], o[6], o[7]));
-                *reinterpret_cast<uint4*>(at(lane, e / 8)) = make_uint4(y.x, y.y, z.x, z.y);
-              }
-              __syncwarp();
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int row = 8 * i + (lane >> 2), r2 = row_base + 32 * warp + row, t2 = p.by_group(r2);
-                if (r2 < row_all) {
-                  const int64_t o = (int64_t)(s.row0 + t2) * p.heads + h * p.group + r2 - t2 * p.group;
-                  *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + 2 * (o * D + 32 * q + 8 * (lane & 3))) =
-                      *reinterpret_cast<const uint4*>(at(row, lane & 3));
+                  for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[e + k]) * inv;
+                  const uint2 y = pack4(A, make_float4(o[0], o[1], o[2], o[3])), z = pack4(A, make_float4(o[4], o[5], o[6], o[7]));
+                  row_out[4 * q + e / 8] = make_uint4(y.x, y.y, z.x, z.y);
                 }
               }
             }
           };
           if (p.act == DUPLEX_DTYPE_F16) put_out(std::integral_constant<int, DUPLEX_DTYPE_F16>{});
           else put_out(std::integral_constant<int, DUPLEX_DTYPE_BF16>{});
-          if (live) put_stats(p, (int64_t)(s.row0 + t_row) * p.heads + h * p.group + rr - t_row * p.group, m, l);
+          if (live) put_stats(p, at, m, l);
         } else {  // a piece's as they come, [dim / 4][row]
           float* part = p.part + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * prompt_part<D>();
           float4* to4 = reinterpret_cast<float4*>(part) + tid;
