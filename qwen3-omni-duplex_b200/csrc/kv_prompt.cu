@@ -8,9 +8,11 @@
 //
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread owns a row.  S from tensor memory, exp2, P back as
 //                    fp16 into S's own columns (the next product's A operand)
-//   warps 8-15       keys and values from the cache's codes to fp16 operands in shared memory (exact:
-//                    code times its block's scale over the sequence's largest, a power of two), two
-//                    buffers each
+//   warps 8-15       keys and values from the cache's codes to fp16 operands in shared memory, two buffers
+//                    each: code times its block's scale over the sequence's largest.  That is exact for
+//                    powers of two up to 2^15 apart; below, a value is off by at most 2^-33 of the largest.
+//                    What else a key's scale has, the softmax multiplies the scores by; a value's scale
+//                    that is no power of two costs two roundings to fp16
 //   warp 16          issues the products: S = Q K^T (both shared memory), O += P V
 //
 // The running maximum is a reference that may lag by 2^kSlack, so O is rescaled rarely.  The products of a
@@ -50,10 +52,17 @@ struct PromptItem {
   int first_pos, last_pos;
 };
 
-struct PromptRef {  // of a sequence and head: largest key and value scale that a row sees, an id out of range
+// Of a sequence and head: the power of two in the largest key scale that a row sees, the largest value scale,
+// and whether scores need a factor or a mask by their block (a key scale that is no power of two, an id out of
+// range).
+struct PromptRef {
   float k, v;
-  int bad, pad;
+  int by_block, pad;
 };
+
+// x = pow2_of(x) * mantissa_of(x)
+DEVI float pow2_of(float x) { return __uint_as_float(__float_as_uint(x) & 0x7F800000u); }
+DEVI float mantissa_of(float x) { return __uint_as_float((__float_as_uint(x) & 0x7FFFFFu) | 0x3F800000u); }
 
 struct PromptParams {
   AttendParams a;
@@ -86,14 +95,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
     const KvSeq s = kv_seq(c, b);
     const int lo_x = p.window ? s.n - s.rows - p.window + 1 : 0, cols = s.rows ? (s.n + c.block - 1) / c.block : 0;
     float mk = 0.f, mv = 0.f;
-    int bad = 0;
+    int by_block = 0;
     for (int col = tid; col < cols; col += kPlanThreads) {
       const int tok = col * c.block;
       if (tok + c.block <= lo_x && tok >= p.sinks) continue;
       const int id = kv_block_at(c, b, col, p.err);
-      if (id < 0) bad = 1;
+      if (id < 0) by_block = 1;
       else {
-        mk = fmaxf(mk, __ldg(c.k_scale + (int64_t)id * c.heads + h));
+        const float k = __ldg(c.k_scale + (int64_t)id * c.heads + h);
+        by_block |= k != pow2_of(k);
+        mk = fmaxf(mk, pow2_of(k));
         mv = fmaxf(mv, __ldg(c.v_scale + (int64_t)id * c.heads + h));
       }
     }
@@ -106,14 +117,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
       s_k[warp] = mk;
       s_v[warp] = mv;
     }
-    bad = __syncthreads_or(bad);
+    by_block = __syncthreads_or(by_block);
     if (tid == 0) {
 #pragma unroll
       for (int w = 1; w < kPlanThreads / 32; ++w) {
         mk = fmaxf(mk, s_k[w]);
         mv = fmaxf(mv, s_v[w]);
       }
-      pp.ref[blockIdx.x - 1] = PromptRef{fmaxf(mk, pow2f(-126)), fmaxf(mv, pow2f(-126)), bad, 0};
+      pp.ref[blockIdx.x - 1] = PromptRef{fmaxf(mk, pow2f(-126)), fmaxf(mv, pow2f(-126)), by_block, 0};
     }
     return;
   }
@@ -408,7 +419,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       for (int j = 0; mine && j < n; ++j) {
         const int base = x.base_of(x.i0 + j);
         // (rows past the last have zeros for a query and are not written: they need no mask)
-        const bool masked = ref.bad || base + kPTok - 1 > t_first ||
+        const bool masked = ref.by_block || base + kPTok - 1 > t_first ||
                             (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
         if (!(ok = wait(s_full + mt, n_s + j))) break;
         tc_fence_after();
@@ -424,18 +435,22 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
             tc_wait_ld();
             auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1; };  // bits of columns < k
             const uint32_t see = below(k_max + 1 - 32 * q) & (~below(k_min + 1 - 32 * q) | below(k_sink - 32 * q));
-#pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = (see >> e) & 1u ? w[e] : __float_as_uint(-INFINITY);
-            if (ref.bad) {
+            if (ref.by_block) {
 #pragma unroll 1
               for (int o = 0; o < 32; o += 16) {  // 16 tokens are in one block
                 const int k = base + 32 * q + o;
-                const bool gone = k < x.it.sp.end && (unsigned)c.table[(int64_t)x.it.b * c.width + k / c.block] >= (unsigned)c.n_blocks;
+                float f = 1.f;
+                if (k < x.it.sp.end) {
+                  const int id = c.table[(int64_t)x.it.b * c.width + k / c.block];
+                  f = (unsigned)id < (unsigned)c.n_blocks ? mantissa_of(__ldg(c.k_scale + (int64_t)id * c.heads + x.h)) : 0.f;
+                }
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                  if (gone && (e >> 4) == (o >> 4)) w[e] = __float_as_uint(-INFINITY);
+                  if ((e >> 4) == (o >> 4)) w[e] = f == 0.f ? __float_as_uint(-INFINITY) : __float_as_uint(__uint_as_float(w[e]) * f);
               }
             }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) w[e] = (see >> e) & 1u ? w[e] : __float_as_uint(-INFINITY);
             __syncwarp();
             tmem_st16(ts + 32 * q, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
             tmem_st16(ts + 32 * q + 16, reinterpret_cast<const uint32_t(&)[16]>(w[16]));
@@ -656,7 +671,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         id = id_next;
         id_next = id_of(i + 2);
         if (use > 0 && !(ok = wait(k_empty + slot, use - 1))) break;
-        put(sm + L::k + slot * L::kTile, base, kx, kr * inv_k);
+        put(sm + L::k + slot * L::kTile, base, kx, pow2_of(kr) * inv_k);
         if (lane == 0) mbar_arrive(k_full + slot);
         if (j + 1 < n) load(i + 1, id, c.k, c.k_scale, kx, kr);
         if (use > 0 && !(ok = wait(v_empty + slot, use - 1))) break;

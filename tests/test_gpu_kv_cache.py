@@ -173,6 +173,27 @@ def test_attend_extreme_sizes(cuda, dt, size):
     assert bool(((lse.double() - rl).abs() <= dp + 2.0 ** -21 * (1 + rl.abs())).all())
 
 
+@pytest.mark.parametrize("rows,lens", [([2, 1], [300, 80]), ([1500, 700], [2900, 700])], ids=["few", "many"])
+@pytest.mark.parametrize("fmt,dt", [("e4m3", "bf16"), ("int8", "fp16")])
+@pytest.mark.parametrize("window", [0, 150])
+def test_attend_scales_of_any_value(cuda, rows, lens, fmt, dt, window):
+    """Scales that another writer chose: not powers of two, and up to 2^9 apart."""
+    from duplex.streaming import kv_cache
+    s = make(cuda, 2, rows, lens, 8, 2, 64, 32, fmt, TYPES[dt], seed=11)
+    g = torch.Generator(device=cuda).manual_seed(5)
+    for n in ("k_scale", "v_scale"):
+        s[n] *= torch.exp2(torch.rand(s[n].shape, generator=g, device=cuda) * 5 - 4)
+    out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, sinks=3, return_lse=True)
+    ro, rl, mean, bulk, _ = kv_ref.attend(s["q"], s["k"], s["v"], s["k_scale"], s["v_scale"], s["table"], lens, rows,
+                                          window, 3, 1 / 8)
+    # a key's scale is a factor in fp32; a value's is rounded to fp16 and so is its product with the code (half a
+    # step each, 2^-11), beside the probability's own rounding
+    dp = 2.0 ** -19 * bulk + 2.0 ** -21 * (1 + bulk)
+    tol = (3 * 2.0 ** -11 + 2 * dp + 2.0 ** -19)[..., None] * mean + torch.finfo(s["q"].dtype).eps / 2 * ro.abs() + 2.0 ** -24
+    assert bool(((lse.double() - rl).abs() <= dp + 2.0 ** -21 * (1 + rl.abs())).all())
+    assert bool(((out.double() - ro).abs() <= tol).all())
+
+
 def test_attend_uniform_rows_and_strides(cuda):
     """cu_q left out; q with strides that need a copy; softmax_scale given."""
     from duplex.streaming import kv_cache
