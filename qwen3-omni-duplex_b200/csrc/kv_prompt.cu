@@ -770,6 +770,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
   static_assert(kJoinThreads == kPRows, "a thread is a row");
   const AttendParams& p = pp.a;
   pdl_wait();
+  pdl_launch_dependents();
   const int64_t total = *pp.total, share = share_of(total, ctas);
   const int64_t u = (int64_t)(blockIdx.x + 1) * share;
   if (u >= total) return;
