@@ -8,7 +8,7 @@
 // rounding, so each is read once.  Short CTAs with a chain of dependent loads (offsets, length, block id,
 // rows): what counts is how many are on an SM, so the rounds are a template argument and registers bounded.
 // One B200: 13,000 new tokens of 4 sequences, 4 KV heads of 128: 14 us (2.3 TB/s; with 98 registers 35 us);
-// 12 sequences of 16,384 tokens to 8192: 80 us, 28 of them the selection.
+// 12 sequences of 16,384 tokens to 8192: 78 us, 28 of them the selection.
 #include <type_traits>
 
 #include "kv.cuh"
@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
   __shared__ int s_digit, s_above;
   const KvView& c = p.c;
   const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
   const int n = kv_seq(c, b).n;
   if (h == 0 && tid == 0) p.new_len[b] = min(n, p.keep);
   int32_t* out = p.index + ((int64_t)b * c.heads + h) * p.keep;
@@ -304,16 +305,18 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 5 : R == 2 ? 3 : 1) kv_gath
   const int P = c.block, D = c.dim, tid = threadIdx.x;
   const int b = blockIdx.y / c.heads, h = blockIdx.y - b * c.heads;
   const int base = blockIdx.x * P, per = D / 16;
-  // the length, the block and the tokens' places are loaded together
+  // the length and the block are loaded while the selection ends, or with the tokens' places (one sequence of
+  // 4096: 20.5 -> 18.4 us); the places by plain loads, since they are written while this kernel starts
+  const int id = p.dst[(int64_t)b * p.dst_width + blockIdx.x];
+  const int count = min(min(kv_seq(c, b).n, p.keep) - base, P);
+  pdl_wait();
   const int32_t* index = p.index + ((int64_t)b * c.heads + h) * p.keep + base;
   int src[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int tok = (tid + i * kThreads) / per;
-    src[i] = tok < min(P, p.keep - base) ? __ldg(index + tok) : -1;
+    src[i] = tok < min(P, p.keep - base) ? index[tok] : -1;
   }
-  const int id = p.dst[(int64_t)b * p.dst_width + blockIdx.x];
-  const int count = min(min(kv_seq(c, b).n, p.keep) - base, P);
   if (count <= 0) return;
   if ((unsigned)id >= (unsigned)c.n_blocks) {
     if (tid == 0) set_error(p.err, DUPLEX_DEVERR_BLOCK);
@@ -336,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 5 : R == 2 ? 3 : 1) kv_gath
   }
   const int64_t at = ((int64_t)id * c.heads + h) * P;
   for (int i = tid; i < count; i += kThreads) {
-    const int s = __ldg(index + i);
+    const int s = index[i];
     c.weights[at + i] = s < 0 ? 0.f : c.weights[((int64_t)(s / P) * c.heads + h) * P + (s & (P - 1))];
   }
 #pragma unroll
@@ -481,15 +484,22 @@ extern "C" int duplex_kv_evict(const duplex_kv_cache* cache, const duplex_kv_bat
     kv_select_kernel<false><<<heads, kSelThreads, 0, st>>>(p);
   }
   if (int rc = record_cuda(cudaGetLastError())) return rc;
-  const dim3 grid((keep + cache->block - 1) / cache->block, batch->batch * cache->kv_heads);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((keep + cache->block - 1) / cache->block, batch->batch * cache->kv_heads);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   const int rounds = (cache->block * cache->dim / 16 + kThreads - 1) / kThreads;
   auto go = [&](auto fmt) {
     constexpr int F = decltype(fmt)::value;
-    if (rounds == 1) kv_gather_kernel<F, 1><<<grid, kThreads, 0, st>>>(p);
-    else if (rounds == 2) kv_gather_kernel<F, 2><<<grid, kThreads, 0, st>>>(p);
-    else kv_gather_kernel<F, 4><<<grid, kThreads, 0, st>>>(p);
+    return rounds == 1   ? cudaLaunchKernelEx(&cfg, kv_gather_kernel<F, 1>, p)
+           : rounds == 2 ? cudaLaunchKernelEx(&cfg, kv_gather_kernel<F, 2>, p)
+                         : cudaLaunchKernelEx(&cfg, kv_gather_kernel<F, 4>, p);
   };
-  if (cache->format == DUPLEX_KV_E4M3) go(std::integral_constant<int, DUPLEX_KV_E4M3>{});
-  else go(std::integral_constant<int, DUPLEX_KV_INT8>{});
-  return record_cuda(cudaGetLastError());
+  return record_cuda(cache->format == DUPLEX_KV_E4M3 ? go(std::integral_constant<int, DUPLEX_KV_E4M3>{})
+                                                     : go(std::integral_constant<int, DUPLEX_KV_INT8>{}));
 }
