@@ -45,6 +45,7 @@ extern "C" {
 #define DUPLEX_DEVERR_NONFINITE 4 /* duplex_stack_forward: a partial layer output was NaN or
                                      beyond +-2^26 and was clamped (its fixed-point sum) */
 #define DUPLEX_DEVERR_BLOCK 8     /* a KV cache's block id outside [0, n_blocks): its tokens were left out */
+#define DUPLEX_DEVERR_OFFSETS 16  /* a KV cache's row offsets fall: the call did nothing */
 /* duplex_stack_forward also records, from this bit up, which of its waits gave up
  * first: 1 ring slot free, 2 routing plan, 3 ring slot filled, 4 grid barrier,
  * 5 drain, 6 cluster exchange. */
@@ -501,7 +502,8 @@ int duplex_moe_forward_noalloc(const void* x, int act_dtype, int32_t T, const vo
  * n_rows; NULL: n_rows / batch each).  All are device memory, read by the kernels: a captured
  * call follows their values.  Rows behind the last sequence's are left alone; lengths and rows
  * are held inside width * block and n_rows; a block id out of range is reported in err
- * (DUPLEX_DEVERR_BLOCK) and its tokens are left out.  batch <= DUPLEX_KV_MAX_BATCH,
+ * (DUPLEX_DEVERR_BLOCK) and its tokens are left out; a call whose row offsets fall anywhere
+ * (cu_rows[b + 1] < cu_rows[b]) reports that (DUPLEX_DEVERR_OFFSETS) and does nothing.  batch <= DUPLEX_KV_MAX_BATCH,
  * batch * kv_heads <= 65535.
  */
 #define DUPLEX_KV_E4M3 0

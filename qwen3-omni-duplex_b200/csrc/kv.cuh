@@ -28,7 +28,7 @@ struct KvView {
 };
 
 // rows [row0, row0 + rows) of sequence b and its number of cached tokens n, held inside the
-// buffers whatever the device arrays say
+// buffers whatever the device arrays say.  (Each sequence by itself: see offsets_fall for all of them.)
 struct KvSeq {
   int row0, rows, n;
 };
@@ -49,6 +49,17 @@ DEVI KvSeq kv_seq(const KvView& c, int b) {
   const int n = max(c.kv_len[b], 0);
   s.n = n > cap ? (int)cap : n;
   return s;
+}
+
+// Whether this thread's share of the row offsets falls somewhere.  Where none does, no row is in two
+// sequences, and what is laid out by rows (the item list, the clusters' grid) has the host's bounds; a
+// call whose offsets fall stores and writes nothing but its error bit.
+DEVI bool offset_falls(const KvView& c, int b) { return c.cu && c.cu[b + 1] < c.cu[b]; }
+
+DEVI bool offsets_fall(const KvView& c) {
+  bool fall = false;
+  for (int b = threadIdx.x; c.cu && b < c.batch; b += blockDim.x) fall |= offset_falls(c, b);
+  return fall;
 }
 
 // the block that holds token j of sequence b, or -1 (and the error bit) if its id is out of range

@@ -40,6 +40,10 @@ struct Plan {
   int64_t total, share;
 };
 
+// The units of a sequence where the row offsets fall: below any sum of the others, and half of
+// DUPLEX_KV_MAX_BATCH of it still a number.
+constexpr int64_t kFalls = -(1ll << 51);
+
 DEVI int tiles_of(const KvSeq& s, int group, int rows) { return (int)(((int64_t)s.rows * group + rows - 1) / rows); }
 
 DEVI int units_of(const KvSeq& s, const AttendParams& p, int rows) {
@@ -62,6 +66,7 @@ DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
     if (b < B) {
       const KvSeq s = kv_seq(p.c, b);
       u = (int64_t)p.c.heads * tiles_of(s, p.group, ROWS) * (ITEMS ? 1 : units_of(s, p, ROWS));
+      if (offset_falls(p.c, b)) u = kFalls;
     }
     int64_t incl = u;
 #pragma unroll
@@ -83,6 +88,10 @@ DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
   }
   if (tid == 0) off[B] = base;
   __syncthreads();
+  if (base < 0) {
+    base = 0;  // no work
+    if (tid == 0) set_error(p.err, DUPLEX_DEVERR_OFFSETS);
+  }
   Plan pl;
   pl.total = base;
   pl.share = (base + ctas - 1) / ctas;
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
   __shared__ uint2 sq[2][kRowChunk / 8][D / 16][32];
   __shared__ float s_sc[2][kRowChunk];
   __shared__ float2 s_st[2][kRowChunk];
-  __shared__ int s_pos[2][kRowChunk];
+  __shared__ int s_pos[2][kRowChunk], s_fall[kWarps];
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
@@ -686,6 +695,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
     pdl_wait();
     return;
   }
+  s_fall[warp] = __any_sync(~0u, offsets_fall(c));
   uint32_t kf[kWU][D / 16][4];  // the keys as fragments, fp16
   float ks[kWU], sum[kWU][2];
   int64_t at[kWU];  // the warp's 16 tokens' slot, or -1
@@ -748,6 +758,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
   pdl_wait();  // for the statistics: the keys were there before (16 sequences of 6000 tokens 54 -> 51 us)
   load(t0 * p.group);
   stage(0);
+  if (s_fall[0] | s_fall[1] | s_fall[2] | s_fall[3]) return;  // (reported by the attention)
   for (int r0 = t0 * p.group; r0 < r1; r0 += kRowChunk, buf ^= 1) {
     const bool more = r0 + kRowChunk < r1;
     if (more) load(r0 + kRowChunk);

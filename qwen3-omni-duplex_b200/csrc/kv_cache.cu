@@ -50,6 +50,12 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
   const int P = c.block, D = c.dim, h = blockIdx.y, tid = threadIdx.x;
   const bool val = blockIdx.z != 0;
   const int64_t w = blockIdx.x;
+  // Every CTA finds out whether the offsets fall before it stores: loads that are under way here, looked at with
+  // the values.  This CTA reports it, whether it has tokens to store or not.
+  int2 cu = make_int2(0, 0);
+  if (c.cu && tid < c.batch) cu = make_int2(c.cu[tid], c.cu[tid + 1]);
+  if (c.cu && w == 0 && h == 0 && !val && __syncthreads_or(offsets_fall(c)) && tid == 0)
+    set_error(p.err, DUPLEX_DEVERR_OFFSETS);
   // the last b whose first item is <= w, 32 sequences a look
   int lo = 0, left = c.batch;
   const int lane = tid & 31;
@@ -101,8 +107,11 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
       amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
   }
+  bool fall = cu.y < cu.x;
+  for (int i = tid + kThreads; c.cu && i < c.batch; i += kThreads) fall |= offset_falls(c, i);
+  amax = block_max(fall ? INFINITY : amax, red);  // (the values are finite)
+  if (amax == INFINITY) return;
   if (bad) set_error(p.err, DUPLEX_DEVERR_NONFINITE);
-  amax = block_max(amax, red);
   int e2 = KvFmt<FMT>::exponent(amax);
   if (new0 > 0) {  // older tokens in the block: its scale never falls, and their codes follow it
     const float old = *scale;

@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
     return before + incl - x;
   };
   int64_t base = 0, all = 0;
+  const bool fall = offsets_fall(c);
   for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int t = 0;
@@ -157,8 +158,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
     base += all;
   }
   if (tid == 0) tiles[B] = (int)base;
-  __syncthreads();
-  const int pairs = tiles[B];
+  // the list has room for the pairs of offsets that rise (max_pairs)
+  const bool none = __syncthreads_or(fall);
+  if (none && tid == 0) set_error(p.err, DUPLEX_DEVERR_OFFSETS);
+  const int pairs = none ? 0 : tiles[B];
   base = 0;
   for (int i0 = 0; i0 < pairs; i0 += kPlanThreads) {
     const int i = i0 + tid;

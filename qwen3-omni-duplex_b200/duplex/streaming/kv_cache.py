@@ -22,8 +22,9 @@ All index tensors are read on the device: a call makes no host synchronisation, 
 follows new lengths, tables and values.  Calls run on the current stream of the cache's device;
 `kv_attend` and `kv_evict` take their workspace from torch's allocator, so calls on several streams
 do not share one.  Inference only, no autograd formula.  Errors in arguments raise RuntimeError;
-block ids out of range and values that are not finite are reported in `err` (int32 [1], bits
-_lib.DEVERR_BLOCK and _lib.DEVERR_NONFINITE) if it is given.
+what the device arrays get wrong is reported in `err` (int32 [1]) if it is given: block ids out of
+range (_lib.DEVERR_BLOCK), values that are not finite (_lib.DEVERR_NONFINITE), and row offsets that
+fall (_lib.DEVERR_OFFSETS; the call then does nothing else, `out` and the caches stay as they were).
 """
 
 from __future__ import annotations
