@@ -10,9 +10,12 @@
 //                    fp16 into S's own columns (the next product's A operand)
 //   warps 8-15       keys and values from the cache's codes to fp16 operands in shared memory, two buffers
 //                    each: code times its block's scale over the sequence's largest.  That is exact for
-//                    powers of two up to 2^15 apart; below, a value is off by at most 2^-33 of the largest.
-//                    What else a key's scale has, the softmax multiplies the scores by; a value's scale
-//                    that is no power of two costs two roundings to fp16
+//                    powers of two up to 2^14 apart.  Where a sequence has others, the operands are the
+//                    codes themselves and the scales are factors in the softmax, in fp32: of the scores for
+//                    keys, of the probabilities for values (over the largest scale that the row has seen,
+//                    with which its O is rescaled like with the maximum).  So a row's result hangs on what
+//                    the row sees, whatever the blocks that it does not.  Such a prompt of 8192: 1.6 times
+//                    the time
 //   warp 16          issues the products: S = Q K^T (both shared memory), O += P V
 //
 // The running maximum is a reference that may lag by 2^kSlack, so O is rescaled rarely.  The products of a
@@ -53,16 +56,15 @@ struct PromptItem {
 };
 
 // Of a sequence and head: the power of two in the largest key scale that a row sees, the largest value scale,
-// and whether scores need a factor or a mask by their block (a key scale that is no power of two, an id out of
-// range).
+// and whether scores and probabilities need a factor by their block: a scale is no power of two, or far below
+// the largest (e4m3's least code is 2^-9, fp16's least step 2^-24), or an id is out of range (a mask).
 struct PromptRef {
   float k, v;
   int by_block, pad;
 };
 
-// x = pow2_of(x) * mantissa_of(x)
 DEVI float pow2_of(float x) { return __uint_as_float(__float_as_uint(x) & 0x7F800000u); }
-DEVI float mantissa_of(float x) { return __uint_as_float((__float_as_uint(x) & 0x7FFFFFu) | 0x3F800000u); }
+DEVI bool far_below(float least, float most) { return least < most * 6.103515625e-5f; }  // 2^-14
 
 struct PromptParams {
   AttendParams a;
@@ -85,7 +87,7 @@ constexpr int kPlanThreads = 256;
 __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptParams pp) {
   extern __shared__ int tiles[];  // [batch + 1] row tiles before each sequence
   __shared__ int64_t warp_sum[kPlanThreads / 32];
-  __shared__ float s_k[kPlanThreads / 32], s_v[kPlanThreads / 32];
+  __shared__ float2 s_k[kPlanThreads / 32], s_v[kPlanThreads / 32];
   const AttendParams& p = pp.a;
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = c.batch;
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
     const int b = (blockIdx.x - 1) / c.heads, h = (blockIdx.x - 1) - b * c.heads;
     const KvSeq s = kv_seq(c, b);
     const int lo_x = p.window ? s.n - s.rows - p.window + 1 : 0, cols = s.rows ? (s.n + c.block - 1) / c.block : 0;
-    float mk = 0.f, mv = 0.f;
+    float mk = 0.f, mv = 0.f, lk = INFINITY, lv = INFINITY;  // largest and least (a scale of 0 is exact anywhere)
     int by_block = 0;
     for (int col = tid; col < cols; col += kPlanThreads) {
       const int tok = col * c.block;
@@ -102,28 +104,35 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
       const int id = kv_block_at(c, b, col, p.err);
       if (id < 0) by_block = 1;
       else {
-        const float k = __ldg(c.k_scale + (int64_t)id * c.heads + h);
-        by_block |= k != pow2_of(k);
+        const float k = __ldg(c.k_scale + (int64_t)id * c.heads + h), v = __ldg(c.v_scale + (int64_t)id * c.heads + h);
+        by_block |= k != pow2_of(k) || v != pow2_of(v);
         mk = fmaxf(mk, pow2_of(k));
-        mv = fmaxf(mv, __ldg(c.v_scale + (int64_t)id * c.heads + h));
+        mv = fmaxf(mv, v);
+        if (k != 0.f) lk = fminf(lk, k);
+        if (v != 0.f) lv = fminf(lv, v);
       }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       mk = fmaxf(mk, __shfl_xor_sync(~0u, mk, o));
       mv = fmaxf(mv, __shfl_xor_sync(~0u, mv, o));
+      lk = fminf(lk, __shfl_xor_sync(~0u, lk, o));
+      lv = fminf(lv, __shfl_xor_sync(~0u, lv, o));
     }
     if (lane == 0) {
-      s_k[warp] = mk;
-      s_v[warp] = mv;
+      s_k[warp] = make_float2(mk, lk);
+      s_v[warp] = make_float2(mv, lv);
     }
     by_block = __syncthreads_or(by_block);
     if (tid == 0) {
 #pragma unroll
       for (int w = 1; w < kPlanThreads / 32; ++w) {
-        mk = fmaxf(mk, s_k[w]);
-        mv = fmaxf(mv, s_v[w]);
+        mk = fmaxf(mk, s_k[w].x);
+        mv = fmaxf(mv, s_v[w].x);
+        lk = fminf(lk, s_k[w].y);
+        lv = fminf(lv, s_v[w].y);
       }
+      by_block |= far_below(lk, mk) || far_below(lv, mv);
       pp.ref[blockIdx.x - 1] = PromptRef{fmaxf(mk, pow2f(-126)), fmaxf(mv, pow2f(-126)), by_block, 0};
     }
     return;
@@ -418,126 +427,171 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       const int t_last = s.n - s.rows + p.by_group(row_hi - 1);
       const bool mine = mt == 0 || x.two;
       const float cs = fmaxf(s_undo[tid] * fabsf(p.scale_log2) * ref.k, 1.2e-38f);  // not 0: hidden scores are -inf
-      float m = -INFINITY, l = 0.f;
-      for (int j = 0; mine && j < n; ++j) {
-        const int base = x.base_of(x.i0 + j);
-        // (rows past the last have zeros for a query and are not written: they need no mask)
-        const bool masked = ref.by_block || base + kPTok - 1 > t_first ||
-                            (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
-        if (!(ok = wait(s_full + mt, n_s + j))) break;
-        tc_fence_after();
-        // The loops are short on purpose: unrolled over the row they outgrow the instruction caches, and
-        // the tile takes 1.8 times as long.
-        float mx = -INFINITY;
-        if (masked) {
-          const int k_max = pos - base, k_min = wlo - base, k_sink = p.sinks - base;  // columns k <= k_max, k > k_min or k < k_sink
+      float m = -INFINITY, l = 0.f, vref = ref.v;  // O is in units of vref
+      auto tiles = [&](auto by) {
+        constexpr bool BY = decltype(by)::value;  // factors by block, of scores and probabilities
+        if (BY) vref = pow2f(-126);
+        for (int j = 0; mine && j < n; ++j) {
+          const int base = x.base_of(x.i0 + j);
+          // (rows past the last have zeros for a query and are not written: they need no mask)
+          const bool masked = BY || base + kPTok - 1 > t_first ||
+                              (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
+          // lane i (of 8): the scales of the block that holds tokens base + 16 i .. + 15; -1: an id out of range
+          float kf = -1.f, vs = 0.f;
+          if (BY) {
+            const int k = base + 16 * (lane & 7), id = k < x.it.sp.end ? c.table[(int64_t)x.it.b * c.width + k / c.block] : -1;
+            if ((unsigned)id < (unsigned)c.n_blocks) {
+              kf = __ldg(c.k_scale + (int64_t)id * c.heads + x.h) / ref.k;
+              vs = __ldg(c.v_scale + (int64_t)id * c.heads + x.h);
+            }
+          }
+          if (!(ok = wait(s_full + mt, n_s + j))) return;
+          tc_fence_after();
+          // The loops are short on purpose: unrolled over the row they outgrow the instruction caches, and
+          // the tile takes 1.8 times as long.
+          float mx = -INFINITY;
+          if (masked) {
+            const int k_max = pos - base, k_min = wlo - base, k_sink = p.sinks - base;  // columns k <= k_max, k > k_min or k < k_sink
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[32];
-            tmem_ld32(ts + 32 * q, w);
-            tc_wait_ld();
-            auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1; };  // bits of columns < k
-            const uint32_t see = below(k_max + 1 - 32 * q) & (~below(k_min + 1 - 32 * q) | below(k_sink - 32 * q));
-            if (ref.by_block) {
-#pragma unroll 1
-              for (int o = 0; o < 32; o += 16) {  // 16 tokens are in one block
-                const int k = base + 32 * q + o;
-                float f = 1.f;
-                if (k < x.it.sp.end) {
-                  const int id = c.table[(int64_t)x.it.b * c.width + k / c.block];
-                  f = (unsigned)id < (unsigned)c.n_blocks ? mantissa_of(__ldg(c.k_scale + (int64_t)id * c.heads + x.h)) : 0.f;
-                }
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[32];
+              tmem_ld32(ts + 32 * q, w);
+              tc_wait_ld();
+              auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1; };  // bits of columns < k
+              const uint32_t see = below(k_max + 1 - 32 * q) & (~below(k_min + 1 - 32 * q) | below(k_sink - 32 * q));
+              if (BY) {
+                const float f[2] = {__shfl_sync(~0u, kf, 2 * q), __shfl_sync(~0u, kf, 2 * q + 1)};
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                  if ((e >> 4) == (o >> 4)) w[e] = f == 0.f ? __float_as_uint(-INFINITY) : __float_as_uint(__uint_as_float(w[e]) * f);
+                  w[e] = f[e >> 4] < 0.f ? __float_as_uint(-INFINITY) : __float_as_uint(__uint_as_float(w[e]) * f[e >> 4]);
+              }
+#pragma unroll
+              for (int e = 0; e < 32; ++e) w[e] = (see >> e) & 1u ? w[e] : __float_as_uint(-INFINITY);
+              __syncwarp();
+              tmem_st16(ts + 32 * q, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
+              tmem_st16(ts + 32 * q + 16, reinterpret_cast<const uint32_t(&)[16]>(w[16]));
+#pragma unroll
+              for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(w[e]));
+            }
+            tc_wait_st();
+          } else {
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) {
+              uint32_t w[2][32];
+              tmem_ld32(ts + 64 * q, w[0]);
+              tmem_ld32(ts + 64 * q + 32, w[1]);
+              tc_wait_ld();
+              float y[4] = {mx, mx, mx, mx};
+#pragma unroll
+              for (int e = 0; e < 32; ++e) y[e & 3] = max3(y[e & 3], __uint_as_float(w[0][e]), __uint_as_float(w[1][e]));
+              mx = max3(y[0], y[1], fmaxf(y[2], y[3]));
+            }
+          }
+          mx *= cs;
+          float vf = 1.f;
+          if (BY) {  // the largest value scale of what the row sees
+            float v = vref;
+#pragma unroll 1
+            for (int i = 0; i < kPTok / 16; ++i) {
+              const float y = __shfl_sync(~0u, vs, i);
+              const int k = base + 16 * i, last = min(k + 15, pos);  // the last of the 16 that the row may see
+              if (last >= k && (last > wlo || k < p.sinks)) v = fmaxf(v, y);
+            }
+            vf = vref / v;
+            vref = v;
+          }
+          if (__any_sync(~0u, mx > m + kSlack || (BY && vf != 1.f))) {
+            const float top = mx > m + kSlack ? mx : m;
+            float f = top == m ? 1.f : ex2(m - top);
+            m = top;
+            l *= f;
+            if (BY) f *= vf;
+            if (j > 0) {
+#pragma unroll 1
+              for (int q = 0; q < D / 16; ++q) {
+                uint32_t o[16];
+                tmem_ld16(to + 16 * q, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(to + 16 * q, o);
               }
             }
-#pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = (see >> e) & 1u ? w[e] : __float_as_uint(-INFINITY);
+          }
+          const float add = kShift - (m == -INFINITY ? 0.f : m);
+          const float2 cs2 = make_float2(cs, cs), add2 = make_float2(add, add);
+          float2 ls = make_float2(0.f, 0.f);
+          if constexpr (BY) {  // the probabilities' sum without, the operand with the value's scale
+            const float rv = 1.f / vref;
             __syncwarp();
-            tmem_st16(ts + 32 * q, reinterpret_cast<const uint32_t(&)[16]>(w[0]));
-            tmem_st16(ts + 32 * q + 16, reinterpret_cast<const uint32_t(&)[16]>(w[16]));
-#pragma unroll
-            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(w[e]));
-          }
-          tc_wait_st();
-        } else {
 #pragma unroll 1
-          for (int q = 0; q < 2; ++q) {
-            uint32_t w[2][32];
-            tmem_ld32(ts + 64 * q, w[0]);
-            tmem_ld32(ts + 64 * q + 32, w[1]);
-            tc_wait_ld();
-            float y[4] = {mx, mx, mx, mx};
-#pragma unroll
-            for (int e = 0; e < 32; ++e) y[e & 3] = max3(y[e & 3], __uint_as_float(w[0][e]), __uint_as_float(w[1][e]));
-            mx = max3(y[0], y[1], fmaxf(y[2], y[3]));
-          }
-        }
-        mx *= cs;
-        if (__any_sync(~0u, mx > m + kSlack)) {
-          const float top = mx > m + kSlack ? mx : m;
-          const float f = top == m ? 1.f : ex2(m - top);
-          m = top;
-          l *= f;
-          if (j > 0) {
-#pragma unroll 1
-            for (int q = 0; q < D / 16; ++q) {
-              uint32_t o[16];
-              tmem_ld16(to + 16 * q, o);
+            for (int q = 0; q < kPTok / 16; ++q) {
+              // (beyond [0, 1], where the row sees none of it, it must not make a NaN of 0)
+              const float f = fmaxf(fminf(__shfl_sync(~0u, vs, q) * rv, 1.f), 0.f);
+              uint32_t w[16], P[8];
+              tmem_ld16(ts + 16 * q, w);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st16(to + 16 * q, o);
+              for (int e = 0; e < 16; e += 2) {
+                const float2 y = fma2(make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])), cs2, add2);
+                const float2 z = make_float2(ex2(y.x), ex2(y.y));
+                ls = add2f(ls, z);
+                P[e / 2] = f2h(z.x * f, z.y * f);
+              }
+              tmem_st8(ts + 8 * q, P);
+              if (q == kPTok / 32 - 1) {
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_half + mt);
+              }
             }
-          }
-        }
-        const float add = kShift - (m == -INFINITY ? 0.f : m);
-        const float2 cs2 = make_float2(cs, cs), add2 = make_float2(add, add);
-        float2 ls = make_float2(0.f, 0.f);
-        {
-          uint32_t va[32], vb[32];
-          auto part = [&](const uint32_t (&w)[32], int q) {  // P's columns 16 q .. + 15 lie over scores that are already read
-            uint32_t P[16];
+          } else {
+            uint32_t va[32], vb[32];
+            auto part = [&](const uint32_t (&w)[32], int q) {  // P's columns 16 q .. + 15 lie over scores that are already read
+              uint32_t P[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = fma2(make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])), cs2, add2);
-              const float2 z = make_float2(ex2(y.x), ex2(y.y));
-              ls = add2f(ls, z);
-              P[e / 2] = f2h(z.x, z.y);
-            }
-            tmem_st16(ts + 16 * q, P);
-          };
-          __syncwarp();
-          tmem_ld32(ts, va);
+              for (int e = 0; e < 32; e += 2) {
+                const float2 y = fma2(make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])), cs2, add2);
+                const float2 z = make_float2(ex2(y.x), ex2(y.y));
+                ls = add2f(ls, z);
+                P[e / 2] = f2h(z.x, z.y);
+              }
+              tmem_st16(ts + 16 * q, P);
+            };
+            __syncwarp();
+            tmem_ld32(ts, va);
 #pragma unroll 1
-          for (int q = 0; q < 4; q += 2) {
-            tc_wait_ld();
-            tmem_ld32(ts + 32 * q + 32, vb);
-            part(va, q);
-            tc_wait_ld();
-            if (q == 0) tmem_ld32(ts + 64, va);
-            part(vb, q + 1);
-            if (q == 0) {  // the products of the first 64 tokens can start
-              tc_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(p_half + mt);
+            for (int q = 0; q < 4; q += 2) {
+              tc_wait_ld();
+              tmem_ld32(ts + 32 * q + 32, vb);
+              part(va, q);
+              tc_wait_ld();
+              if (q == 0) tmem_ld32(ts + 64, va);
+              part(vb, q + 1);
+              if (q == 0) {  // the products of the first 64 tokens can start
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_half + mt);
+              }
             }
           }
+          l += ls.x + ls.y;
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_ready + mt);
         }
-        l += ls.x + ls.y;
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + mt);
-      }
+      };
+      if (__builtin_expect(!ref.by_block, 1)) tiles(std::false_type{});
+      else tiles(std::true_type{});
       // ---- the row's result.  Once all products are done (both tiles wait for them) the next piece's rows
       // take the query rows' place, so its first scores are computed under the writing of this one's results.
       if (!ok) break;
       const bool whole = x.whole, first = u == u_begin;
       const int h = x.h;
-      const float inv = whole ? (l == 0.f ? 0.f : ref.v / l) : ref.v;
+      const float inv = whole ? (l == 0.f ? 0.f : vref / l) : vref;
       u += x.len;
       if (u < u_end) next();
       if (n > 0 && !(ok = wait(o_full, n_o))) break;
@@ -617,7 +671,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       find_piece(pp, u, u_end, pi, x);
       const int n = x.n, end = x.i0 + n;
       const int lo_x = p.window ? x.it.first_pos - p.window + 1 : 0;  // the first token past the sinks that a row sees
-      const float inv_k = 1.f / pp.ref[x.it.b * c.heads + x.h].k, inv_v = 1.f / pp.ref[x.it.b * c.heads + x.h].v;
+      const PromptRef ref = pp.ref[x.it.b * c.heads + x.h];
+      const float inv_k = ref.by_block ? 0.f : 1.f / ref.k, inv_v = ref.by_block ? 0.f : 1.f / ref.v;  // 0: codes as they are
       uint4 kx[2][KC], vx[2][KC];
       float kr = 0.f, vr = 0.f;
       // the id of the block that holds the warp's tokens of tile i, as the table has it; -1: not looked at
@@ -674,11 +729,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
         id = id_next;
         id_next = id_of(i + 2);
         if (use > 0 && !(ok = wait(k_empty + slot, use - 1))) break;
-        put(sm + L::k + slot * L::kTile, base, kx, pow2_of(kr) * inv_k);
+        put(sm + L::k + slot * L::kTile, base, kx, inv_k == 0.f ? 1.f : kr * inv_k);
         if (lane == 0) mbar_arrive(k_full + slot);
         if (j + 1 < n) load(i + 1, id, c.k, c.k_scale, kx, kr);
         if (use > 0 && !(ok = wait(v_empty + slot, use - 1))) break;
-        put(sm + L::v + slot * L::kTile, base, vx, vr * inv_v);
+        put(sm + L::v + slot * L::kTile, base, vx, inv_v == 0.f ? 1.f : vr * inv_v);
         if (lane == 0) mbar_arrive(v_full + slot);
         if (j + 1 < n) load(i + 1, id, c.v, c.v_scale, vx, vr);
       }

@@ -78,9 +78,9 @@ def kv_attend(q, k, v, k_scale, v_scale, block_table, kv_len, *, cu_q=None, wind
     rows that do not: 0 * NaN.  kv_append stores none.)  A row that sees nothing (kv_len smaller than
     its sequence's rows) gets 0 and -inf.  Rows behind the last sequence's are left as they were.
 
-    Scales need not be powers of two; those of values that are not cost prompts two more roundings to
-    fp16.  Beside its relative error a row's out may be off by 2^-30 of the largest value it sees (a
-    probability times a block's scale is held in fp16).
+    Scales need not be powers of two, nor near one another; prompts are slower where a sequence and head
+    has others than powers of two within 2^14 of its largest.  Beside its relative error a row's out may
+    be off by 2^-30 of the largest value it sees (a probability times a block's scale is held in fp16).
 
     weights [n_blocks, kv_heads, block] fp32: each seen token's entry grows by its attention weights,
     summed over the call's rows and the query heads of its KV head.  `out` must not overlap q."""

@@ -1,11 +1,13 @@
 """Calls of the 8-bit paged KV cache at the edge of what its documentation allows, each of which once gave a
 wrong result or went unreported: against float64 (kv_ref) with test_gpu_kv_cache.py's bars."""
 
+import math
+
 import pytest
 import torch
 
 import kv_ref
-from test_gpu_kv_cache import TYPES, cache_args, check_attend, make
+from test_gpu_kv_cache import cache_args, check_attend, make
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +40,78 @@ def test_offsets_that_fall_do_nothing(cuda, rows, cu, track):
     base = weights.clone() if track else None
     kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], weights=weights, out=out, lse=lse)
     check_attend(s, [rows, 0, 0, 0], lens, 0, 0, out, lse, weights, base)
+
+
+# ------------------------------------------------------------------ block scales far apart
+def spread_scales(s, names, cuts, P, lens, before, after):
+    """Blocks that begin at token `cut` of their sequence or later get their scales times `after`, the others times
+    `before`; both may be no powers of two."""
+    for b, (n, cut) in enumerate(zip(lens, cuts)):
+        for col in range(-(-n // P)):
+            for name in names:
+                s[name + "_scale"][int(s["table"][b, col])] *= after if col * P >= cut else before
+
+
+def check_rows(s, rows, lens, fmt, window, sinks, out, lse, scale):
+    """check_attend with one more term, by what each row sees: a probability times its block's scale over the largest
+    scale seen is held in fp16, whose half step is 2^-25 below its normal numbers, and a row's sum of probabilities is
+    at least 2^7 (its reference's own), so each token adds up to 2^-32 of top times that scale."""
+    ro, rl, mean, bulk, _ = kv_ref.attend(s["q"], s["k"], s["v"], s["k_scale"], s["v_scale"], s["table"], lens, rows, window,
+                                          sinks, scale)
+    P, first = s["k"].shape[2], 0
+    step = torch.zeros_like(rl)
+    for b, (n, t) in enumerate(zip(lens, rows)):
+        p = torch.arange(n - t, n, device=out.device)[:, None]
+        j = torch.arange(n, device=out.device)
+        seen = (j <= p) & ((j > p - window) | (j < sinks) if window else True)
+        blocks = s["table"][b, : -(-n // P)].long()
+        blocks = torch.where(torch.nn.functional.pad(seen, (0, -n % P)).view(t, -1, P).any(0).any(-1), blocks, 0)
+        for h in range(s["k"].shape[1]):
+            top = (seen * s["v_scale"][blocks, h].double().repeat_interleave(P)[:n]).amax(1) * kv_ref.TOP[fmt]
+            G = out.shape[1] // s["k"].shape[1]
+            step[first: first + t, h * G: h * G + G] = (2.0 ** -32 * top * seen.sum(1))[:, None]
+        first += t
+    dp = 2.0 ** -19 * bulk + 2.0 ** -21 * (1 + bulk)
+    tol = (2.0 ** -11 + 2 * dp + 2.0 ** -19)[..., None] * mean + torch.finfo(out.dtype).eps / 2 * ro.abs() + step[..., None] + 2.0 ** -24
+    err = (out.double() - ro).abs()
+    assert bool((err <= tol).all()), f"out: {float((err / tol).max())} of the bar"
+    le = (lse.double() - rl).abs()
+    assert bool((le <= dp + 2.0 ** -21 * (1 + rl.abs())).all()), f"lse: {float((le / dp).max())}"
+
+
+FAR = [
+    # rows, lens, cuts, Hq, H, D, P, fmt, window, sinks
+    ([2100], [2100], [300], 8, 2, 128, 64, "e4m3", 0, 0),        # the first rows see the first blocks alone
+    ([2100], [2100], [304], 8, 2, 64, 16, "int8", 0, 0),         # ... the border inside a row tile and a tile of tokens
+    ([1500, 900], [3001, 900], [1664, 800], 8, 2, 128, 32, "e4m3", 0, 0),
+    ([1500], [3001], [1792], 8, 2, 128, 128, "int8", 200, 0),    # windows on both sides of the border
+    ([1500], [3001], [1664], 8, 2, 64, 64, "e4m3", 200, 20),
+]
+SPREADS = {"small first": (2.0 ** -30, 1.0), "small last": (1.0, 2.0 ** -30), "by 1.4, small first": (1.4 * 2.0 ** -22, 1.1)}
+
+
+@pytest.mark.parametrize("spread", SPREADS)
+@pytest.mark.parametrize("names", ["k", "v", "kv"])
+@pytest.mark.parametrize("case", FAR, ids=lambda c: f"{c[3]}x{c[4]}x{c[5]}-p{c[6]}-{c[7]}-w{c[8]}-{max(c[0])}of{max(c[1])}")
+def test_prompt_rows_that_see_small_blocks(cuda, case, names, spread):
+    """A row's result hangs on what it sees: blocks 2^30 below the sequence's largest keep their bits for the
+    rows that see no larger ones, keys and values."""
+    from duplex.streaming import kv_cache
+    rows, lens, cuts, Hq, H, D, P, fmt, window, sinks = case
+    before, after = SPREADS[spread]
+    s = make(cuda, len(rows), rows, lens, Hq, H, D, P, fmt, torch.bfloat16, seed=21)
+    spread_scales(s, names, cuts, P, lens, before, after)
+    scale, low = 1 / math.sqrt(D), min(before, after)
+    if "k" in names:                           # scores of the usual size for every row, by the largest block that it sees
+        scale, at = scale / low, 0
+        for t, n, cut in zip(rows, lens, cuts):
+            edge = -(-cut // P) * P
+            for p in range(n - t, n):
+                large = p >= edge if before < after else not window or p - window + 1 < edge or sinks > 0
+                s["q"][at] *= low / max(before, after) if large else 1.0
+                at += 1
+    if "v" in names:
+        s["v_scale"] /= low                    # the small ones are of the usual size, the large ones 2^30 of it
+    out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, sinks=sinks, softmax_scale=scale,
+                                  return_lse=True)
+    check_rows(s, rows, lens, fmt, window, sinks, out, lse, scale)
