@@ -23,6 +23,7 @@
 // kv_combine_kernel joins in order: no atomics, the same bits on each run.  Few row tiles are given a
 // cluster of 8 CTAs each instead, joined in the same launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attend.cuh"
 
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       }
     }
     float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126);
-    float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim
+    float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim, 15 + d
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
@@ -346,10 +347,25 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         for (int j = 0; j < 4; ++j) O[nt][i][j] = 0.f;
     }
 
-    auto step = [&](const uint8_t* st, int tok) {
+    // O is in units of the largest value scale so far, vref.  Where the tile's rows are of several tokens, one may not see
+    // the block that has it.  If its own largest is far below, by 2^d, the row's probabilities are held 2^d larger (m
+    // lower by d; l and O with it), so that what fp16 holds, p times scale / vref, is as large as if the row were
+    // alone.  That costs a tenth of the time: the steps take it (APART) from the first one on that not all rows see and
+    // whose scale is more than 4 times those before, which all rows have seen, or, without a window, more than 4 times
+    // its other 16 tokens' (who sees the second 16 sees the first).  False: this is that step.
+    const bool several = first_pos != last_pos;
+    auto step = [&](auto apart, const uint8_t* st, int tok) -> bool {
+      constexpr bool APART = decltype(apart)::value;
       const float4 sc = *reinterpret_cast<const float4*>(st + 64 * D);
       const float ks[2] = {sc.x, sc.z}, vs[2] = {sc.y, sc.w};
-      if (fmaxf(vs[0], vs[1]) < 0.f) return;
+      if (fmaxf(vs[0], vs[1]) < 0.f) return true;
+      // rows past the last have zeros for a query and are not written: they need no mask
+      const bool plain = tok + 31 <= first_pos && (!p.window || tok > last_pos - p.window || tok + 31 < p.sinks) &&
+                         fminf(vs[0], vs[1]) >= 0.f;
+      if (!APART && several && !plain) {
+        const float low = p.window ? 0.f : fminf(vs[0] < 0.f ? vs[1] : vs[0], vs[1] < 0.f ? vs[0] : vs[1]);
+        if (fmaxf(vs[0], vs[1]) > 4.f * fmaxf(vref, low)) return false;
+      }
       float S[2][NT][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -363,10 +379,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         for (int nt = 0; nt < NT; ++nt) S[x][nt][0] = S[x][nt][1] = S[x][nt][2] = S[x][nt][3] = 0.f;
         qk<D, FMT, NT>(kr, qf, S[x]);
       }
-      // rows past the last have zeros for a query and are not written: they need no mask
-      const bool plain = tok + 31 <= first_pos && (!p.window || tok > last_pos - p.window || tok + 31 < p.sinks) &&
-                         fminf(vs[0], vs[1]) >= 0.f;
-      bool grow = false;
+      bool grow = APART;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -386,7 +399,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         }
       const float vmax = fmaxf(vs[0], vs[1]);
       if (__any_sync(~0u, grow || vmax > vref)) {
-        const float vf = vmax > vref ? vref / vmax : 1.f;
+        const float vold = vref, vf = vmax > vref ? vref / vmax : 1.f;
         if (vmax > vref) vref = vmax;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -397,12 +410,25 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
             y = fmaxf(y, __shfl_xor_sync(~0u, y, 4));
             y = fmaxf(y, __shfl_xor_sync(~0u, y, 8));
             y = fmaxf(y, __shfl_xor_sync(~0u, y, 16));
-            const float top = fmaxf(m[nt][j], y - ad[nt][j]);
+            float d0 = 0.f, d = 0.f;
+            if constexpr (APART) {
+              float v = fmaxf(fmaxf(S[0][nt][j], S[0][nt][j + 2]) > -INFINITY ? vs[0] : 0.f,
+                              fmaxf(S[1][nt][j], S[1][nt][j + 2]) > -INFINITY ? vs[1] : 0.f);
+              v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
+              v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
+              v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
+              if (lim[nt][j] != -INFINITY) {  // the row has seen something before
+                d0 = lim[nt][j] - (kShift + kSlack);
+                v = fmaxf(v, vold * ex2(-d0));
+              }
+              if (v > 0.f && vref > v) d = (float)min((int)(__float_as_uint(vref / v) >> 23) - 127, 80);  // (l has room)
+            }
+            const float top = fmaxf(m[nt][j] + d0, y - ad[nt][j]) - d;
             a[j] = top == m[nt][j] ? 1.f : ex2(m[nt][j] - top);
             m[nt][j] = top;
             const float to = kShift - (top == -INFINITY ? 0.f : top), by = to - ad[nt][j];
             ad[nt][j] = to;
-            lim[nt][j] = top == -INFINITY ? -INFINITY : kShift + kSlack;
+            lim[nt][j] = top == -INFINITY ? -INFINITY : kShift + kSlack + d;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               S[x][nt][j] += by;
@@ -476,15 +502,25 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           }
         }
       }
+      return true;
     };
 
-#pragma unroll 1
-    for (int i = i0; i < i1; ++i) {
+    auto arrive = [&](int i) {
       cp_async_wait<ST - 2>();
       __syncwarp();  // everyone's copies of step i are there, and step i - 1's slot is read
       issue(i + ST - 1, id);
       id = ids_of(i + ST);
-      step(ring + (i % ST) * kStage, base_of(i));
+    };
+    int i = i0;
+#pragma unroll 1
+    for (; i < i1; ++i) {
+      arrive(i);
+      if (!step(std::false_type{}, ring + (i % ST) * kStage, base_of(i))) break;
+    }
+#pragma unroll 1
+    while (i < i1) {
+      step(std::true_type{}, ring + (i % ST) * kStage, base_of(i));
+      if (++i < i1) arrive(i);
     }
     cp_async_wait<0>();
     __syncthreads();  // the ring becomes the place where the warps meet

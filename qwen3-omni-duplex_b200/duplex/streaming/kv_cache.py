@@ -80,7 +80,7 @@ def kv_attend(q, k, v, k_scale, v_scale, block_table, kv_len, *, cu_q=None, wind
 
     Scales need not be powers of two, nor near one another; prompts are slower where a sequence and head
     has others than powers of two within 2^14 of its largest.  Beside its relative error a row's out may
-    be off by 2^-30 of the largest value it sees (a probability times a block's scale is held in fp16).
+    be off by 2^-28 of the largest value it sees (a probability times a block's scale is held in fp16).
 
     weights [n_blocks, kv_heads, block] fp32: each seen token's entry grows by its attention weights,
     summed over the call's rows and the query heads of its KV head.  `out` must not overlap q."""

@@ -115,3 +115,25 @@ def test_prompt_rows_that_see_small_blocks(cuda, case, names, spread):
     out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, sinks=sinks, softmax_scale=scale,
                                   return_lse=True)
     check_rows(s, rows, lens, fmt, window, sinks, out, lse, scale)
+
+
+@pytest.mark.parametrize("apart", [2.0 ** 34, 1.7 * 2.0 ** 40])
+@pytest.mark.parametrize("case", [
+    # rows, lens, cuts, Hq, H, D, P, fmt, window, sinks, whether the large values come first
+    ([2], [17], [16], 4, 2, 64, 16, "e4m3", 0, 0, False),              # row 0 does not see the last block
+    ([5, 3], [1010, 34], [1008, 32], 4, 1, 128, 16, "int8", 0, 0, False),
+    ([5], [1010], [1008], 16, 4, 128, 16, "e4m3", 3, 0, False),
+    ([3], [194], [192], 4, 1, 128, 64, "e4m3", 0, 0, False),
+    ([6], [2230], [128], 4, 1, 64, 64, "e4m3", 2100, 0, True),         # rows 3 and on do not see the first two blocks
+    ([6], [2230], [128], 8, 1, 128, 128, "int8", 2101, 0, True),
+    ([5] * 40, [1010] * 40, [1008] * 40, 4, 1, 128, 16, "e4m3", 0, 0, False),     # pieces of row tiles
+    ([3], [194], [192], 4, 1, 64, 16, "e4m3", 100, 5, False),
+], ids=lambda c: f"{c[3]}x{c[4]}x{c[5]}-p{c[6]}-{c[7]}-w{c[8]}-{max(c[0])}of{max(c[1])}")
+def test_few_rows_that_see_small_values(cuda, case, apart):
+    """Rows of one tile beside a row that sees a block with values 2^34 times as large: they do not see it."""
+    from duplex.streaming import kv_cache
+    rows, lens, cuts, Hq, H, D, P, fmt, window, sinks, first = case
+    s = make(cuda, len(rows), rows, lens, Hq, H, D, P, fmt, torch.bfloat16, seed=22)
+    spread_scales(s, "v", cuts, P, lens, apart if first else 1.0, 1.0 if first else apart)
+    out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, sinks=sinks, return_lse=True)
+    check_rows(s, rows, lens, fmt, window, sinks, out, lse, 1 / math.sqrt(D))
