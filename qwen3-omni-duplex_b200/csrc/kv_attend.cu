@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         pos[nt][j] = r2 < row_all ? s.n - s.rows + r2 / p.group : -1;
       }
     }
-    float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126);
+    float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126), rv = pow2f(126);  // rv = 1 / vref
     float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim, 15 + d
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -400,7 +400,10 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       const float vmax = fmaxf(vs[0], vs[1]);
       if (__any_sync(~0u, grow || vmax > vref)) {
         const float vold = vref, vf = vmax > vref ? vref / vmax : 1.f;
-        if (vmax > vref) vref = vmax;
+        if (vmax > vref) {
+          vref = vmax;
+          rv = 1.f / vmax;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float a[2];
@@ -425,15 +428,20 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
             }
             const float top = fmaxf(m[nt][j] + d0, y - ad[nt][j]) - d;
             a[j] = top == m[nt][j] ? 1.f : ex2(m[nt][j] - top);
+            // by what the step's x move: the largest to kShift + d, whatever the rounding of a large reference
+            const float by = y - ad[nt][j] > m[nt][j] + d0 ? kShift + d - y : d - d0;
             m[nt][j] = top;
-            const float to = kShift - (top == -INFINITY ? 0.f : top), by = to - ad[nt][j];
-            ad[nt][j] = to;
-            lim[nt][j] = top == -INFINITY ? -INFINITY : kShift + kSlack + d;
+            ad[nt][j] = kShift - (top == -INFINITY ? 0.f : top);
+            const float most = top == -INFINITY ? -INFINITY : kShift + kSlack + d;
+            lim[nt][j] = most;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              S[x][nt][j] += by;
-              S[x][nt][j + 2] += by;
-            }
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float& z = S[x][nt][j + 2 * i];
+                z += by;
+                z = z > most ? most : z;  // (that rounding again; a NaN stays)
+              }
             l[nt][j] *= a[j];
             a[j] *= vf;
           }
@@ -446,8 +454,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           }
         }
       }
-      const bool same = vs[0] == vref && vs[1] == vref;
-      const float vf[2] = {same ? 1.f : vs[0] / vref, same ? 1.f : vs[1] / vref};
+      const float vf[2] = {vs[0] * rv, vs[1] * rv};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         uint32_t pb[NT][2];
@@ -458,7 +465,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           for (int j = 0; j < 4; ++j) {
             y[j] = ex2(S[x][nt][j]);
             l[nt][j & 1] += y[j];
-            if (!same) y[j] *= vf[x];
+            y[j] *= vf[x];
           }
           pb[nt][0] = movmatrix_trans(f2h(y[0], y[1]));
           pb[nt][1] = movmatrix_trans(f2h(y[2], y[3]));
@@ -717,7 +724,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
   __shared__ uint2 sq[2][kRowChunk / 8][D / 16][32];
   __shared__ float s_sc[2][kRowChunk];
   __shared__ float2 s_st[2][kRowChunk];
-  __shared__ int s_pos[2][kRowChunk], s_fall[kWarps];
+  __shared__ int s_pos[2][kRowChunk], s_huge[2][kWarps], s_fall[kWarps];
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
@@ -783,6 +790,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
     const float undo = make_q<D>(p, raw, qf);
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) sq[buf][r >> 3][e][(r & 7) * 4 + t] = qf[e];
+    s_huge[buf][warp] = __any_sync(~0u, fabsf(st.x) > kHuge);
     if (t == 0) {
       s_sc[buf][r] = undo * p.scale_log2;
       s_st[buf][r] = st;
@@ -800,7 +808,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
     if (more) load(r0 + kRowChunk);
     // all rows of the chunk see all tokens of the tile
     const int first = start + p.by_group(r0), last = start + p.by_group(min(r0 + kRowChunk, r1) - 1);
-    const bool plain = tile_end - 1 <= first && (!p.window || tile > last - p.window || tile_end <= p.sinks);
+    const bool plain = tile_end - 1 <= first && (!p.window || tile > last - p.window || tile_end <= p.sinks) &&
+                       !(s_huge[buf][0] | s_huge[buf][1] | s_huge[buf][2] | s_huge[buf][3]);
     float part[kWU][2];  // a chunk's sum by itself: thousands of rows added one by one would lose bits
 #pragma unroll
     for (int x = 0; x < kWU; ++x) part[x][0] = part[x][1] = 0.f;
@@ -829,8 +838,10 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int k = tile + x * kWUnit + 16 * warp + g + 8 * (j >> 1), q = pos[j & 1];
-            if (k <= q && (!p.window || k > q - p.window || k < p.sinks)) 
-              part[x][j >> 1] = fmaf(ex2(fmaf(S[x][j], f[j & 1], st2[j & 1].x)), st2[j & 1].y, part[x][j >> 1]);
+            if (k <= q && (!p.window || k > q - p.window || k < p.sinks)) {
+              const float w = ex2(fmaf(S[x][j], f[j & 1], st2[j & 1].x)) * st2[j & 1].y;
+              part[x][j >> 1] += w > 1.f ? 1.f : w;  // (kHuge: the attention's s may be some steps away; a NaN stays)
+            }
           }
         }
       }

@@ -11,6 +11,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 // p = exp2(s - m + kShift) is what fp16 holds: the reference m may be 2^kSlack behind the true
 // maximum (so it rarely moves), p stays below 2^15, and a p of 2^-21 of the reference is still normal.
 constexpr float kShift = 7.f, kSlack = 8.f;
+// A reference beyond this has steps that count: s - m is then taken of the rounded s, so that the largest is 0.
+constexpr float kHuge = 1048576.f;
 
 struct AttendParams {
   KvView c;

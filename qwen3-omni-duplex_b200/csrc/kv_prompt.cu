@@ -427,25 +427,28 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       const int t_last = s.n - s.rows + p.by_group(row_hi - 1);
       const bool mine = mt == 0 || x.two;
       const float cs = fmaxf(s_undo[tid] * fabsf(p.scale_log2) * ref.k, 1.2e-38f);  // not 0: hidden scores are -inf
-      float m = -INFINITY, l = 0.f, vref = ref.v;  // O is in units of vref
-      auto tiles = [&](auto by) {
-        constexpr bool BY = decltype(by)::value;  // factors by block, of scores and probabilities
-        if (BY) vref = pow2f(-126);
-        for (int j = 0; mine && j < n; ++j) {
+      float m = -INFINITY, l = 0.f, vref = ref.by_block ? pow2f(-126) : ref.v;  // O is in units of vref
+      // Tiles from j on; BY block, with factors of scores and probabilities, and s - m of the rounded s.  The others end
+      // at the first tile with scores beyond kHuge, and return it.
+      auto tiles = [&](auto by, int j) {
+        constexpr bool BY = decltype(by)::value;
+        for (; mine && j < n; ++j) {
           const int base = x.base_of(x.i0 + j);
           // (rows past the last have zeros for a query and are not written: they need no mask)
           const bool masked = BY || base + kPTok - 1 > t_first ||
                               (p.window && base <= t_last - p.window && base + kPTok > p.sinks);
           // lane i (of 8): the scales of the block that holds tokens base + 16 i .. + 15; -1: an id out of range
-          float kf = -1.f, vs = 0.f;
-          if (BY) {
+          float kf = 1.f, vs = vref;
+          if (BY && ref.by_block) {
             const int k = base + 16 * (lane & 7), id = k < x.it.sp.end ? c.table[(int64_t)x.it.b * c.width + k / c.block] : -1;
+            kf = -1.f;
+            vs = 0.f;
             if ((unsigned)id < (unsigned)c.n_blocks) {
               kf = __ldg(c.k_scale + (int64_t)id * c.heads + x.h) / ref.k;
               vs = __ldg(c.v_scale + (int64_t)id * c.heads + x.h);
             }
           }
-          if (!(ok = wait(s_full + mt, n_s + j))) return;
+          if (!(ok = wait(s_full + mt, n_s + j))) return n;
           tc_fence_after();
           // The loops are short on purpose: unrolled over the row they outgrow the instruction caches, and
           // the tile takes 1.8 times as long.
@@ -503,6 +506,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
           if (__any_sync(~0u, mx > m + kSlack || (BY && vf != 1.f))) {
             const float top = mx > m + kSlack ? mx : m;
             float f = top == m ? 1.f : ex2(m - top);
+            if (!BY && __any_sync(~0u, fabsf(top) > kHuge && top != -INFINITY)) return j;
             m = top;
             l *= f;
             if (BY) f *= vf;
@@ -521,8 +525,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
           const float add = kShift - (m == -INFINITY ? 0.f : m);
           const float2 cs2 = make_float2(cs, cs), add2 = make_float2(add, add);
           float2 ls = make_float2(0.f, 0.f);
-          if constexpr (BY) {  // the probabilities' sum without, the operand with the value's scale
-            const float rv = 1.f / vref;
+          if constexpr (BY) {  // the probabilities' sum without, the operand with the value's scale; s - m of the rounded s
+            const float rv = 1.f / vref, ref_m = m == -INFINITY ? 0.f : m;
             __syncwarp();
 #pragma unroll 1
             for (int q = 0; q < kPTok / 16; ++q) {
@@ -533,8 +537,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
               tc_wait_ld();
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                const float2 y = fma2(make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])), cs2, add2);
-                const float2 z = make_float2(ex2(y.x), ex2(y.y));
+                auto p_of = [&](uint32_t s) { return ex2(__fsub_rn(__fmul_rn(__uint_as_float(s), cs), ref_m) + kShift); };
+                const float2 z = make_float2(p_of(w[e]), p_of(w[e + 1]));
                 ls = add2f(ls, z);
                 P[e / 2] = f2h(z.x * f, z.y * f);
               }
@@ -583,9 +587,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
           __syncwarp();
           if (lane == 0) mbar_arrive(p_ready + mt);
         }
+        return n;
       };
-      if (__builtin_expect(!ref.by_block, 1)) tiles(std::false_type{});
-      else tiles(std::true_type{});
+      const int rest = ref.by_block ? 0 : tiles(std::false_type{}, 0);
+      if (rest < n) tiles(std::true_type{}, rest);
       // ---- the row's result.  Once all products are done (both tiles wait for them) the next piece's rows
       // take the query rows' place, so its first scores are computed under the writing of this one's results.
       if (!ok) break;

@@ -137,3 +137,55 @@ def test_few_rows_that_see_small_values(cuda, case, apart):
     spread_scales(s, "v", cuts, P, lens, apart if first else 1.0, 1.0 if first else apart)
     out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, sinks=sinks, return_lse=True)
     check_rows(s, rows, lens, fmt, window, sinks, out, lse, 1 / math.sqrt(D))
+
+
+# ------------------------------------------------------------------ very large scores
+def scores(s, b, h, n, t, first, window, scale):
+    """[t, group, n] float64 of one sequence and KV head, -inf where a row does not see."""
+    P, G = s["k"].shape[2], s["q"].shape[1] // s["k"].shape[1]
+    p = torch.arange(n - t, n, device=s["q"].device)[:, None]
+    j = torch.arange(n, device=s["q"].device)
+    seen = (j <= p) & (j > p - window if window else True)
+    blocks = s["table"][b, : -(-n // P)].long()
+    blocks = torch.where(torch.nn.functional.pad(seen, (0, -n % P)).view(t, -1, P).any(0).any(-1), blocks, 0)
+    k = kv_ref.values(s["k"], s["k_scale"], blocks, h, n).nan_to_num(0, 0, 0)
+    x = torch.einsum("tgd,nd->tgn", s["q"][first: first + t, h * G: h * G + G].double(), k) * scale
+    return x.masked_fill(~seen[:, None], -math.inf)
+
+
+@pytest.mark.parametrize("by", [2.0 ** 22, 2.0 ** 27, -2.0 ** 30, 2.0 ** 45])
+@pytest.mark.parametrize("rows,lens,window,odd", [([1, 3], [700, 90], 0, 1.0), ([2, 5], [9000, 40], 100, 1.0),
+                                                  ([1500, 900], [2900, 900], 0, 1.0), ([1500, 900], [2900, 900], 200, 1.3)])
+def test_large_scores(cuda, rows, lens, window, odd, by):
+    """Scores of 1e7 to 1e14, whose fp32 steps are far above 1: where one stands out by more than the bars of a score, the
+    row is its value alone; elsewhere the result is some mean of values.  The weights' pass computes a score anew, off from
+    the attention's by up to 2 ds, where ds is 2^-19 bulk > 8 here: exp(2 ds) leaves of a weight only that it is a number
+    from 0 to 1 for each row and head."""
+    from duplex.streaming import kv_cache
+    s = make(cuda, 2, rows, lens, 8, 2, 128, 32, "e4m3", torch.bfloat16, seed=31)
+    s["k_scale"] *= odd
+    weights = torch.zeros(s["k"].shape[:3], device=cuda)
+    out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, softmax_scale=by, weights=weights,
+                                  return_lse=True)
+    ro, rl, mean, bulk, _ = kv_ref.attend(s["q"], s["k"], s["v"], s["k_scale"], s["v_scale"], s["table"], lens, rows, window,
+                                          0, by)
+    ds = 2.0 ** -19 * bulk + 2.0 ** -21 * (1 + bulk)
+    assert bool(((lse.double() - rl).abs() <= ds + 2.0 ** -21 * (1 + rl.abs())).all())
+    gap, first = torch.zeros_like(rl), 0
+    for b, (n, t) in enumerate(zip(lens, rows)):
+        for h in range(2):
+            top = torch.topk(scores(s, b, h, n, t, first, window, by), 2, -1).values
+            gap[first: first + t, 4 * h: 4 * h + 4] = top[..., 0] - top[..., 1]
+        first += t
+    alone = gap > 2 * ds + 40
+    assert float(alone.double().mean()) > 0.5
+    tol = (2.0 ** -10 * mean + 2.0 ** -8 * ro.abs() + 2.0 ** -24)
+    assert bool(((out.double() - ro).abs() <= tol)[alone].all())
+    vmax = float(s["v_scale"].max()) * 448
+    assert bool((out.abs() <= vmax * 1.01).all())
+    assert float(ds.median()) > 8
+    assert bool(((weights >= 0) & (weights <= 4 * sum(rows) * (1 + 2.0 ** -19))).all())
+    # as for NaN: it stays in its row
+    s["q"][0, 0, 0] = float("nan")
+    got = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, softmax_scale=by)
+    assert bool(torch.isnan(got[0, 0]).all()) and int(torch.isnan(got).any(-1).sum()) == 1
