@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 5 : R == 2 ? 3 : 1) kv_gath
     for (int i = 0; i < R; ++i) {
       const int e = tid + i * kThreads;
       if (e / per >= count) continue;
-      const float f = sc[y][i] * inv;
+      const float f = fminf(sc[y][i] * inv, 3e38f);  // (of a zero token beside much smaller ones: 0 times it must be 0)
       uint4 q;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {

@@ -189,3 +189,43 @@ def test_large_scores(cuda, rows, lens, window, odd, by):
     s["q"][0, 0, 0] = float("nan")
     got = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, softmax_scale=by)
     assert bool(torch.isnan(got[0, 0]).all()) and int(torch.isnan(got).any(-1).sum()) == 1
+
+
+# ------------------------------------------------------------------ eviction of zeros
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("small", [False, True])
+@pytest.mark.parametrize("keep", [16, 17, 37])
+def test_evict_zero_tokens(cuda, keep, small, fmt):
+    """Zero tokens out of blocks with a large scale: zeros at the smallest scale, in a full block and in a tail of one;
+    and beside a small token of another block, which sets the scale."""
+    from duplex.streaming import kv_cache
+    H, D, P, n = 2, 64, 16, 80
+    s = make(cuda, 1, [1], [n], H, H, D, P, fmt, torch.float16, spare=4, seed=3)
+    w = torch.zeros(s["k"].shape[:3], device=cuda)
+    zero = torch.zeros(H, P, D, device=cuda)
+    for col in range(5):
+        blk = int(s["table"][0, col])
+        for name in "kv":
+            code = zero.clone()
+            code[:, 5] = 100.0                                   # one large token a block, which is not kept
+            if small and col == 1:
+                code[:, 7, 3] = 1.0
+            s[name][blk] = code.to(s[name].dtype)
+            s[name + "_scale"][blk] = 2.0 ** (-100 if small and col == 1 else 100 if small else 3)
+        w[blk] = 1.0
+        w[blk, :, 5] = 0.0
+    dst = s["free"][:3].view(1, 3).contiguous()
+    before = {m: s[m].clone() for m in ("k", "v", "k_scale", "v_scale")}
+    kv_cache.kv_evict(*cache_args(s), w, dst, keep=keep)
+    at = [j for j in range(n) if j % P != 5][:keep]
+    for h in range(H):
+        for name in "kv":
+            x = kv_ref.values(before[name], before[name + "_scale"], s["table"][0].long(), h, n).cpu()[torch.tensor(at)]
+            for i in range(-(-keep // P)):
+                part, blk = x[i * P: i * P + P], int(dst[0, i])
+                two = kv_ref.scale_of(part, fmt)
+                got = s[name][blk, h, : len(part)].double().cpu()
+                assert torch.equal(got, kv_ref.rounded(part / two, fmt)), (name, i)
+                assert float(s[name + "_scale"][blk, h]) == two
+    out = kv_cache.kv_attend(s["q"][:1], *cache_args(s)[:4], dst, torch.tensor([keep], dtype=torch.int32, device=cuda))
+    assert bool(torch.isfinite(out).all())
