@@ -562,7 +562,7 @@ int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_batch* batch,
  * NaN counts as the largest), in their order.  They are written to the blocks of dst_table
  * [batch][dst_width] (dst_width * block >= keep), with their weights and with scales of their
  * own; a sequence of no more than keep tokens is copied whole.  new_len [batch] = min(kv_len,
- * keep).  The source blocks are left as they are, so they may be shared between sequences; no
+ * keep), which may be written over kv_len.  The source blocks are left as they are, so they may be shared between sequences; no
  * destination block may be a source block of the call or appear twice.  keep >= sinks + recent.
  * cu_rows and n_rows are not used.
  */

@@ -193,7 +193,6 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
   const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
   const int n = kv_seq(c, b).n;
-  if (h == 0 && tid == 0) p.new_len[b] = min(n, p.keep);
   int32_t* out = p.index + ((int64_t)b * c.heads + h) * p.keep;
   int32_t* ids = reinterpret_cast<int32_t*>(keys + (int64_t)c.width * c.block);  // the sequence's block ids (SM_KEYS)
   const int shift_p = __ffs(c.block) - 1;
@@ -326,6 +325,9 @@ __global__ void __launch_bounds__(kThreads, R == 1 ? 5 : R == 2 ? 3 : 1) kv_gath
     const int tok = (tid + i * kThreads) / per;
     src[i] = tok < min(P, p.keep - base) ? index[tok] : -1;
   }
+  // here, where the selection has read all lengths, and since min(n, keep) is the same before and after: new_len may
+  // be kv_len
+  if (base == 0 && h == 0 && tid == 0) p.new_len[b] = min(kv_seq(c, b).n, p.keep);
   if (count <= 0) return;
   if ((unsigned)id >= (unsigned)c.n_blocks) {
     if (tid == 0) set_error(p.err, DUPLEX_DEVERR_BLOCK);

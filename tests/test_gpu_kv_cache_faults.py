@@ -1,6 +1,7 @@
 """Calls of the 8-bit paged KV cache at the edge of what its documentation allows, each of which once gave a
 wrong result or went unreported: against float64 (kv_ref) with test_gpu_kv_cache.py's bars."""
 
+import ctypes
 import math
 
 import pytest
@@ -229,3 +230,38 @@ def test_evict_zero_tokens(cuda, keep, small, fmt):
                 assert float(s[name + "_scale"][blk, h]) == two
     out = kv_cache.kv_attend(s["q"][:1], *cache_args(s)[:4], dst, torch.tensor([keep], dtype=torch.int32, device=cuda))
     assert bool(torch.isfinite(out).all())
+
+
+# ------------------------------------------------------------------ eviction that writes the lengths in place
+def test_evict_lengths_in_place(cuda):
+    """duplex_kv_evict with new_len = kv_len: every head reads the old length, however many there are."""
+    from duplex import _lib
+    from duplex.streaming import kv_cache
+    H, D, P, n, keep, B = 400, 64, 16, 48, 20, 2                # more selections than run at once
+    s = make(cuda, B, [1] * B, [n] * B, H, H, D, P, "int8", torch.float16, spare=2 * B, seed=4)
+    w = torch.rand(s["k"].shape[:3], device=cuda)
+    dst = s["free"][: 2 * B].view(B, 2).contiguous()
+    names = ("k", "v", "k_scale", "v_scale")
+    state = [s[m].clone() for m in names] + [w.clone()]
+    new = kv_cache.kv_evict(*cache_args(s), w, dst, keep=keep, sinks=1, recent=3)
+    want = [s[m].clone() for m in names] + [w.clone()]
+    for m, t in zip(names, state):
+        s[m].copy_(t)
+    w.copy_(state[-1])
+    lib = _lib.load()
+    cache = _lib.KVCache(k=s["k"].data_ptr(), v=s["v"].data_ptr(), k_scale=s["k_scale"].data_ptr(),
+                         v_scale=s["v_scale"].data_ptr(), weights=w.data_ptr(), n_blocks=s["k"].shape[0], kv_heads=H,
+                         block=P, dim=D, format=_lib.KV_INT8)
+    batch = _lib.KVBatch(block_table=s["table"].data_ptr(), kv_len=s["kv_len"].data_ptr(), cu_rows=None,
+                         width=s["table"].shape[1], batch=B, n_rows=0)
+    ws = torch.empty(B * H * keep * 4, dtype=torch.uint8, device=cuda)
+    torch.cuda.synchronize()
+    rc = lib.duplex_kv_evict(ctypes.byref(cache), ctypes.byref(batch), dst.data_ptr(), 2, keep, 1, 3, s["kv_len"].data_ptr(),
+                             ws.data_ptr(), ws.numel(), None, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert s["kv_len"].tolist() == new.tolist() == [keep] * B
+    for m, t in zip(names, want):
+        used = dst.flatten().long()
+        assert torch.equal(s[m][used], t[used]), m
+    assert torch.equal(w, want[-1])
