@@ -46,6 +46,7 @@ extern "C" {
                                      beyond +-2^26 and was clamped (its fixed-point sum) */
 #define DUPLEX_DEVERR_BLOCK 8     /* a KV cache's block id outside [0, n_blocks): its tokens were left out */
 #define DUPLEX_DEVERR_OFFSETS 16  /* a KV cache's row offsets fall: the call did nothing */
+#define DUPLEX_DEVERR_LENGTH 32   /* a KV cache's kv_len beyond its table: the tokens past it were left out */
 /* duplex_stack_forward also records, from this bit up, which of its waits gave up
  * first: 1 ring slot free, 2 routing plan, 3 ring slot filled, 4 grid barrier,
  * 5 drain, 6 cluster exchange. */
@@ -500,8 +501,9 @@ int duplex_moe_forward_noalloc(const void* x, int act_dtype, int32_t T, const vo
  * last token are not read), kv_len [batch] (its tokens, the call's own rows included: row t of
  * T is token kv_len - T + t), cu_rows [batch + 1] (its rows are [cu_rows[b], cu_rows[b+1]) of
  * n_rows; NULL: n_rows / batch each).  All are device memory, read by the kernels: a captured
- * call follows their values.  Rows behind the last sequence's are left alone; lengths and rows
- * are held inside width * block and n_rows; a block id out of range is reported in err
+ * call follows their values.  Rows behind the last sequence's are left alone; rows are held
+ * inside n_rows; where kv_len is beyond width * block, that is reported (DUPLEX_DEVERR_LENGTH) and
+ * tokens past the table are left out: not stored, not seen, not kept; a block id out of range is reported in err
  * (DUPLEX_DEVERR_BLOCK) and its tokens are left out; a call whose row offsets fall anywhere
  * (cu_rows[b + 1] < cu_rows[b]) reports that (DUPLEX_DEVERR_OFFSETS) and does nothing.  batch <= DUPLEX_KV_MAX_BATCH,
  * batch * kv_heads <= 65535.

@@ -25,12 +25,16 @@ struct KvView {
   const int32_t* kv_len; // [batch]
   const int32_t* cu;     // [batch + 1] row offsets, or null: rows split evenly
   int width, batch, n_rows;
+  int cap;               // tokens that a row of the table holds
+  int len_max;           // what is made of a kv_len beyond: 2^29 past the table, which is past any window's reach
+                         // into it, so that sums of positions stay numbers
 };
 
-// rows [row0, row0 + rows) of sequence b and its number of cached tokens n, held inside the
-// buffers whatever the device arrays say.  (Each sequence by itself: see offsets_fall for all of them.)
+// rows [row0, row0 + rows) of sequence b, the first row's token, and the number of cached tokens n, held
+// inside the buffers whatever the device arrays say.  (Each sequence by itself: see offsets_fall for all
+// of them.)  kv_len counts more than the table holds: tokens from n on are not there (see too_long).
 struct KvSeq {
-  int row0, rows, n;
+  int row0, rows, n, first;
 };
 
 DEVI KvSeq kv_seq(const KvView& c, int b) {
@@ -45,11 +49,14 @@ DEVI KvSeq kv_seq(const KvView& c, int b) {
     r1 = s.row0 + t;
   }
   s.rows = r1 - s.row0;
-  const long long cap = (long long)c.width * c.block;
-  const int n = max(c.kv_len[b], 0);
-  s.n = n > cap ? (int)cap : n;
+  const int n = min(max(c.kv_len[b], 0), c.len_max);
+  s.n = min(n, c.cap);
+  s.first = n - s.rows;
   return s;
 }
+
+// whether sequence b, of this call, has more tokens than its table
+DEVI bool too_long(const KvView& c, const KvSeq& s) { return s.rows > 0 && s.first + s.rows > s.n; }
 
 // Whether this thread's share of the row offsets falls somewhere.  Where none does, no row is in two
 // sequences, and what is laid out by rows (the item list, the clusters' grid) has the host's bounds; a

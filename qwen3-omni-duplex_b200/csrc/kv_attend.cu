@@ -61,6 +61,7 @@ DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
   __shared__ int64_t warp_sum[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = p.c.batch;
   int64_t base = 0;
+  int bits = 0;
   for (int b0 = 0; b0 < B; b0 += kWarps * 32) {
     const int b = b0 + tid;
     int64_t u = 0;
@@ -68,6 +69,7 @@ DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
       const KvSeq s = kv_seq(p.c, b);
       u = (int64_t)p.c.heads * tiles_of(s, p.group, ROWS) * (ITEMS ? 1 : units_of(s, p, ROWS));
       if (offset_falls(p.c, b)) u = kFalls;
+      if (too_long(p.c, s)) bits = DUPLEX_DEVERR_LENGTH;
     }
     int64_t incl = u;
 #pragma unroll
@@ -91,8 +93,9 @@ DEVI Plan make_plan(const AttendParams& p, int64_t* off, int ctas) {
   __syncthreads();
   if (base < 0) {
     base = 0;  // no work
-    if (tid == 0) set_error(p.err, DUPLEX_DEVERR_OFFSETS);
+    bits = DUPLEX_DEVERR_OFFSETS;
   }
+  if (bits) set_error(p.err, bits);
   Plan pl;
   pl.total = base;
   pl.share = (base + ctas - 1) / ctas;
@@ -266,9 +269,9 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
     const int len = i1 - i0;
     const int h = it / rt_all, rt = it - h * rt_all;
     const int row_base = rt * ROWS, row_all = s.rows * p.group;
-    const int first_pos = s.n - s.rows + row_base / p.group;
+    const int first_pos = s.first + row_base / p.group;
     const int last_row = min(row_base + ROWS, row_all) - 1;
-    const int last_pos = s.n - s.rows + last_row / p.group;
+    const int last_pos = s.first + last_row / p.group;
     const Span sp = span_of<kUnit>(p, first_pos, last_pos, s.n);
     if (CL) {
       const int n = sp.sink_units + (sp.end > sp.lo ? (sp.end - sp.lo + kUnit - 1) / kUnit : 0);
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       const int tok = base_of(i), lim = i < i1 ? (i < sp.sink_units ? sp.sink_end : sp.end) : 0;
       auto id = [&](int k) {
         const bool gap = p.window && k + 15 <= first_pos - p.window && k >= p.sinks;  // between sinks and window
-        return k < lim && !gap ? kv_block_at(c, b, k >> psh, p.err) : -1;
+        return (unsigned)k < (unsigned)lim && !gap ? kv_block_at(c, b, k >> psh, p.err) : -1;
       };
       return make_int2(id(tok), id(tok + 16));
     };
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       for (int j = 0; j < 2; ++j) {
         csc[nt][j] = __shfl_sync(~0u, undo, (2 * t + j) * 4) * p.scale_log2;
         const int r2 = row_base + nt * 8 + 2 * t + j;
-        pos[nt][j] = r2 < row_all ? s.n - s.rows + r2 / p.group : -1;
+        pos[nt][j] = r2 < row_all ? s.first + r2 / p.group : -1;
       }
     }
     float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126), rv = pow2f(126);  // rv = 1 / vref
@@ -399,10 +402,12 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         }
       const float vmax = fmaxf(vs[0], vs[1]);
       if (__any_sync(~0u, grow || vmax > vref)) {
-        const float vold = vref, vf = vmax > vref ? vref / vmax : 1.f;
+        const float vold = vref;
+        float vf = 1.f;
         if (vmax > vref) {
-          vref = vmax;
           rv = 1.f / vmax;
+          vf = vref * rv;
+          vref = vmax;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -729,7 +734,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv_weights_kernel(AttendParams
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
   const KvSeq s = kv_seq(c, b);
-  const int tile = blockIdx.x * (kWU * kWUnit), tile_end = tile + kWU * kWUnit, start = s.n - s.rows;
+  const int tile = blockIdx.x * (kWU * kWUnit), tile_end = tile + kWU * kWUnit, start = s.first;
   // the sequence's rows that see a token of the tile
   const int t0 = max(tile - start, 0);
   int t1 = s.rows;

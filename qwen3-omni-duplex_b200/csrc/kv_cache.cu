@@ -9,6 +9,7 @@
 // rows): what counts is how many are on an SM, so the rounds are a template argument and registers bounded.
 // One B200: 13,000 new tokens of 4 sequences, 4 KV heads of 128: 14 us (2.3 TB/s; with 98 registers 35 us);
 // 12 sequences of 16,384 tokens to 8192: 78 us, 28 of them the selection.
+#include <algorithm>
 #include <type_traits>
 
 #include "kv.cuh"
@@ -66,14 +67,18 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
     left = min(step, lo + left - (lo + i * step));
     lo += i * step;
   }
+  bool fall = cu.y < cu.x;
   const int b = lo;
   const KvSeq s = kv_seq(c, b);
   if (s.rows == 0) return;
-  const int first = s.n - s.rows;  // slot of the sequence's first new token (< 0: no room for it)
+  const int first = s.first;  // slot of the sequence's first new token (< 0: no room for it)
   const int64_t item = w - (s.row0 / P + 2ll * b);
   if (item < 0) return;  // rows before the first sequence's
   const int64_t col = max(first, 0) / P + item;
-  if (col * P >= s.n) return;
+  if (col * P >= s.n) {  // no more tokens, or no more table (which some CTA's block is past if kv_len is)
+    if (tid == 0 && too_long(c, s)) set_error(p.err, DUPLEX_DEVERR_LENGTH);
+    return;
+  }
   const int id = kv_block_at(c, b, (int)col, tid == 0 ? p.err : nullptr);
   if (id < 0) return;
   const int base = (int)col * P;                  // slot of the block's first token
@@ -107,7 +112,6 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
       amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
   }
-  bool fall = cu.y < cu.x;
   for (int i = tid + kThreads; c.cu && i < c.batch; i += kThreads) fall |= offset_falls(c, i);
   amax = block_max(fall ? INFINITY : amax, red);  // (the values are finite)
   if (amax == INFINITY) return;
@@ -193,6 +197,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictParams p) {
   const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
   const int n = kv_seq(c, b).n;
+  if (h == 0 && tid == 0 && c.kv_len[b] > n) set_error(p.err, DUPLEX_DEVERR_LENGTH);
   int32_t* out = p.index + ((int64_t)b * c.heads + h) * p.keep;
   int32_t* ids = reinterpret_cast<int32_t*>(keys + (int64_t)c.width * c.block);  // the sequence's block ids (SM_KEYS)
   const int shift_p = __ffs(c.block) - 1;
@@ -408,9 +413,10 @@ int kv_check(const duplex_kv_cache* c, const duplex_kv_batch* b, KvView* out) {
   if ((int64_t)b->width * c->block + b->n_rows > 0x7FFFFFFFll - 256) return DUPLEX_ERR_UNSUPPORTED;
   if (!b->cu_rows && b->n_rows % b->batch) return DUPLEX_ERR_ARG;
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return DUPLEX_ERR_ALIGN;
+  const int cap = b->width * c->block;
   *out = KvView{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale, c->weights,
                 c->n_blocks, c->kv_heads, c->block, c->dim, c->format, b->block_table, b->kv_len, b->cu_rows,
-                b->width, b->batch, b->n_rows};
+                b->width, b->batch, b->n_rows, cap, (int)std::min((int64_t)cap + (1 << 29), (int64_t)INT32_MAX)};
   return DUPLEX_OK;
 }
 

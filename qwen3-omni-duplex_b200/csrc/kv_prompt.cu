@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
   if (blockIdx.x > 0) {
     const int b = (blockIdx.x - 1) / c.heads, h = (blockIdx.x - 1) - b * c.heads;
     const KvSeq s = kv_seq(c, b);
-    const int lo_x = p.window ? s.n - s.rows - p.window + 1 : 0, cols = s.rows ? (s.n + c.block - 1) / c.block : 0;
+    const int lo_x = p.window ? s.first - p.window + 1 : 0, cols = s.rows ? (s.n + c.block - 1) / c.block : 0;
     float mk = 0.f, mv = 0.f, lk = INFINITY, lv = INFINITY;  // largest and least (a scale of 0 is exact anywhere)
     int by_block = 0;
     for (int col = tid; col < cols; col += kPlanThreads) {
@@ -161,7 +161,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
   for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int t = 0;
-    if (b < B) t = (int)(((int64_t)kv_seq(c, b).rows * p.group + kPRows - 1) / kPRows);
+    if (b < B) {
+      const KvSeq s = kv_seq(c, b);
+      t = (int)(((int64_t)s.rows * p.group + kPRows - 1) / kPRows);
+      if (too_long(c, s)) set_error(p.err, DUPLEX_DEVERR_LENGTH);
+    }
     const int64_t at = scan(t, all);
     if (b < B) tiles[b] = (int)(base + at);
     base += all;
@@ -184,8 +188,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_prompt_plan_kernel(PromptPara
       it.b = lo;
       it.rt = i - tiles[lo];
       it.s = kv_seq(c, lo);
-      it.first_pos = it.s.n - it.s.rows + it.rt * kPRows / p.group;
-      it.last_pos = it.s.n - it.s.rows + (min(it.rt * kPRows + kPRows, it.s.rows * p.group) - 1) / p.group;
+      it.first_pos = it.s.first + it.rt * kPRows / p.group;
+      it.last_pos = it.s.first + (min(it.rt * kPRows + kPRows, it.s.rows * p.group) - 1) / p.group;
       it.sp = span_of<kPTok>(p, it.first_pos, it.last_pos, it.s.n);
       it.per = units_in(it.sp) + kPOver;
     }
@@ -420,11 +424,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const __grid_co
       const KvSeq s = x.it.s;
       const int rr = row_base + tid, t_row = p.by_group(rr);
       const bool live = rr < row_all;
-      const int pos = live ? s.n - s.rows + t_row : -1;
+      const int pos = live ? s.first + t_row : -1;
       const int wlo = p.window ? pos - p.window : -1;  // tokens k > wlo, or k < sinks
       const int row_lo = row_base + mt * 128, row_hi = min(row_lo + 128, row_all);
-      const int t_first = s.n - s.rows + p.by_group(min(row_lo, row_all - 1));  // positions of the tile's rows
-      const int t_last = s.n - s.rows + p.by_group(row_hi - 1);
+      const int t_first = s.first + p.by_group(min(row_lo, row_all - 1));  // positions of the tile's rows
+      const int t_last = s.first + p.by_group(row_hi - 1);
       const bool mine = mt == 0 || x.two;
       const float cs = fmaxf(s_undo[tid] * fabsf(p.scale_log2) * ref.k, 1.2e-38f);  // not 0: hidden scores are -inf
       float m = -INFINITY, l = 0.f, vref = ref.by_block ? pow2f(-126) : ref.v;  // O is in units of vref

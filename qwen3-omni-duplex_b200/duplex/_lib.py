@@ -18,7 +18,8 @@ _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("DUPLEX_B200_LIB", _PKG / "libduplex_b200.so"))
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
-DEVERR_EXPERT, DEVERR_TIMEOUT, DEVERR_NONFINITE, DEVERR_BLOCK, DEVERR_OFFSETS = 1, 2, 4, 8, 16
+DEVERR_EXPERT, DEVERR_TIMEOUT, DEVERR_NONFINITE, DEVERR_BLOCK = 1, 2, 4, 8
+DEVERR_OFFSETS, DEVERR_LENGTH = 16, 32
 KV_E4M3, KV_INT8 = 0, 1
 
 _c_int, _c_i32, _c_i64, _c_ptr, _c_size, _c_f32 = (ctypes.c_int, ctypes.c_int32, ctypes.c_int64,

@@ -321,7 +321,9 @@ class ClockStack:
 
     def step_into(self, x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         """Enqueue one decode step for x [T, H] on the current stream; result in out.  With caches,
-        the T streams grow by a token each."""
+        the T streams grow by a token each.  (A step that the caller captures is not counted against
+        their capacity when it is replayed: a token that finds no room is not stored, and device_errors()
+        says so, DEVERR_LENGTH.)"""
         if self.fused:
             return self.persistent().run(x, out)
         if self.caches is not None and not torch.cuda.is_current_stream_capturing():
@@ -385,9 +387,10 @@ class ClockStack:
         return out_host
 
     def device_errors(self) -> int:
-        n = sum(L.moe.device_errors() for L in self.layers)
-        if self.caches is not None:
-            n += sum(c.device_errors() for c in self.caches.layers)
+        """The device error words of all layers and caches in one, read and cleared."""
+        n = 0
+        for x in [L.moe for L in self.layers] + (self.caches.layers if self.caches is not None else []):
+            n |= x.device_errors()
         if self._persist is not None:
-            n += self._persist.device_errors()
+            n |= self._persist.device_errors()
         return n

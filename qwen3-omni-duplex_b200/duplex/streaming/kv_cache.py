@@ -23,8 +23,10 @@ follows new lengths, tables and values.  Calls run on the current stream of the 
 `kv_attend` and `kv_evict` take their workspace from torch's allocator, so calls on several streams
 do not share one.  Inference only, no autograd formula.  Errors in arguments raise RuntimeError;
 what the device arrays get wrong is reported in `err` (int32 [1]) if it is given: block ids out of
-range (_lib.DEVERR_BLOCK), values that are not finite (_lib.DEVERR_NONFINITE), and row offsets that
-fall (_lib.DEVERR_OFFSETS; the call then does nothing else, `out` and the caches stay as they were).
+range (_lib.DEVERR_BLOCK), values that are not finite (_lib.DEVERR_NONFINITE), a kv_len beyond what its
+row of the table holds (_lib.DEVERR_LENGTH; tokens past the table are left out: not stored, not seen,
+not kept), and row offsets that fall (_lib.DEVERR_OFFSETS; the call then does nothing else, `out` and
+the caches stay as they were).
 """
 
 from __future__ import annotations

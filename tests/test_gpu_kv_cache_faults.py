@@ -265,3 +265,83 @@ def test_evict_lengths_in_place(cuda):
         used = dst.flatten().long()
         assert torch.equal(s[m][used], t[used]), m
     assert torch.equal(w, want[-1])
+
+
+# ------------------------------------------------------------------ tables that are too narrow
+def dense(q, k, v, first, n, window, sinks, scale):
+    """Rows q [T, Hq, D] at positions first + t over tokens k, v [H, n, D], float64: out, lse."""
+    T, Hq, D = q.shape
+    G = Hq // k.shape[0]
+    p = first + torch.arange(T, device=q.device)[:, None]
+    j = torch.arange(n, device=q.device)
+    seen = (j <= p) & ((j > p - window) | (j < sinks) if window else True)
+    s = torch.einsum("thd,hnd->thn", q.double(), k.repeat_interleave(G, 0)) * scale
+    s = s.masked_fill(~seen[:, None], -math.inf)
+    l = torch.logsumexp(s, -1)
+    pr = torch.exp(s - torch.where(l == -math.inf, 0, l)[..., None]) * seen[:, None]
+    return torch.einsum("thn,hnd->thd", pr, v.repeat_interleave(G, 0)), l, pr
+
+
+@pytest.mark.parametrize("T,n,W,P,window,sinks", [(5, 35, 2, 16, 0, 0), (5, 35, 2, 16, 8, 2), (1, 40, 2, 16, 0, 0), (1, 40, 2, 16, 3, 1),
+                                                  (1500, 2100, 32, 64, 0, 0), (1500, 2100, 32, 64, 100, 5),
+                                                  (3, 2 ** 31 - 1, 2, 16, 0, 0), (3, 2 ** 31 - 1, 2, 16, 5, 3),
+                                                  (1500, 2 ** 31 - 1, 32, 64, 100, 5)])
+def test_table_too_narrow(cuda, T, n, W, P, window, sinks):
+    """A length beyond its table: reported; tokens past the table are not stored, and not seen by rows that keep
+    their positions; stored tokens and the other sequence stay as they are."""
+    from duplex import _lib
+    from duplex.streaming import kv_cache
+    cap, H, Hq, D = W * P, 2, 8, 64
+    s = make(cuda, 2, [T, 1], [cap, 30], Hq, H, D, P, "int8", torch.float16, seed=8)
+    s["kv_len"][0] = n
+    weights, err = torch.zeros(s["k"].shape[:3], device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    want = {m: s[m].double().cpu() for m in ("k", "v", "k_scale", "v_scale")}
+    k_new, v_new = (0.5 * torch.randn(T + 1, H, D, device=cuda).half() for _ in range(2))
+    fit = max(cap - (n - T), 0)                                  # rows that the table has room for
+    some = [*range(fit), T]
+    kv_ref.append(want, k_new[some].cpu(), v_new[some].cpu(), s["table"].cpu(), [min(n, cap), 30], [fit, 1], "int8")
+    kv_cache.kv_append(k_new, v_new, *cache_args(s), cu_q=s["cu"], err=err)
+    assert int(err) == _lib.DEVERR_LENGTH
+    for m in want:
+        assert torch.equal(s[m].double().cpu().nan_to_num(1000.0), want[m].nan_to_num(1000.0)), m
+    err.zero_()
+    out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, sinks=sinks, weights=weights,
+                                  return_lse=True, err=err)
+    assert int(err) == _lib.DEVERR_LENGTH
+    blocks = s["table"][0].long()
+    k, v = (torch.stack([kv_ref.values(s[m], s[m + "_scale"], blocks, h, cap) for h in range(H)]) for m in "kv")
+    ro, rl, pr = dense(s["q"][:T], k, v, n - T, cap, window, sinks, 1 / 8)
+    assert torch.equal(lse[:T] == -math.inf, rl == -math.inf)
+    some = rl > -math.inf
+    big = float(v.abs().max())
+    assert bool(((lse[:T] - rl).abs() < 1e-3)[some].all()) and bool(((out[:T] - ro).abs() < 4e-3 * big).all())
+    rw = pr.view(T, H, Hq // H, cap).sum((0, 2)).view(H, W, P).transpose(0, 1)
+    assert torch.allclose(weights[blocks].double(), rw, rtol=1e-3, atol=1e-3)
+    one = kv_cache.kv_attend(s["q"][T:], *cache_args(s)[:4], s["table"][1:], s["kv_len"][1:], window=window, sinks=sinks)
+    assert torch.allclose(out[T:].float(), one.float(), rtol=2.0 ** -9, atol=2.0 ** -9 * big)
+    new = kv_cache.kv_evict(*cache_args(s), weights, torch.full((2, 1), -1, dtype=torch.int32, device=cuda), keep=1, err=err)
+    assert int(err) == _lib.DEVERR_LENGTH | _lib.DEVERR_BLOCK and new.tolist() == [1, 1]
+
+
+def test_replays_past_the_capacity_are_reported(cuda):
+    """A step that the caller captured, replayed more often than the streams have room: nothing stored is lost."""
+    from duplex import _lib
+    from test_gpu_clock_attention import build
+    _, st = build(cuda, 2, tokens=16, fmt="int8")
+    x, out = torch.randn(2, 256, device=cuda).half(), torch.zeros(2, 256, device=cuda).half()
+    st.step_into(x, out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        st.step_into(x, out)
+    state = lambda: [t.clone() for c in st.caches.layers for t in (c.k, c.v, c.k_scale, c.v_scale)]  # noqa: E731
+    for _ in range(15):
+        x.copy_(torch.randn_like(x))
+        g.replay()
+    assert st.device_errors() == 0 and st.caches.kv_len.tolist() == [16, 16]
+    before = state()
+    for _ in range(2):
+        x.copy_(torch.randn_like(x))
+        g.replay()
+    assert st.device_errors() == _lib.DEVERR_LENGTH
+    assert all(torch.equal(a, b) for a, b in zip(before, state()))
