@@ -354,11 +354,16 @@ class ClockStack:
             self.step_into(self.x_in, self.out)      # warm: workspaces, attributes
         else:                                        # ... on caches of its own: a token that is taken
             c = self.caches                          # back could have raised a block's scale
-            self.caches = StreamCaches(len(self.layers), self.T, 1, c.heads, c.kv_heads, c.head_dim,
-                                       c.layers[0].block, c.layers[0].fmt, c.window, c.sinks,
-                                       c.evictable, self.device)
-            self._chain(self.x_in, self.out)
-            self.caches = c
+            warm = StreamCaches(len(self.layers), self.T, 1, c.heads, c.kv_heads, c.head_dim,
+                                c.layers[0].block, c.layers[0].fmt, c.window, c.sinks, c.evictable,
+                                self.device)
+            # tables as wide as the session's, which is what the kernels are chosen by
+            warm.table = warm.table.expand(-1, c.table.shape[1]).contiguous()
+            self.caches = warm
+            try:
+                self._chain(self.x_in, self.out)
+            finally:
+                self.caches = c
         torch.cuda.synchronize(self.device)
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))

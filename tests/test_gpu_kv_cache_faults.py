@@ -345,3 +345,41 @@ def test_replays_past_the_capacity_are_reported(cuda):
         g.replay()
     assert st.device_errors() == _lib.DEVERR_LENGTH
     assert all(torch.equal(a, b) for a, b in zip(before, state()))
+
+
+# ------------------------------------------------------------------ the clock stack's captured steps
+def test_capture_warms_the_sessions_kernels(cuda):
+    """The step before the capture takes the kernels that the session's tables ask for; a capture that fails leaves the session."""
+    from duplex.streaming.kv_cache import PackedKVCache
+    from test_gpu_clock_attention import build
+    _, st = build(cuda, 2, fmt="int8", tokens=13_000)
+    seen, real = [], PackedKVCache.attend
+
+    def attend(self, q, table, *a, **kw):
+        seen.append((tuple(table.shape), torch.cuda.is_current_stream_capturing()))
+        return real(self, q, table, *a, **kw)
+
+    x = torch.randn(2, 256, device=cuda).half()
+    out = torch.zeros_like(x)
+    PackedKVCache.attend = attend
+    try:
+        st.capture()
+    finally:
+        PackedKVCache.attend = real
+    assert {w for w, c in seen if c} == {w for w, c in seen if not c} == {(2, 813)}
+    caches = st.caches
+    st.x_in.copy_(x)
+    st.replay()
+    torch.cuda.synchronize()
+    got = st.out.clone()
+    _, other = build(cuda, 2, fmt="int8", tokens=13_000)
+    other.step_into(x, out)
+    assert torch.equal(got, out)
+
+    def fails(*a, **kw):
+        raise ValueError("no")
+
+    st._chain = fails
+    with pytest.raises(ValueError):
+        st.capture()
+    assert st.caches is caches and caches.kv_len.tolist() == [1, 1]
