@@ -553,6 +553,9 @@ int duplex_kv_append(const duplex_kv_cache* cache, const duplex_kv_batch* batch,
  */
 int duplex_kv_attend_workspace_bytes(const duplex_kv_cache* cache, const duplex_kv_batch* batch,
                                      int32_t heads, size_t* bytes);
+/* the kernels that such a call launches on the current device */
+int duplex_kv_attend_launches(const duplex_kv_cache* cache, const duplex_kv_batch* batch, int32_t heads,
+                              int32_t window, int32_t sinks, int32_t* launches);
 int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_batch* batch, const void* q,
                      int act_dtype, int32_t heads, int64_t q_row_stride, int64_t q_head_stride,
                      float softmax_scale, int32_t window, int32_t sinks, void* out, float* lse,

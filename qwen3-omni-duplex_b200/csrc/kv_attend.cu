@@ -888,10 +888,14 @@ static size_t part_bytes(const KvView& c, int nt) {
 // 8 sequences of 4096 14.5 / 22.8; 13 (416 CTAs) of 4096 24.8 / 22.2.
 constexpr double kClusterTokens = 12288;
 
-template <int D, int FMT, int NT>
-static int run_attend(const AttendParams& p, cudaStream_t st) {
+struct AttendGrid {
+  bool cluster;
+  int ctas;
+};
+
+template <int D, int NT>
+static int grid_of(const AttendParams& p, AttendGrid* g) {
   constexpr int ROWS = 8 * NT;
-  const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = front_smem<D, NT>() + plan;
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   // no more CTAs than units there can be
@@ -900,15 +904,27 @@ static int run_attend(const AttendParams& p, cudaStream_t st) {
                         : p.c.cu            ? rows / ROWS + p.c.batch
                                             : (rows / p.c.batch + ROWS - 1) / ROWS * p.c.batch;
   const int64_t units = tiles * p.c.heads * (((int64_t)p.c.width * p.c.block + kUnit - 1) / kUnit);
-  const int ctas = (int)std::min(std::min((int64_t)sms * attend_ctas<D, NT>(), (int64_t)kMaxCtas), units);
-  constexpr int most = front_smem<D, NT>() + 8 * (DUPLEX_KV_MAX_BATCH + 1);
   double seen = (double)p.c.width * p.c.block;
   if (p.window) seen = std::min(seen, (double)p.sinks + p.window + ROWS);
-  if (tiles * p.c.heads * kCluster <= (int64_t)sms * attend_ctas<D, NT>() * 2 / 3 && seen <= kClusterTokens) {
+  g->cluster = tiles * p.c.heads * kCluster <= (int64_t)sms * attend_ctas<D, NT>() * 2 / 3 && seen <= kClusterTokens;
+  g->ctas = (int)(g->cluster ? tiles * p.c.heads * kCluster
+                             : std::min(std::min((int64_t)sms * attend_ctas<D, NT>(), (int64_t)kMaxCtas), units));
+  return DUPLEX_OK;
+}
+
+template <int D, int FMT, int NT>
+static int run_attend(const AttendParams& p, cudaStream_t st) {
+  constexpr int ROWS = 8 * NT;
+  const size_t plan = sizeof(int64_t) * (p.c.batch + 1), smem = front_smem<D, NT>() + plan;
+  AttendGrid g;
+  if (int rc = grid_of<D, NT>(p, &g)) return rc;
+  const int ctas = g.ctas;
+  constexpr int most = front_smem<D, NT>() + 8 * (DUPLEX_KV_MAX_BATCH + 1);
+  if (g.cluster) {
     const auto kern = kv_attend_kernel<D, FMT, NT, true>;
     if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), most)) return rc;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * p.c.heads * kCluster));
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -962,6 +978,21 @@ static int run_all(const AttendParams& p, void* workspace, cudaStream_t st) {
   return record_cuda(cudaLaunchKernelEx(&cfg, kv_weights_kernel<D, FMT>, p));
 }
 
+template <int D>
+static int launches_of(const AttendParams& p, int32_t* n) {
+  *n = p.c.weights ? 1 : 0;
+  if (kv_prompt_takes(p)) {
+    int ctas = 0;
+    if (int rc = kv_prompt_ctas(p, &ctas)) return rc;
+    *n += ctas > 1 ? 3 : 2;
+    return DUPLEX_OK;
+  }
+  AttendGrid g;
+  if (int rc = nt_of(p.c, p.group) == 1 ? grid_of<D, 1>(p, &g) : grid_of<D, 2>(p, &g)) return rc;
+  *n += g.cluster || g.ctas < 2 ? 1 : 2;
+  return DUPLEX_OK;
+}
+
 // either kernel's (the choice depends on the window too); the rows' statistics lie behind it
 static size_t front_bytes(const KvView& c, int group) {
   const size_t few = part_bytes(c, nt_of(c, group));
@@ -985,6 +1016,19 @@ extern "C" int duplex_kv_attend_workspace_bytes(const duplex_kv_cache* cache, co
   if (!bytes || heads < 1 || heads % cache->kv_heads) return DUPLEX_ERR_ARG;
   *bytes = front_bytes(v, heads / cache->kv_heads) + (size_t)batch->n_rows * heads * (cache->weights ? 12 : 4);
   return DUPLEX_OK;
+}
+
+extern "C" int duplex_kv_attend_launches(const duplex_kv_cache* cache, const duplex_kv_batch* batch, int32_t heads,
+                                         int32_t window, int32_t sinks, int32_t* launches) {
+  AttendParams p{};
+  if (int rc = kv_check(cache, batch, &p.c)) return rc;
+  if (!launches || heads < 1 || heads % cache->kv_heads || window < 0 || sinks < 0) return DUPLEX_ERR_ARG;
+  *launches = 0;
+  if (batch->n_rows == 0) return DUPLEX_OK;
+  p.heads = heads;
+  p.set_group(heads / cache->kv_heads);
+  p.set_mask(window, sinks);
+  return cache->dim == 128 ? launches_of<128>(p, launches) : launches_of<64>(p, launches);
 }
 
 extern "C" int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_batch* batch, const void* q,
@@ -1011,9 +1055,7 @@ extern "C" int duplex_kv_attend(const duplex_kv_cache* cache, const duplex_kv_ba
   p.set_group(heads / cache->kv_heads);
   // a row tile's rows are counted in 32 bits
   if ((int64_t)batch->n_rows * p.group > 0x7FFFFFFFll - 256) return DUPLEX_ERR_UNSUPPORTED;
-  const int64_t cap = (int64_t)batch->width * cache->block;  // a window of all that can be cached is none
-  p.window = window >= cap ? 0 : window;
-  p.sinks = (int)std::min((int64_t)sinks, cap);
+  p.set_mask(window, sinks);
   p.scale_log2 = softmax_scale * kLog2e;
   p.out = out;
   p.part = static_cast<float*>(workspace);

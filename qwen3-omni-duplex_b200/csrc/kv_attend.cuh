@@ -35,6 +35,10 @@ struct AttendParams {
     while ((1ull << group_shift) < (uint64_t)g) ++group_shift;
     group_mul = (uint32_t)((((1ull << group_shift) - (uint64_t)g) << 32) / (uint64_t)g + 1);
   }
+  void set_mask(int w, int s) {  // a window of all that can be cached is none
+    window = w >= c.cap ? 0 : w;
+    sinks = s < c.cap ? s : c.cap;
+  }
 };
 
 DEVI float ex2(float x) {
@@ -85,6 +89,7 @@ int device_sms(int* sms);
 // kv_prompt.cu
 bool kv_prompt_takes(const AttendParams& p);
 size_t kv_prompt_workspace(const KvView& c, int group);
+int kv_prompt_ctas(const AttendParams& p, int* ctas);
 int kv_prompt_run(const AttendParams& p, void* workspace, cudaStream_t st);
 
 }  // namespace duplex

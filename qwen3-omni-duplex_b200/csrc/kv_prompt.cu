@@ -942,6 +942,14 @@ static int run(const PromptParams& pp, int ctas, cudaStream_t st) {
   return record_cuda(cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<D>, pp, ctas));
 }
 
+int kv_prompt_ctas(const AttendParams& a, int* ctas) {
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  const int64_t units = max_pairs(a.c, a.group) * a.c.heads * (((int64_t)a.c.width * a.c.block + kPTok - 1) / kPTok + kPOver);
+  *ctas = (int)std::min({(int64_t)sms, (int64_t)kPMaxCtas, units});
+  return DUPLEX_OK;
+}
+
 int kv_prompt_run(const AttendParams& a, void* workspace, cudaStream_t st) {
   PromptParams pp{};
   pp.a = a;
@@ -952,10 +960,8 @@ int kv_prompt_run(const AttendParams& a, void* workspace, cudaStream_t st) {
   pp.total = reinterpret_cast<int64_t*>(ws);
   pp.n_pairs = reinterpret_cast<int*>(ws + 8);
   pp.a.part = reinterpret_cast<float*>(ws + list + (ref_bytes(a.c) + 127) / 128 * 128);
-  int sms = 0;
-  if (int rc = device_sms(&sms)) return rc;
-  const int64_t units = max_pairs(a.c, a.group) * a.c.heads * (((int64_t)a.c.width * a.c.block + kPTok - 1) / kPTok + kPOver);
-  const int ctas = (int)std::min({(int64_t)sms, (int64_t)kPMaxCtas, units});
+  int ctas = 0;
+  if (int rc = kv_prompt_ctas(a, &ctas)) return rc;
   if (a.c.dim == 128)
     return a.c.format == DUPLEX_KV_E4M3 ? run<128, DUPLEX_KV_E4M3>(pp, ctas, st) : run<128, DUPLEX_KV_INT8>(pp, ctas, st);
   return a.c.format == DUPLEX_KV_E4M3 ? run<64, DUPLEX_KV_E4M3>(pp, ctas, st) : run<64, DUPLEX_KV_INT8>(pp, ctas, st);

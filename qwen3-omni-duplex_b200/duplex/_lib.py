@@ -133,6 +133,7 @@ _SIGNATURES = {
                           _c_ptr, _c_ptr], _c_int),
     "duplex_kv_attend_workspace_bytes": ([_c_ptr, _c_ptr, _c_i32, ctypes.POINTER(ctypes.c_size_t)],
                                          _c_int),
+    "duplex_kv_attend_launches": ([_c_ptr, _c_ptr, _c_i32, _c_i32, _c_i32, ctypes.POINTER(_c_i32)], _c_int),
     "duplex_kv_attend": ([_c_ptr, _c_ptr, _c_ptr, _c_int, _c_i32, _c_i64, _c_i64, _c_f32, _c_i32,
                           _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr, _c_ptr], _c_int),
     "duplex_kv_evict_workspace_bytes": ([_c_ptr, _c_ptr, _c_i32, ctypes.POINTER(ctypes.c_size_t)],

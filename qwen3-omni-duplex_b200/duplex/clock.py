@@ -31,6 +31,7 @@ graph replay, device -> host copy of the result.
 
 from __future__ import annotations
 
+import ctypes
 from types import SimpleNamespace as NS
 
 import torch
@@ -188,6 +189,20 @@ class StreamCaches:
         self.tokens += 1
 
 
+    def attend_launches(self) -> int:
+        """Kernels of a layer's attention."""
+        c, n = self.layers[0], ctypes.c_int32()
+        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        cache = _lib.KVCache(p(c.k), p(c.v), p(c.k_scale), p(c.v_scale), p(c.weights), *c.k.shape,
+                             _lib.KV_INT8 if c.fmt == "int8" else _lib.KV_E4M3)
+        batch = _lib.KVBatch(p(self.table), p(self.kv_len), None, self.table.shape[1], *[self.table.shape[0]] * 2)
+        with torch.cuda.device(self.table.device):
+            _lib.check(_lib.load().duplex_kv_attend_launches(ctypes.byref(cache), ctypes.byref(batch), self.heads,
+                                                             self.window, self.sinks, ctypes.byref(n)),
+                       "kv_attend_launches")
+        return n.value
+
+
 class ClockStack:
     """Thinker layers [0, n) of the clock path on the B200 kernels (batch T <= 8)."""
 
@@ -262,8 +277,9 @@ class ClockStack:
         return n
 
     def kernels_per_step(self) -> int:
-        if self.caches is not None:          # append, attend and its combine; the weights' pass
-            return (8 + self.caches.evictable) * len(self.layers)
+        """This package's kernels in a step."""
+        if self.caches is not None:          # and append, and what attention over such tables takes
+            return (6 + self.caches.attend_launches()) * len(self.layers)
         return 1 if self.fused else 5 * len(self.layers)
 
     def attach_cache(self, tokens, block=64, fmt="e4m3", window=0, sinks=0, evictable=False,

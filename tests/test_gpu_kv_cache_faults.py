@@ -383,3 +383,51 @@ def test_capture_warms_the_sessions_kernels(cuda):
     with pytest.raises(ValueError):
         st.capture()
     assert st.caches is caches and caches.kv_len.tolist() == [1, 1]
+
+
+def captured_kernels(call):
+    """The kernel launches of a call, counted in a graph of it."""
+    from cuda.bindings import driver
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        call()
+    raw = driver.CUgraph(g.raw_cuda_graph())
+    _, _, n = driver.cuGraphGetNodes(raw)
+    _, nodes, n = driver.cuGraphGetNodes(raw, n)
+    kernel = driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL
+    return sum(driver.cuGraphNodeGetType(v)[1] == kernel for v in nodes[:n])
+
+
+@pytest.mark.parametrize("tokens,kw", [(None, {}), (64, {}), (64, {"evictable": True}), (13_000, {}), (13_000, {"evictable": True}),
+                                       (13_000, {"window": 100})])
+def test_kernels_per_step(cuda, tokens, kw):
+    """kernels_per_step is the number of this package's kernels in a captured step (the lengths' increment is torch's)."""
+    from duplex.clock import ClockStack
+    from test_gpu_clock import small_layers
+    st = ClockStack.from_arrays(small_layers(2), top_k=4, device=cuda, T=2, fused=False)
+    if tokens:
+        st.attach_cache(tokens, block=16, head_dim=64, **kw)
+    x, out = torch.zeros(2, 256, device=cuda).half(), torch.zeros(2, 256, device=cuda).half()
+    st.step_into(x, out)
+    torch.cuda.synchronize()
+    assert st.kernels_per_step() == captured_kernels(lambda: st.step_into(x, out)) - bool(tokens)
+
+
+@pytest.mark.parametrize("B,T,width,window,launches", [(1, 1, 4, 0, 1), (40, 1, 4, 0, 2), (1, 1, 1000, 0, 2), (1, 1, 1000, 64, 1),
+                                                       (1, 900, 100, 0, 3), (2, 900, 100, 200, 3)])
+@pytest.mark.parametrize("track", [False, True])
+def test_attend_launches(cuda, B, T, width, window, launches, track):
+    """duplex_kv_attend_launches counts what a call launches: clusters, pieces and their join, the prompt kernels, weights."""
+    from duplex import _lib
+    from duplex.streaming.kv_cache import PackedKVCache
+    c = PackedKVCache(8, 1, 128, 16, "int8", track_weights=track, device=cuda)
+    table, kv_len = torch.zeros(B, width, dtype=torch.int32, device=cuda), torch.full((B,), 1, dtype=torch.int32, device=cuda)
+    q = torch.randn(B * T, 8, 128, device=cuda).half()
+    call = lambda: c.attend(q, table, kv_len, window=window)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    n, p = ctypes.c_int32(), lambda t: t.data_ptr()
+    cache = _lib.KVCache(p(c.k), p(c.v), p(c.k_scale), p(c.v_scale), p(c.weights) if track else None, *c.k.shape, _lib.KV_INT8)
+    batch = _lib.KVBatch(p(table), p(kv_len), None, width, B, B * T)
+    assert _lib.load().duplex_kv_attend_launches(ctypes.byref(cache), ctypes.byref(batch), 8, window, 0, ctypes.byref(n)) == 0
+    assert n.value == launches + track == captured_kernels(call)

@@ -37,3 +37,18 @@ def test_falling_offsets_would_not():
     """Which is why a call whose offsets fall does nothing."""
     n_rows = 8192
     assert pairs([0, n_rows, 0, n_rows], n_rows, 8) == 512 > room(3, n_rows, 8) + 1
+
+
+def test_attend_launches_refuses():
+    import ctypes
+
+    from duplex import _build, _lib
+    from test_kv_cache import batch, cache
+    _build.build()
+    lib, n = _lib.load(), ctypes.c_int32(7)
+    call = lambda c, b, heads=8, window=0, sinks=0, to=ctypes.byref(n): lib.duplex_kv_attend_launches(  # noqa: E731
+        ctypes.byref(c), ctypes.byref(b), heads, window, sinks, to)
+    assert call(cache(k=None), batch()) == 1 and call(cache(dim=96), batch()) == 6 and call(cache(), batch(width=0)) == 1
+    assert call(cache(), batch(), heads=7) == 1 and call(cache(), batch(), window=-1) == 1
+    assert call(cache(), batch(), sinks=-1) == 1 and call(cache(), batch(), to=None) == 1
+    assert call(cache(), batch(n_rows=0)) == 0 and n.value == 0
