@@ -51,12 +51,10 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
   const int P = c.block, D = c.dim, h = blockIdx.y, tid = threadIdx.x;
   const bool val = blockIdx.z != 0;
   const int64_t w = blockIdx.x;
-  // Every CTA finds out whether the offsets fall before it stores: loads that are under way here, looked at with
-  // the values.  This CTA reports it, whether it has tokens to store or not.
+  // Every CTA finds out whether the offsets fall before it stores: a thread has a pair of them, on their way from here,
+  // and what they say goes with the values' maximum.
   int2 cu = make_int2(0, 0);
   if (c.cu && tid < c.batch) cu = make_int2(c.cu[tid], c.cu[tid + 1]);
-  if (c.cu && w == 0 && h == 0 && !val && __syncthreads_or(offsets_fall(c)) && tid == 0)
-    set_error(p.err, DUPLEX_DEVERR_OFFSETS);
   // the last b whose first item is <= w, 32 sequences a look
   int lo = 0, left = c.batch;
   const int lane = tid & 31;
@@ -67,17 +65,19 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
     left = min(step, lo + left - (lo + i * step));
     lo += i * step;
   }
-  bool fall = cu.y < cu.x;
   const int b = lo;
   const KvSeq s = kv_seq(c, b);
-  if (s.rows == 0) return;
+  auto idle = [&] {
+    if (offsets_fall(c)) set_error(p.err, DUPLEX_DEVERR_OFFSETS);
+  };
+  if (s.rows == 0) return idle();
   const int first = s.first;  // slot of the sequence's first new token (< 0: no room for it)
   const int64_t item = w - (s.row0 / P + 2ll * b);
-  if (item < 0) return;  // rows before the first sequence's
+  if (item < 0) return idle();  // rows before the first sequence's
   const int64_t col = max(first, 0) / P + item;
   if (col * P >= s.n) {  // no more tokens, or no more table (which some CTA's block is past if kv_len is)
     if (tid == 0 && too_long(c, s)) set_error(p.err, DUPLEX_DEVERR_LENGTH);
-    return;
+    return idle();
   }
   const int id = kv_block_at(c, b, (int)col, tid == 0 ? p.err : nullptr);
   if (id < 0) return;
@@ -112,7 +112,10 @@ __global__ void __launch_bounds__(kThreads, kRounds == 1 ? 6 : kRounds == 2 ? 4 
       amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
   }
+  asm volatile("" : "+r"(cu.x), "+r"(cu.y));  // looked at no earlier: 13,000 tokens 13.9 us if they are, 13.6 here
+  bool fall = cu.y < cu.x;
   for (int i = tid + kThreads; c.cu && i < c.batch; i += kThreads) fall |= offset_falls(c, i);
+  if (fall) set_error(p.err, DUPLEX_DEVERR_OFFSETS);
   amax = block_max(fall ? INFINITY : amax, red);  // (the values are finite)
   if (amax == INFINITY) return;
   if (bad) set_error(p.err, DUPLEX_DEVERR_NONFINITE);

@@ -431,3 +431,18 @@ def test_attend_launches(cuda, B, T, width, window, launches, track):
     batch = _lib.KVBatch(p(table), p(kv_len), None, width, B, B * T)
     assert _lib.load().duplex_kv_attend_launches(ctypes.byref(cache), ctypes.byref(batch), 8, window, 0, ctypes.byref(n)) == 0
     assert n.value == launches + track == captured_kernels(call)
+
+
+def test_offsets_that_fall_are_reported_whatever_else(cuda):
+    """Where no sequence has a token to store, and where they fall behind the 256th sequence."""
+    from duplex import _lib
+    from duplex.streaming import kv_cache
+    for B, cu in ((2, [0, 3, 1]), (600, [0] * 400 + [2] + [1] * 200)):
+        s = make(cuda, B, [3] + [0] * (B - 1), [16] * B, 2, 1, 64, 16, "int8", torch.float16)
+        fall = torch.tensor(cu, dtype=torch.int32, device=cuda)
+        before = s["k"].clone()
+        for n in (0, 16):
+            s["kv_len"].fill_(n)
+            err = torch.zeros(1, dtype=torch.int32, device=cuda)
+            kv_cache.kv_append(s["q"][:, :1], s["q"][:, 1:2], *cache_args(s), cu_q=fall, err=err)
+            assert int(err) == _lib.DEVERR_OFFSETS and torch.equal(s["k"], before)
