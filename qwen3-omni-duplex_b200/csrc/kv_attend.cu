@@ -13,9 +13,10 @@
 // fill ahead.  The codes are converted to fp16 in registers, exactly.  The products take a sixth of the
 // tensor pipe; what competes with the copies is the issue of the rest (conversions, softmax, addresses),
 // hence 32 tokens for one set of addresses, one vote and one rescale.
-// One B200, 32 query heads on 4, dim 128, 64 sequences of 12,288 tokens (805 MB): 143 us, 5.6 TB/s, 86 %
-// of a plain copy's rate.  With 16 tokens a step 165 us; with the next 16 tokens in registers instead of
-// a ring 182 us.  One sequence of 2000: 10.5 us, all of it latency (list, copies, two steps, join).
+// One B200, captured calls one after another, 32 query heads on 4, dim 128, 64 sequences of 12,288 tokens
+// (805 MB): 136 us, 5.9 TB/s, 90 % of a plain copy's rate.  (Before its last steps: 143 us with 32 tokens a
+// step, 165 with 16, 182 with the next 16 tokens in registers instead of a ring.)  One sequence of 2000: 8.4 us,
+// all of it latency (list, copies, two steps, join).
 //
 // The work of a launch is one list of 128-token units over (sequence, KV head, row tile); every CTA
 // takes an equal, contiguous piece of it, whatever the lengths, and reads the lengths itself (a
@@ -119,9 +120,7 @@ DEVI uint32_t movmatrix_trans(uint32_t a) {
   return d;
 }
 
-// fp16 query fragments of 8 rows: row r's 16 dims at 64 cc + 16 t, scaled by a power of two that
-// brings the row's largest into [2^14, 2^15): bf16's 8 bits fit fp16's 11, and only values below
-// 2^-28 of the row's largest lose bits.  Returns the factor that undoes it.
+// Query rows of 8: row r's 16 dims at 64 cc + 16 t, as they come.
 template <int D>
 DEVI void load_raw(const AttendParams& p, int64_t row, int head, int t, bool live, uint4 (&raw)[D / 64][2]) {
   const uint8_t* src = static_cast<const uint8_t*>(p.q) + 2 * (row * p.q_row + head * p.q_head);
@@ -132,6 +131,9 @@ DEVI void load_raw(const AttendParams& p, int64_t row, int head, int t, bool liv
       raw[cc][j] = live ? __ldg(reinterpret_cast<const uint4*>(src + 2 * (64 * cc + 16 * t + 8 * j))) : make_uint4(0, 0, 0, 0);
 }
 
+// ... and as fp16 fragments, scaled by a power of two that brings the row's largest into [2^14, 2^15): bf16's
+// 8 bits fit fp16's 11, and only values below 2^-28 of the row's largest lose bits.  Returns the factor that
+// undoes it.
 template <int D>
 DEVI float make_q(const AttendParams& p, const uint4 (&raw)[D / 64][2], uint2 (&qf)[D / 16]) {
   float amax = 0.f;
@@ -884,8 +886,9 @@ static size_t part_bytes(const KvView& c, int nt) {
 
 // Clusters up to two thirds of what is resident at once (beyond, clusters of 8 wait for one another's
 // places) and up to here in tokens (8 CTAs a row tile are too few then).  With / without, 32 query heads on
-// 4, dim 128, us: 1 sequence of 2000 tokens 10.5 / 14.9, of 8192 16.8 / 22.9, of 16,384 26.9 / 25.0;
-// 8 sequences of 4096 14.5 / 22.8; 13 (416 CTAs) of 4096 24.8 / 22.2.
+// 4, dim 128, us: 1 sequence of 2000 tokens 8.4 / 12.3, of 8192 15.9 / 20.4, of 16,384 25.2 / 22.7;
+// 8 sequences of 4096 14.0 / 21.2; 13 (416 CTAs) of 4096 26.6 / 22.5.  Tokens are the table's, which the host
+// knows, not the lengths: a short sequence in a wide table goes without.
 constexpr double kClusterTokens = 12288;
 
 struct AttendGrid {

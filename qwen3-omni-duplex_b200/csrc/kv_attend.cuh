@@ -10,6 +10,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // p = exp2(s - m + kShift) is what fp16 holds: the reference m may be 2^kSlack behind the true
 // maximum (so it rarely moves), p stays below 2^15, and a p of 2^-21 of the reference is still normal.
+// That p (times its block's scale over the largest) is rounded to fp16, half a step 2^-11, because the second
+// product's operands have 16 bits; l sums it unrounded, in fp32.  The tokens' errors are independent, so a row's
+// is about the result's own rounding for fp16 (2.4e-4 from 64 bits where 32-bit probabilities give 2.1e-4), and
+// disappears in bf16's.
 constexpr float kShift = 7.f, kSlack = 8.f;
 // A reference beyond this has steps that count: s - m is then taken of the rounded s, so that the largest is 0.
 constexpr float kHuge = 1048576.f;
@@ -41,6 +45,7 @@ struct AttendParams {
   }
 };
 
+// off by at most 2^-22 of it, a thousandth of the rounding to fp16 that follows; numbers below 2^-126 are 0
 DEVI float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

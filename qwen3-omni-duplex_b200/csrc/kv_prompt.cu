@@ -14,17 +14,17 @@
 //                    codes themselves and the scales are factors in the softmax, in fp32: of the scores for
 //                    keys, of the probabilities for values (over the largest scale that the row has seen,
 //                    with which its O is rescaled like with the maximum).  So a row's result hangs on what
-//                    the row sees, whatever the blocks that it does not.  Such a prompt of 8192: 1.6 times
+//                    the row sees, whatever the blocks that it does not.  Such a prompt of 8192: 1.7 times
 //                    the time
 //   warp 16          issues the products: S = Q K^T (both shared memory), O += P V
 //
 // The running maximum is a reference that may lag by 2^kSlack, so O is rescaled rarely.  The products of a
 // tile's first 64 tokens start while the softmax is at the second 64.
 //
-// One B200, 32 query heads on 4, dim 128: a prompt of 8192 tokens takes 617 us, 890 TFLOP/s, 53 % of a
-// plain bf16 product's rate; 4200 cycles a step of 256 rows and 128 tokens, of which products are 2048.  A
-// step is a chain: softmax of a tile (2500), its products (1500); the other tile's chain fills in, but two
-// tiles are what 512 columns hold.  Skipping the exponentials, or the search for the maximum, or the
+// One B200, 32 query heads on 4, dim 128: a prompt of 8192 tokens takes 649 us (captured calls one
+// after another), 847 TFLOP/s, 51 % of a plain bf16 product's rate; 4200 cycles a step of 256 rows and 128
+// tokens, of which products are 2048.  A step is a chain: softmax of a tile (2500), its products (1500); the
+// other tile's chain fills in, but two tiles are what 512 columns hold.  Skipping the exponentials, or the search for the maximum, or the
 // conversion each gains 3 to 8 %.  An item costs 4 steps more: query rows in, results out, masks.
 //
 // Work is one list of (row tile, head) items, 128 tokens a unit, cut into equal contiguous pieces, one
@@ -889,8 +889,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
 
 // Which kernel is faster, by the time each takes as measured on one B200 (128 dims, 32 query heads on 4;
 // its own / kv_attend_kernel's us):
-//   7 sequences of 3000 tokens, 4 rows each 42 / 31, 8 rows 43 / 40, 16 rows 39 / 58, 32 rows 47 / 97
-//   64 of 4096: 4 rows 187 / 139, 8 rows 188 / 254      1 of 8192: 4 rows 46 / 23, 32 rows 50 / 48
+//   7 sequences of 3000 tokens, 4 rows each 36 / 27, 8 rows 36 / 37, 16 rows 37 / 55, 32 rows 45 / 95
+//   64 of 4096: 4 rows 174 / 139, 8 rows 174 / 258      1 of 8192: 4 rows 39 / 20, 32 rows 47 / 44 (the
+//   one of these where the rule takes the slower)
 // A 128-token step of 16 rows, two CTAs an SM, takes there as long as one of 256 rows takes here, 2.3 us;
 // the rest is what a call costs before and after.  Lengths are the block table's, which the host knows.
 bool kv_prompt_takes(const AttendParams& p) {

@@ -78,7 +78,8 @@ def kv_attend(q, k, v, k_scale, v_scale, block_table, kv_len, *, cu_q=None, wind
     kept ones.  Blocks that no row sees are not read, and their table entries may be anything; slots
     that no row sees may hold any code.  (An e4m3 NaN in a token that one row of a call sees may reach
     rows that do not: 0 * NaN.  kv_append stores none.)  A row that sees nothing (kv_len smaller than
-    its sequence's rows) gets 0 and -inf.  Rows behind the last sequence's are left as they were.
+    its sequence's rows) gets 0 and -inf.  Rows behind the last sequence's are left as they were
+    (without `out` and `lse`: they may hold anything).
 
     Scales need not be powers of two, nor near one another; prompts are slower where a sequence and head
     has others than powers of two within 2^14 of its largest.  Beside its relative error a row's out may
