@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       }
     }
     float O[NT][D / 16][4], m[NT][2], l[NT][2], vref = pow2f(-126), rv = pow2f(126);  // rv = 1 / vref
-    float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim, 15 + d
+    float ad[NT][2], lim[NT][2];  // x = s + ad is what exp2 takes; the reference moves if an x is above lim
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
@@ -353,13 +353,13 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
     }
 
     // O is in units of the largest value scale so far, vref.  Where the tile's rows are of several tokens, one may not see
-    // the block that has it.  If its own largest is far below, by 2^d, the row's probabilities are held 2^d larger (m
-    // lower by d; l and O with it), so that what fp16 holds, p times scale / vref, is as large as if the row were
-    // alone.  That costs a tenth of the time: the steps take it (APART) from the first one on that not all rows see and
-    // whose scale is more than 4 times those before, which all rows have seen, or, without a window, more than 4 times
-    // its other 16 tokens' (who sees the second 16 sees the first).  False: this is that step.
+    // the block that has it, and would lose what lies far below it.  So O has a unit for each row, 1 / ru, the largest
+    // scale that the row has seen, in the steps APART: from the first one on that not all rows see and whose scale is
+    // more than 4 times those before, which all rows have seen, or, without a window, more than 4 times its other 16
+    // tokens' (who sees the second 16 sees the first).  False: this is that step.  (Everywhere it would cost a twentieth
+    // of the time, in registers.)
     const bool several = first_pos != last_pos;
-    auto step = [&](auto apart, const uint8_t* st, int tok) -> bool {
+    auto step = [&](auto apart, float (&ru)[NT][2], const uint8_t* st, int tok) -> bool {
       constexpr bool APART = decltype(apart)::value;
       const float4 sc = *reinterpret_cast<const float4*>(st + 64 * D);
       const float ks[2] = {sc.x, sc.z}, vs[2] = {sc.y, sc.w};
@@ -404,9 +404,8 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
         }
       const float vmax = fmaxf(vs[0], vs[1]);
       if (__any_sync(~0u, grow || vmax > vref)) {
-        const float vold = vref;
         float vf = 1.f;
-        if (vmax > vref) {
+        if (!APART && vmax > vref) {
           rv = 1.f / vmax;
           vf = vref * rv;
           vref = vmax;
@@ -420,26 +419,23 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
             y = fmaxf(y, __shfl_xor_sync(~0u, y, 4));
             y = fmaxf(y, __shfl_xor_sync(~0u, y, 8));
             y = fmaxf(y, __shfl_xor_sync(~0u, y, 16));
-            float d0 = 0.f, d = 0.f;
+            const float top = fmaxf(m[nt][j], y - ad[nt][j]);
+            a[j] = top == m[nt][j] ? 1.f : ex2(m[nt][j] - top);
             if constexpr (APART) {
               float v = fmaxf(fmaxf(S[0][nt][j], S[0][nt][j + 2]) > -INFINITY ? vs[0] : 0.f,
                               fmaxf(S[1][nt][j], S[1][nt][j + 2]) > -INFINITY ? vs[1] : 0.f);
               v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
               v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
               v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-              if (lim[nt][j] != -INFINITY) {  // the row has seen something before
-                d0 = lim[nt][j] - (kShift + kSlack);
-                v = fmaxf(v, vold * ex2(-d0));
-              }
-              if (v > 0.f && vref > v) d = (float)min((int)(__float_as_uint(vref / v) >> 23) - 127, 80);  // (l has room)
+              const float up = v * ru[nt][j];
+              vf = up > 1.f ? 1.f / up : 1.f;
+              if (up > 1.f) ru[nt][j] = 1.f / v;
             }
-            const float top = fmaxf(m[nt][j] + d0, y - ad[nt][j]) - d;
-            a[j] = top == m[nt][j] ? 1.f : ex2(m[nt][j] - top);
-            // by what the step's x move: the largest to kShift + d, whatever the rounding of a large reference
-            const float by = y - ad[nt][j] > m[nt][j] + d0 ? kShift + d - y : d - d0;
+            // by what the step's x move: the largest to kShift, whatever the rounding of a large reference
+            const float by = y - ad[nt][j] > m[nt][j] ? kShift - y : 0.f;
             m[nt][j] = top;
             ad[nt][j] = kShift - (top == -INFINITY ? 0.f : top);
-            const float most = top == -INFINITY ? -INFINITY : kShift + kSlack + d;
+            const float most = top == -INFINITY ? -INFINITY : kShift + kSlack;
             lim[nt][j] = most;
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -461,7 +457,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           }
         }
       }
-      const float vf[2] = {vs[0] * rv, vs[1] * rv};
+      const float vf[2] = {APART ? vs[0] : vs[0] * rv, APART ? vs[1] : vs[1] * rv};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         uint32_t pb[NT][2];
@@ -472,7 +468,7 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
           for (int j = 0; j < 4; ++j) {
             y[j] = ex2(S[x][nt][j]);
             l[nt][j & 1] += y[j];
-            y[j] *= vf[x];
+            y[j] *= APART ? fminf(vf[x] * ru[nt][j & 1], 1.f) : vf[x];  // (beyond 1: y is 0)
           }
           pb[nt][0] = movmatrix_trans(f2h(y[0], y[1]));
           pb[nt][1] = movmatrix_trans(f2h(y[2], y[3]));
@@ -526,15 +522,29 @@ __global__ void __launch_bounds__(kWarps * 32, attend_ctas<D, NT>()) kv_attend_k
       id = ids_of(i + ST);
     };
     int i = i0;
+    float ru[NT][2];
 #pragma unroll 1
     for (; i < i1; ++i) {
       arrive(i);
-      if (!step(std::false_type{}, ring + (i % ST) * kStage, base_of(i))) break;
+      if (!step(std::false_type{}, ru, ring + (i % ST) * kStage, base_of(i))) break;
     }
+    if (i < i1) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ru[nt][j] = lim[nt][j] == -INFINITY ? pow2f(126) : rv;  // (a row that has seen nothing)
 #pragma unroll 1
-    while (i < i1) {
-      step(std::true_type{}, ring + (i % ST) * kStage, base_of(i));
-      if (++i < i1) arrive(i);
+      while (i < i1) {
+        step(std::true_type{}, ru, ring + (i % ST) * kStage, base_of(i));
+        if (++i < i1) arrive(i);
+      }
+      vref = 1.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) O[nt][x][j] *= 1.f / ru[nt][j & 1];
     }
     cp_async_wait<0>();
     __syncthreads();  // the ring becomes the place where the warps meet

@@ -446,3 +446,16 @@ def test_offsets_that_fall_are_reported_whatever_else(cuda):
             err = torch.zeros(1, dtype=torch.int32, device=cuda)
             kv_cache.kv_append(s["q"][:, :1], s["q"][:, 1:2], *cache_args(s), cu_q=fall, err=err)
             assert int(err) == _lib.DEVERR_OFFSETS and torch.equal(s["k"], before)
+
+
+def test_lse_beside_large_values(cuda):
+    """What the values' scales ask of a row's outputs leaves its sum of probabilities alone: lse keeps its last bits."""
+    from duplex.streaming import kv_cache
+    rows, lens = [300, 777, 777], [350, 777, 778]
+    s = make(cuda, 3, rows, lens, 2, 2, 64, 16, "int8", torch.bfloat16, seed=41)
+    g = torch.Generator(device=cuda).manual_seed(41)
+    s["v_scale"] *= torch.exp2(torch.randint(-60, 1, s["v_scale"].shape, generator=g, device=cuda).float())
+    for window, sinks in ((1, 0), (1, 5), (2, 1)):                     # a tile's rows see different blocks, and few tokens
+        out, lse = kv_cache.kv_attend(s["q"], *cache_args(s), cu_q=s["cu"], window=window, sinks=sinks, softmax_scale=0.00125,
+                                      return_lse=True)
+        check_rows(s, rows, lens, "int8", window, sinks, out, lse, 0.00125)
