@@ -14,8 +14,8 @@
 // tensor pipe; what competes with the copies is the issue of the rest (conversions, softmax, addresses),
 // hence 32 tokens for one set of addresses, one vote and one rescale.
 // One B200, captured calls one after another, 32 query heads on 4, dim 128, 64 sequences of 12,288 tokens
-// (805 MB): 136 us, 5.9 TB/s, 90 % of a plain copy's rate.  (Before its last steps: 143 us with 32 tokens a
-// step, 165 with 16, 182 with the next 16 tokens in registers instead of a ring.)  One sequence of 2000: 8.4 us,
+// (805 MB): 135 us, 5.9 TB/s, 91 % of a plain copy's rate.  (Before its last steps: 143 us with 32 tokens a
+// step, 165 with 16, 182 with the next 16 tokens in registers instead of a ring.)  One sequence of 2000: 8.2 us,
 // all of it latency (list, copies, two steps, join).
 //
 // The work of a launch is one list of 128-token units over (sequence, KV head, row tile); every CTA
@@ -896,8 +896,8 @@ static size_t part_bytes(const KvView& c, int nt) {
 
 // Clusters up to two thirds of what is resident at once (beyond, clusters of 8 wait for one another's
 // places) and up to here in tokens (8 CTAs a row tile are too few then).  With / without, 32 query heads on
-// 4, dim 128, us: 1 sequence of 2000 tokens 8.4 / 12.3, of 8192 15.9 / 20.4, of 16,384 25.2 / 22.7;
-// 8 sequences of 4096 14.0 / 21.2; 13 (416 CTAs) of 4096 26.6 / 22.5.  Tokens are the table's, which the host
+// 4, dim 128, us: 1 sequence of 2000 tokens 8.2 / 12.2, of 8192 15.2 / 19.4, of 16,384 24.4 / 22.8;
+// 8 sequences of 4096 13.8 / 21.3; 13 (416 CTAs) of 4096 26.1 / 22.6.  Tokens are the table's, which the host
 // knows, not the lengths: a short sequence in a wide table goes without.
 constexpr double kClusterTokens = 12288;
 

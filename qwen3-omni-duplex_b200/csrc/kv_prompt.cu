@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_prompt_join_kernel(PromptPara
 // Which kernel is faster, by the time each takes as measured on one B200 (128 dims, 32 query heads on 4;
 // its own / kv_attend_kernel's us):
 //   7 sequences of 3000 tokens, 4 rows each 36 / 27, 8 rows 36 / 37, 16 rows 37 / 55, 32 rows 45 / 95
-//   64 of 4096: 4 rows 174 / 139, 8 rows 174 / 258      1 of 8192: 4 rows 39 / 20, 32 rows 47 / 44 (the
+//   64 of 4096: 4 rows 174 / 138, 8 rows 174 / 257      1 of 8192: 4 rows 39 / 20, 32 rows 47 / 44 (the
 //   one of these where the rule takes the slower)
 // A 128-token step of 16 rows, two CTAs an SM, takes there as long as one of 256 rows takes here, 2.3 us;
 // the rest is what a call costs before and after.  Lengths are the block table's, which the host knows.
